@@ -191,6 +191,85 @@ QM_API int32_t qm_matvec_selected(qm_ctx *ctx, qm_weight w, int32_t experts, uin
 QM_API int32_t qm_matmul_bf16(qm_ctx *ctx, qm_weight w, uint64_t a_dev, int32_t m, int64_t lda, uint64_t c_dev,
                               int64_t ldc);
 
+/* ---- Low-rank adapters beside a stored projection ----------------------------------------------
+ * No counterpart in the reference. A qm_lora holds up to `adapters` (<= 256) pairs A [rank][cols], B [rows][rank] with a
+ * scale, of ranks up to max_rank (<= 128), for one projection of `rows` x `cols` weights that all requests share
+ * (cols a multiple of 32, <= 32768; rows <= 2^22); a batch names for each token the adapter of its request:
+ *   y[t] = base[t] + scale_a * B_a (A_a f(x[t])),   a = ids[t] (int32, on the device; ids_dev = 0: slot 0 for all).
+ * A token whose id is outside [0, adapters) or names an empty slot keeps base[t]. base_dev = 0 stands for zeros; it may be
+ * y_dev itself with ldb = ldy, any other overlap of y with an input is refused. All sums are float32; adapters are held in
+ * bf16. max_tokens (<= 2^20) bounds the tokens of one bf16 call and sizes the handle's workspace: calls with bf16
+ * activations and their graphs that share a handle must be ordered, on one stream or with events.
+ * Capture into a graph is allowed; everything is asynchronous on the context's stream. Device pointers.
+ *
+ * qm_lora_set: fills a slot from device memory, A [rank][cols] and B [rows][rank] row by row, `type` a GGUF tensor type
+ *   (QM_TYPE_F32, QM_TYPE_F16, QM_TYPE_BF16; rounded to bf16). rank 0 empties the slot. Ordered with the products on the
+ *   stream, so a training step may set its adapters anew; the two arrays are free again once the stream is past the call.
+ * qm_lora_matvec: 1..8 float32 rows, x, x2 and flags as for qm_matvec (the same input transforms f); for single tokens.
+ * qm_lora_matmul_bf16: any number of tokens up to max_tokens, x bf16 [tokens][ldx] (16-byte aligned, ldx a multiple
+ *   of 8), f the identity.
+ * qm_lora_backward: gradients of qm_lora_matmul_bf16. dy bf16 [tokens][lddy] (16-byte aligned, lddy a multiple of 8):
+ *   dx[t] = base[t] + scale_a A_a^T (B_a^T dy[t])   float32 [tokens][lddx] (base: the frozen weights' share, as above)
+ *   da[a] = scale_a sum_t (B_a^T dy[t]) x[t]^T      float32 [adapters][max_rank][cols]
+ *   db[a] = scale_a sum_t dy[t] (A_a x[t])^T        float32 [adapters][rows][max_rank]
+ *   over the tokens of each adapter, added in a fixed order (the same bits in every run); ranks past a slot's own and
+ *   adapters without a token get zeros. dx_dev, da_dev or db_dev may be 0: not wanted.
+ * qm_matvec_lora, qm_matmul_bf16_lora: qm_matvec / qm_matmul_bf16 with the stored matrix w, then the adapters onto its
+ *   result; w must have the handle's rows and cols. */
+#define QM_TYPE_F32 0
+#define QM_TYPE_F16 1
+#define QM_TYPE_BF16 30
+typedef struct qm_lora qm_lora;
+QM_API int32_t qm_lora_create(qm_ctx *ctx, int64_t rows, int64_t cols, int32_t adapters, int32_t max_rank, int32_t max_tokens,
+                              qm_lora **out);
+QM_API int32_t qm_lora_destroy(qm_ctx *ctx, qm_lora *lora);
+QM_API int32_t qm_lora_set(qm_ctx *ctx, qm_lora *lora, int32_t slot, int32_t rank, float scale, uint64_t a_dev, uint64_t b_dev,
+                           int32_t type);
+QM_API int32_t qm_lora_matvec(qm_ctx *ctx, qm_lora *lora, uint64_t x_dev, uint64_t x2_dev, int32_t m, int64_t ldx,
+                              uint64_t ids_dev, uint64_t base_dev, int64_t ldb, uint64_t y_dev, int64_t ldy, uint32_t flags);
+QM_API int32_t qm_lora_matmul_bf16(qm_ctx *ctx, qm_lora *lora, uint64_t x_bf16_dev, int32_t tokens, int64_t ldx,
+                                   uint64_t ids_dev, uint64_t base_dev, int64_t ldb, uint64_t y_dev, int64_t ldy);
+QM_API int32_t qm_lora_backward(qm_ctx *ctx, qm_lora *lora, uint64_t x_bf16_dev, int64_t ldx, uint64_t dy_bf16_dev, int64_t lddy,
+                                int32_t tokens, uint64_t ids_dev, uint64_t base_dev, int64_t ldb, uint64_t dx_dev, int64_t lddx,
+                                uint64_t da_dev, uint64_t db_dev);
+QM_API int32_t qm_matvec_lora(qm_ctx *ctx, qm_weight w, qm_lora *lora, uint64_t x_dev, uint64_t x2_dev, int32_t m, int64_t ldx,
+                              uint64_t ids_dev, uint64_t y_dev, int64_t ldy, uint32_t flags);
+QM_API int32_t qm_matmul_bf16_lora(qm_ctx *ctx, qm_weight w, qm_lora *lora, uint64_t a_dev, int32_t m, int64_t lda,
+                                   uint64_t ids_dev, uint64_t c_dev, int64_t ldc);
+
+/* ---- Norm and rotation of query and key heads --------------------------------------------------
+ * What follows a q|k|v product, in one pass: each head of head_dim elements is RMS normalised and multiplied with a gain,
+ * and its first rot_dim elements are turned pairwise by the token's position (the other elements stay). No counterpart in
+ * the reference.
+ * qm_rope_create: angle_i = position * theta^(-2i/rot_dim) / factors[i] (factors: rot_dim/2 positive floats on the host, or
+ *   NULL: ones), taken modulo a turn in float64, so far positions keep their fraction. Pairs are (i, i + rot_dim/2), with
+ *   QM_ROPE_INTERLEAVED (2i, 2i+1). head_dim even, <= 512; rot_dim even, 0..head_dim.
+ * qm_qk_norm_rope: x float32 [tokens][ldx], q_heads query heads, then k_heads key heads, side by side (either may be 0; a v
+ *   part behind them is not touched); gains float32 [head_dim] or 0 (ones); pos int32 [tokens], any value;
+ *   q_out [tokens][ldq], k_out [tokens][ldk]: float32, or bf16 with QM_QK_BF16. QM_QK_NO_NORM: rotation only (gains and eps
+ *   are ignored). A float32 result may lie on the heads it comes from (q_out = x_dev, k_out = the first key head, the same
+ *   row pitch); other overlaps are refused.
+ * qm_qk_norm_rope_backward: dq, dk the gradients of the results (float32, bf16 with QM_QK_BF16), x and the rest as in the
+ *   forward call. dx float32 [tokens][lddx] (the q and k parts; may lie on x, or on float32 dq and dk, place for place),
+ *   dq_gain, dk_gain float32 [head_dim] or 0: summed over tokens and heads in a fixed order. Calls with gain gradients, and
+ *   graphs of them, that share a handle must be ordered.
+ * Asynchronous on the context's stream; zero tokens are allowed. */
+#define QM_ROPE_INTERLEAVED 1u
+#define QM_QK_NO_NORM 1u
+#define QM_QK_BF16 2u
+typedef struct qm_rope qm_rope;
+QM_API int32_t qm_rope_create(qm_ctx *ctx, int32_t head_dim, int32_t rot_dim, float theta, const float *factors, uint32_t flags,
+                              qm_rope **out);
+QM_API int32_t qm_rope_destroy(qm_ctx *ctx, qm_rope *rope);
+QM_API int32_t qm_qk_norm_rope(qm_ctx *ctx, qm_rope *rope, uint64_t x_dev, int64_t ldx, int32_t tokens, int32_t q_heads,
+                               int32_t k_heads, uint64_t q_gain_dev, uint64_t k_gain_dev, float eps, uint64_t pos_dev,
+                               uint64_t q_out, int64_t ldq, uint64_t k_out, int64_t ldk, uint32_t flags);
+QM_API int32_t qm_qk_norm_rope_backward(qm_ctx *ctx, qm_rope *rope, uint64_t x_dev, int64_t ldx, int32_t tokens,
+                                        int32_t q_heads, int32_t k_heads, uint64_t q_gain_dev, uint64_t k_gain_dev, float eps,
+                                        uint64_t pos_dev, uint64_t dq_dev, int64_t lddq, uint64_t dk_dev, int64_t lddk,
+                                        uint64_t dx_dev, int64_t lddx, uint64_t dq_gain_dev, uint64_t dk_gain_dev,
+                                        uint32_t flags);
+
 /* GroupedTopKRouter.Route (lm/moe/moe.go:73-141) for `tokens` tokens at once: experts ranked by
  * logit + bias (descending, ties to the lower index), weights = softmax over the selected
  * experts' UNBIASED logits (exp in double, rounded to float32, float32 sum in selection order).

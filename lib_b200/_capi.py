@@ -13,6 +13,9 @@ Q4_0, Q8_0, Q2_K, Q4_K, IQ2_XXS = 2, 8, 10, 12, 16
 XOP_NONE, XOP_RMSNORM, XOP_ADD_RMSNORM, XOP_SWIGLU = 0, 1, 2, 3
 FLAG_PDL = 0x100
 FLAG_X_Q8_1 = 0x200
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30
+ROPE_INTERLEAVED = 1
+QK_NO_NORM, QK_BF16 = 1, 2
 
 
 class QmError(RuntimeError):
@@ -53,6 +56,19 @@ def _load():
         "qm_matvec": (i32, [p, u64, u64, u64, i32, i64, u64, i64, u32]),
         "qm_matvec_host": (i32, [p, u64, p, i32, i64, p, i64, u32]),
         "qm_matmul_bf16": (i32, [p, u64, u64, i32, i64, u64, i64]),
+        "qm_lora_create": (i32, [p, i64, i64, i32, i32, i32, ctypes.POINTER(p)]),
+        "qm_lora_destroy": (i32, [p, p]),
+        "qm_lora_set": (i32, [p, p, i32, i32, ctypes.c_float, u64, u64, i32]),
+        "qm_lora_matvec": (i32, [p, p, u64, u64, i32, i64, u64, u64, i64, u64, i64, u32]),
+        "qm_lora_matmul_bf16": (i32, [p, p, u64, i32, i64, u64, u64, i64, u64, i64]),
+        "qm_lora_backward": (i32, [p, p, u64, i64, u64, i64, i32, u64, u64, i64, u64, i64, u64, u64]),
+        "qm_matvec_lora": (i32, [p, u64, p, u64, u64, i32, i64, u64, u64, i64, u32]),
+        "qm_matmul_bf16_lora": (i32, [p, u64, p, u64, i32, i64, u64, u64, i64]),
+        "qm_rope_create": (i32, [p, i32, i32, ctypes.c_float, p, u32, ctypes.POINTER(p)]),
+        "qm_rope_destroy": (i32, [p, p]),
+        "qm_qk_norm_rope": (i32, [p, p, u64, i64, i32, i32, i32, u64, u64, ctypes.c_float, u64, u64, i64, u64, i64, u32]),
+        "qm_qk_norm_rope_backward": (i32, [p, p, u64, i64, i32, i32, i32, u64, u64, ctypes.c_float, u64, u64, i64, u64, i64, u64,
+                                           i64, u64, u64, u32]),
         "qm_moe_route": (i32, [p, u64, i32, i64, i32, i32, u64, u64, u64]),
         "qm_moe_grouped": (i32, [p, p, p, i32, u64, i32, i64, u64, u64, i32, u64, i64]),
         "qm_moe_dispatch": (i32, [p, u64, i32, i32, i32, u64, i64, i32, u64, u64, p]),
@@ -276,6 +292,20 @@ class Context:
         """qm_matmul_bf16: c[m][rows] = a[m][cols] (bf16) x W^T on tcgen05, fp32 out."""
         _check(lib.qm_matmul_bf16(self._h, w.handle, a_dev, m, lda, c_dev, ldc), "matmul_bf16")
 
+    def matvec_lora(self, w, lora, x_dev, m, ldx, ids_dev, y_dev, ldy, flags=0, x2_dev=0):
+        """qm_matvec_lora: qm_matvec, then the adapters of the rows' requests onto y."""
+        _check(lib.qm_matvec_lora(self._h, w.handle, lora._h, x_dev, x2_dev, m, ldx, ids_dev, y_dev, ldy, flags), "matvec_lora")
+
+    def matmul_bf16_lora(self, w, lora, a_dev, m, lda, ids_dev, c_dev, ldc):
+        """qm_matmul_bf16_lora: qm_matmul_bf16, then the adapters of the tokens' requests onto c."""
+        _check(lib.qm_matmul_bf16_lora(self._h, w.handle, lora._h, a_dev, m, lda, ids_dev, c_dev, ldc), "matmul_bf16_lora")
+
+    def lora(self, rows, cols, adapters, max_rank, max_tokens):
+        return Lora(self, rows, cols, adapters, max_rank, max_tokens)
+
+    def rope(self, head_dim, rot_dim, theta, factors=None, interleaved=False):
+        return Rope(self, head_dim, rot_dim, theta, factors, interleaved)
+
     def moe_route(self, logits_dev, tokens, ld, experts, topk, ids_dev, weights_dev, bias_dev=0):
         _check(lib.qm_moe_route(self._h, logits_dev, tokens, ld, experts, topk, bias_dev, ids_dev, weights_dev),
                "moe_route")
@@ -367,6 +397,69 @@ class Context:
         _check(lib.qm_matvec_host(self._h, w.handle, x2.ctypes.data, m, x2.shape[1], y.ctypes.data,
                                   y.shape[-1], flags), "matvec")
         return y[0] if (x.ndim == 1 and out is None) else y
+
+
+class Lora:
+    """qm_lora: low-rank adapters of many requests beside one stored projection."""
+
+    def __init__(self, ctx, rows, cols, adapters, max_rank, max_tokens):
+        self.ctx, self.rows, self.cols, self.adapters, self.max_rank, self.max_tokens = ctx, rows, cols, adapters, max_rank, max_tokens
+        h = ctypes.c_void_p()
+        _check(lib.qm_lora_create(ctx._h, rows, cols, adapters, max_rank, max_tokens, ctypes.byref(h)), "lora_create")
+        self._h = h
+
+    def set(self, slot, rank, scale, a_dev, b_dev, type=TYPE_BF16):
+        """A [rank][cols] and B [rows][rank] of device memory into a slot; rank 0 empties it."""
+        _check(lib.qm_lora_set(self.ctx._h, self._h, slot, rank, scale, a_dev, b_dev, type), "lora_set")
+
+    def matvec(self, x_dev, m, ldx, ids_dev, base_dev, ldb, y_dev, ldy, flags=0, x2_dev=0):
+        """y = base + the adapters' share for 1..8 float32 rows; ids_dev 0: slot 0 for all, base_dev 0: zeros."""
+        _check(lib.qm_lora_matvec(self.ctx._h, self._h, x_dev, x2_dev, m, ldx, ids_dev, base_dev, ldb, y_dev, ldy, flags),
+               "lora_matvec")
+
+    def matmul_bf16(self, x_dev, tokens, ldx, ids_dev, base_dev, ldb, y_dev, ldy):
+        """The same for up to max_tokens bf16 rows."""
+        _check(lib.qm_lora_matmul_bf16(self.ctx._h, self._h, x_dev, tokens, ldx, ids_dev, base_dev, ldb, y_dev, ldy),
+               "lora_matmul_bf16")
+
+    def backward(self, x_dev, ldx, dy_dev, lddy, tokens, ids_dev, base_dev, ldb, dx_dev, lddx, da_dev, db_dev):
+        """Gradients of matmul_bf16: dx (onto base), A's and B's of every slot; 0 for what is not wanted."""
+        _check(lib.qm_lora_backward(self.ctx._h, self._h, x_dev, ldx, dy_dev, lddy, tokens, ids_dev, base_dev, ldb, dx_dev, lddx,
+                                    da_dev, db_dev), "lora_backward")
+
+    def close(self):
+        if self._h:
+            lib.qm_lora_destroy(self.ctx._h, self._h)
+            self._h = None
+
+
+class Rope:
+    """qm_rope: the rotation of query and key heads by position, with their norm in the same pass."""
+
+    def __init__(self, ctx, head_dim, rot_dim, theta, factors=None, interleaved=False):
+        self.ctx, self.head_dim, self.rot_dim = ctx, head_dim, rot_dim
+        f = None if factors is None else np.ascontiguousarray(factors, dtype=np.float32).reshape(-1)
+        if f is not None and f.size != rot_dim // 2:
+            raise ValueError("factors: one for each of the rot_dim/2 pairs")
+        h = ctypes.c_void_p()
+        _check(lib.qm_rope_create(ctx._h, head_dim, rot_dim, theta, None if f is None else f.ctypes.data,
+                                  ROPE_INTERLEAVED if interleaved else 0, ctypes.byref(h)), "rope_create")
+        self._h = h
+
+    def qk_norm(self, x_dev, ldx, tokens, q_heads, k_heads, q_gain_dev, k_gain_dev, eps, pos_dev, q_dev, ldq, k_dev, ldk, flags=0):
+        _check(lib.qm_qk_norm_rope(self.ctx._h, self._h, x_dev, ldx, tokens, q_heads, k_heads, q_gain_dev, k_gain_dev, eps, pos_dev,
+                                   q_dev, ldq, k_dev, ldk, flags), "qk_norm_rope")
+
+    def qk_norm_backward(self, x_dev, ldx, tokens, q_heads, k_heads, q_gain_dev, k_gain_dev, eps, pos_dev, dq_dev, lddq, dk_dev, lddk,
+                         dx_dev, lddx, dq_gain_dev=0, dk_gain_dev=0, flags=0):
+        _check(lib.qm_qk_norm_rope_backward(self.ctx._h, self._h, x_dev, ldx, tokens, q_heads, k_heads, q_gain_dev, k_gain_dev, eps,
+                                            pos_dev, dq_dev, lddq, dk_dev, lddk, dx_dev, lddx, dq_gain_dev, dk_gain_dev, flags),
+               "qk_norm_rope_backward")
+
+    def close(self):
+        if self._h:
+            lib.qm_rope_destroy(self.ctx._h, self._h)
+            self._h = None
 
 
 class ExpertParallel:

@@ -59,6 +59,8 @@ QM_INCBIN(qm_cubin_pair, QM_STR(QM_CUBIN_DIR) "/qm_gemm_pair.sm_100a.cubin")
 QM_INCBIN(qm_cubin_moe, QM_STR(QM_CUBIN_DIR) "/qm_moe.sm_100a.cubin")
 QM_INCBIN(qm_cubin_kq, QM_STR(QM_CUBIN_DIR) "/qm_gemv_kq.sm_100a.cubin")
 QM_INCBIN(qm_cubin_q81, QM_STR(QM_CUBIN_DIR) "/qm_q8_1.sm_100a.cubin")
+QM_INCBIN(qm_cubin_lora, QM_STR(QM_CUBIN_DIR) "/qm_lora.sm_100a.cubin")
+QM_INCBIN(qm_cubin_rope, QM_STR(QM_CUBIN_DIR) "/qm_rope.sm_100a.cubin")
 
 struct KernelImage {
     const unsigned char *begin;
@@ -73,6 +75,8 @@ static const KernelImage kImages[QM_MOD_COUNT] = {
     {qm_cubin_moe, qm_cubin_moe_end},
     {qm_cubin_kq, qm_cubin_kq_end},
     {qm_cubin_q81, qm_cubin_q81_end},
+    {qm_cubin_lora, qm_cubin_lora_end},
+    {qm_cubin_rope, qm_cubin_rope_end},
 };
 struct KernelName {
     int module;
@@ -120,6 +124,14 @@ static const KernelName kKernels[QM_K_COUNT] = {
     {QM_MOD_Q4K, "qm_fused_q4k_dd_c2d2_x4"}, {QM_MOD_Q4K, "qm_fused_q4k_dd_c2d3_x4"}, {QM_MOD_Q4K, "qm_fused_q4k_dd_c2d4_x4"},
     {QM_MOD_Q4K, "qm_fused_q4k_dd_n2d2_x4"}, {QM_MOD_Q4K, "qm_fused_q4k_dd_n2d3_x4"},
     {QM_MOD_Q4K, "qm_fused_q4k_dd_n2d2"}, {QM_MOD_Q4K, "qm_fused_q4k_dd_n2d3"},
+    {QM_MOD_LORA, "qm_lora_set"},      {QM_MOD_LORA, "qm_lora_rows"},     {QM_MOD_LORA, "qm_lora_lists"},
+    {QM_MOD_LORA, "qm_lora_shrink_r16"}, {QM_MOD_LORA, "qm_lora_shrink_r32"}, {QM_MOD_LORA, "qm_lora_shrink_r64"},
+    {QM_MOD_LORA, "qm_lora_shrink_r128"}, {QM_MOD_LORA, "qm_lora_expand_r16"}, {QM_MOD_LORA, "qm_lora_expand_r32"},
+    {QM_MOD_LORA, "qm_lora_expand_r64"}, {QM_MOD_LORA, "qm_lora_expand_r128"}, {QM_MOD_LORA, "qm_lora_outer_r16"},
+    {QM_MOD_LORA, "qm_lora_outer_r32"}, {QM_MOD_LORA, "qm_lora_outer_r64"}, {QM_MOD_LORA, "qm_lora_outer_r128"},
+    {QM_MOD_ROPE, "qm_qk_norm_w1"},    {QM_MOD_ROPE, "qm_qk_norm_w2"},    {QM_MOD_ROPE, "qm_qk_norm_w4"},
+    {QM_MOD_ROPE, "qm_qk_norm_s8"},    {QM_MOD_ROPE, "qm_qk_grad_w1"},    {QM_MOD_ROPE, "qm_qk_grad_w2"},
+    {QM_MOD_ROPE, "qm_qk_grad_w4"},    {QM_MOD_ROPE, "qm_qk_grad_s8"},    {QM_MOD_ROPE, "qm_qk_gain_sum"},
 };
 
 // ---- errors --------------------------------------------------------------------------
@@ -226,6 +238,10 @@ extern "C" int32_t qm_init(int32_t device, qm_ctx **out) {
             if (r != CUDA_SUCCESS) err = (int32_t)r;
         }
         for (int k = QM_K_GEMV_Q40_M4; k <= QM_K_GEMV_Q80_M8 && !err; k++) {
+            r = d->cuFuncSetAttribute(c->fn[k], CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, QM_GEMV_SMEM_MAX);
+            if (r != CUDA_SUCCESS) err = (int32_t)r;
+        }
+        for (int k = QM_K_LORA_ROWS; k <= QM_K_LORA_OUTER_R128 && !err; k++) {
             r = d->cuFuncSetAttribute(c->fn[k], CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, QM_GEMV_SMEM_MAX);
             if (r != CUDA_SUCCESS) err = (int32_t)r;
         }

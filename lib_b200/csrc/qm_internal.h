@@ -10,7 +10,7 @@
 #define QM_CTX_MAGIC 0x514D4358u     // "QMCX"
 #define QM_WEIGHT_MAGIC 0x514D5754u  // "QMWT"
 
-enum { QM_MOD_GEMV = 0, QM_MOD_DEQUANT, QM_MOD_Q4K, QM_MOD_GEMM, QM_MOD_PAIR, QM_MOD_MOE, QM_MOD_KQ, QM_MOD_Q81, QM_MOD_COUNT };
+enum { QM_MOD_GEMV = 0, QM_MOD_DEQUANT, QM_MOD_Q4K, QM_MOD_GEMM, QM_MOD_PAIR, QM_MOD_MOE, QM_MOD_KQ, QM_MOD_Q81, QM_MOD_LORA, QM_MOD_ROPE, QM_MOD_COUNT };
 enum {
     QM_K_GEMV_Q40_M4 = 0, QM_K_GEMV_Q40_M8, QM_K_GEMV_Q80_M4,
     QM_K_GEMV_Q80_M8, QM_K_DEQUANT_Q4K, QM_K_DEQUANT_Q2K, QM_K_DEQUANT_Q40, QM_K_DEQUANT_Q80,
@@ -33,7 +33,12 @@ enum {
     QM_K_Q80_LEAN_C4D3, QM_K_Q80_LEAN_C4D2, QM_K_Q80_LEAN_C2D3, QM_K_Q80_LEAN_C2D2, QM_K_Q80_LEAN_C2N2D3, QM_K_Q80_LEAN_C2N2D2,
     QM_K_LEAN_SUM, QM_K_Q40_LEAN_X2_D4, QM_K_Q40_LEAN_X2_D2, QM_K_Q80_LEAN_X2_D2,
     QM_K_DD_X4_C2D2, QM_K_DD_X4_C2D3, QM_K_DD_X4_C2D4, QM_K_DD_X4_N2D2, QM_K_DD_X4_N2D3,
-    QM_K_FUSED_Q4K_DD_N2D2, QM_K_FUSED_Q4K_DD_N2D3, QM_K_COUNT
+    QM_K_FUSED_Q4K_DD_N2D2, QM_K_FUSED_Q4K_DD_N2D3,
+    QM_K_LORA_SET, QM_K_LORA_ROWS, QM_K_LORA_LISTS, QM_K_LORA_SHRINK_R16, QM_K_LORA_SHRINK_R32, QM_K_LORA_SHRINK_R64,
+    QM_K_LORA_SHRINK_R128, QM_K_LORA_EXPAND_R16, QM_K_LORA_EXPAND_R32, QM_K_LORA_EXPAND_R64, QM_K_LORA_EXPAND_R128,
+    QM_K_LORA_OUTER_R16, QM_K_LORA_OUTER_R32, QM_K_LORA_OUTER_R64, QM_K_LORA_OUTER_R128,
+    QM_K_QK_NORM_W1, QM_K_QK_NORM_W2, QM_K_QK_NORM_W4, QM_K_QK_NORM_S8, QM_K_QK_GRAD_W1, QM_K_QK_GRAD_W2, QM_K_QK_GRAD_W4,
+    QM_K_QK_GRAD_S8, QM_K_QK_GAIN_SUM, QM_K_COUNT
 };
 
 #define QM_GEMV_SMEM_MAX (227 * 1024)

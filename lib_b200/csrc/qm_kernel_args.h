@@ -384,3 +384,103 @@ struct QmRepackArgs {
     int64_t row_offset, nrows;
     int32_t cols, units;
 };
+
+// Norm and rotation of the q and k heads of q|k|v rows, and its backward pass (qm_rope.cu).
+struct QmQkArgs {
+    const float *x;          // [tokens][ldx]: q heads, then k heads, dim floats each
+    const float *gain_q, *gain_k;  // [dim] or null: ones
+    const int32_t *pos;      // [tokens]
+    const double *freq;      // [rot/2] turns per position
+    void *q, *k;             // forward: results; backward: gradients of the results (float32 or bf16)
+    float *dx;               // backward: [tokens][lddx]
+    float *partial;          // backward: [CTAs][2][dim] sums of the gains' gradients, or null
+    int64_t ldx, ldq, ldk, lddx;
+    int32_t tokens, hq, hk, dim, rot;
+    int32_t interleaved, norm, bf16;
+    int32_t chunk, chunks;   // heads of one warp, and how many such groups a token has
+    float eps;
+    int32_t pad_;
+};
+
+// The gains' gradients from the CTAs' sums (qm_qk_gain_sum).
+struct QmGainSumArgs {
+    const float *partial;    // [ctas][2][dim]
+    float *dq, *dk;          // [dim] or null
+    int32_t ctas, dim;
+};
+
+// Low-rank adapters beside a stored projection (qm_lora.cu). A slot's A lies as [rpad][cols] and its B transposed as
+// [rpad][np], np = rows rounded up to 8, both bf16, ranks past the slot's own and columns past `rows` zero.
+#define QM_LORA_TILE 64      // tokens of one tile: neighbours in the order by adapter
+#define QM_LORA_CLUSTER 8    // CTAs that share the rows of one adapter (qm_lora_rows)
+#define QM_LORA_CHUNK 256    // columns of B that a CTA of qm_lora_rows holds at a time
+#define QM_LORA_SHRINK_STAGES 4
+#define QM_LORA_OUTER_STAGES 3
+
+struct QmLoraSetArgs {
+    const void *a, *b;       // [rank][cols], [rows][rank]
+    uint16_t *da, *db;       // the slot's A and transposed B
+    float *scale_out;
+    int32_t *rank_out;
+    int32_t rows, cols, np, rpad, rank, type;
+    float scale;
+    int32_t pad_;
+};
+
+// 1..8 float32 rows (qm_lora_rows).
+struct QmLoraRowsArgs {
+    const float *x, *x2;
+    const int32_t *ids;      // null: every row uses slot 0
+    const float *base;       // null: zeros
+    float *y;
+    const uint16_t *a, *b;
+    const float *scale;
+    const int32_t *rank;     // 0: the slot is empty
+    int64_t ldx, ldb, ldy;
+    int32_t rows, cols, np, rpad, slots, m;
+    int32_t xop;
+    float eps;
+    int32_t nsplit;          // clusters that share the columns of one group of rows
+    int32_t pad_;
+};
+
+// Tokens in the order of their adapters (qm_lora_lists): group g < slots are the tokens of slot g, group `slots` those
+// without an adapter.
+struct QmLoraListsArgs {
+    const int32_t *ids;
+    const int32_t *rank;
+    int32_t *list;           // [tokens]
+    int32_t *offsets;        // [slots + 2]
+    int32_t *tiles;          // [0] their number, then from [4] on four words each: slot or -1, first place in list, tokens, 0
+    int32_t tokens, slots;
+};
+
+// One product with a narrow matrix: a side of the adapters. Forward: x with A; backward also dy with B.
+struct QmLoraSide {
+    const uint16_t *x;       // [tokens][ldx] bf16
+    const uint16_t *w;       // [slots][rpad][pitch] bf16
+    uint16_t *low;           // [3][max_tokens][rpad]: the products, split into three bf16 that add up to the float32 value
+    float *grad;             // gradient of w, or null
+    int64_t ldx, pitch;
+    int64_t grad_slot, grad_rank, grad_col;   // its strides
+    int32_t cols, pad_;
+};
+
+struct QmLoraBatchArgs {
+    QmLoraSide side[2];
+    const int32_t *list;     // null: token order, slot 0
+    const int32_t *offsets;
+    const int32_t *tiles;
+    const float *scale;
+    const int32_t *rank;
+    const float *base;       // expand: [tokens][ldb] or null
+    float *y;                // expand: [tokens][ldy]
+    int64_t ldb, ldy;
+    int64_t plane;           // max_tokens * rpad
+    int32_t tokens, tiles_max, rpad, slots, max_rank;
+    int32_t split;           // CTAs of a cluster that share one tile's columns (shrink) or tokens (gradients)
+    int32_t out_side;        // expand: the side whose w is multiplied by side[!out_side].low
+    int32_t vec;             // expand: base and y take float2
+    int32_t outer_units;     // gradients: column blocks times slots of the wider side
+    int32_t pad_;
+};

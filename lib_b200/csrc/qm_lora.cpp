@@ -1,0 +1,379 @@
+// qm_lora.cpp — host side of the low-rank adapters beside a stored projection (include/qmatmul.h).
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+#include <new>
+
+#include "qm_internal.h"
+
+#define QM_LORA_MAGIC 0x514D4C52u  // "QMLR"
+
+struct qm_lora {
+    uint32_t magic;
+    qm_ctx *ctx;
+    int64_t rows, cols, np;
+    int32_t slots, max_rank, rpad, max_tokens;
+    CUdeviceptr a, b;            // [slots][rpad][cols], [slots][rpad][np] bf16
+    CUdeviceptr scale, rank;     // [slots]
+    CUdeviceptr low[2];          // [3][max_tokens][rpad] bf16: u, v
+    CUdeviceptr list, offsets, tiles;
+};
+
+static int32_t lora_check(qm_ctx *c, const qm_lora *l) { return l && l->magic == QM_LORA_MAGIC && l->ctx == c ? QM_OK : QM_ERR_ARG; }
+
+// The most tiles that `tokens` tokens make: whole ones, and one that ends early for every group that has any.
+static int64_t lora_tiles(const qm_lora *l, int64_t tokens, bool listed) {
+    const int64_t whole = (tokens + QM_LORA_TILE - 1) / QM_LORA_TILE;
+    return listed ? whole + std::min<int64_t>(tokens, l->slots + 1) : whole;
+}
+
+static void lora_release(qm_ctx *c, qm_lora *l) {
+    CUdeviceptr all[] = {l->a, l->b, l->scale, l->rank, l->low[0], l->low[1], l->list, l->offsets, l->tiles};
+    for (CUdeviceptr p : all)
+        if (p) c->drv->cuMemFree_v2(p);
+    l->magic = 0;
+    delete l;
+}
+
+extern "C" int32_t qm_lora_create(qm_ctx *c, int64_t rows, int64_t cols, int32_t adapters, int32_t max_rank, int32_t max_tokens,
+                                  qm_lora **out) {
+    CHECK_CTX(c);
+    if (!out) return QM_ERR_ARG;
+    *out = nullptr;
+    if (rows < 1 || cols < 32 || cols % 32 != 0 || adapters < 1 || max_rank < 1 || max_tokens < 1) return QM_ERR_SHAPE;
+    // (cols: eight staged rows of x and a chunk of B fit in the shared memory of qm_lora_rows)
+    if (rows > (1 << 22) || cols > 32768 || adapters > 256 || max_rank > 128 || max_tokens > (1 << 20)) return QM_ERR_LIMIT;
+    qm_lora *l = new (std::nothrow) qm_lora();
+    if (!l) return QM_ERR_NOMEM;
+    l->magic = QM_LORA_MAGIC;
+    l->ctx = c;
+    l->rows = rows;
+    l->cols = cols;
+    l->np = (rows + 7) & ~(int64_t)7;
+    l->slots = adapters;
+    l->max_rank = max_rank;
+    l->rpad = max_rank <= 16 ? 16 : max_rank <= 32 ? 32 : max_rank <= 64 ? 64 : 128;
+    l->max_tokens = max_tokens;
+    CtxGuard g(c);
+    CUresult r = g.rc;
+    const int64_t low = 3ll * max_tokens * l->rpad * 2;
+    struct {
+        CUdeviceptr *p;
+        int64_t bytes;
+    } need[] = {{&l->a, (int64_t)adapters * l->rpad * cols * 2}, {&l->b, (int64_t)adapters * l->rpad * l->np * 2},
+                {&l->scale, adapters * 4ll}, {&l->rank, adapters * 4ll}, {&l->low[0], low}, {&l->low[1], low},
+                {&l->list, max_tokens * 4ll}, {&l->offsets, (adapters + 2) * 4ll},
+                {&l->tiles, 16 + 16 * lora_tiles(l, max_tokens, true)}};
+    for (auto &n : need)
+        if (r == CUDA_SUCCESS) r = c->drv->cuMemAlloc_v2(n.p, (size_t)n.bytes);
+    if (r == CUDA_SUCCESS) r = c->drv->cuMemsetD8Async(l->rank, 0, (size_t)adapters * 4, c->stream);
+    if (r != CUDA_SUCCESS) {
+        lora_release(c, l);
+        return (int32_t)r;
+    }
+    *out = l;
+    return QM_OK;
+}
+
+extern "C" int32_t qm_lora_destroy(qm_ctx *c, qm_lora *l) {
+    CHECK_CTX(c);
+    if (int32_t rc = lora_check(c, l)) return rc;
+    CtxGuard g(c);
+    DRV(g.rc);
+    c->drv->cuStreamSynchronize(c->stream);
+    lora_release(c, l);
+    return QM_OK;
+}
+
+extern "C" int32_t qm_lora_set(qm_ctx *c, qm_lora *l, int32_t slot, int32_t rank, float scale, uint64_t a_dev, uint64_t b_dev,
+                               int32_t type) {
+    CHECK_CTX(c);
+    if (int32_t rc = lora_check(c, l)) return rc;
+    if (slot < 0 || slot >= l->slots || rank < 0 || rank > l->max_rank) return QM_ERR_SHAPE;
+    if (type != QM_TYPE_F32 && type != QM_TYPE_F16 && type != QM_TYPE_BF16) return QM_ERR_FORMAT;
+    const uint64_t part = type == QM_TYPE_F32 ? 3 : 1;
+    if (!isfinite(scale) || (rank && (!a_dev || !b_dev || ((a_dev | b_dev) & part)))) return QM_ERR_ARG;
+    CtxGuard g(c);
+    DRV(g.rc);
+    QmLoraSetArgs a;
+    memset(&a, 0, sizeof a);
+    a.a = (const void *)(uintptr_t)a_dev;
+    a.b = (const void *)(uintptr_t)b_dev;
+    a.da = (uint16_t *)(uintptr_t)l->a + (int64_t)slot * l->rpad * l->cols;
+    a.db = (uint16_t *)(uintptr_t)l->b + (int64_t)slot * l->rpad * l->np;
+    a.scale_out = (float *)(uintptr_t)l->scale + slot;
+    a.rank_out = (int32_t *)(uintptr_t)l->rank + slot;
+    a.rows = (int32_t)l->rows;
+    a.cols = (int32_t)l->cols;
+    a.np = (int32_t)l->np;
+    a.rpad = l->rpad;
+    a.rank = rank;
+    a.type = type;
+    a.scale = scale;
+    const int64_t work = rank ? (int64_t)l->rpad * std::max(l->cols, l->np) / 1024 : 1;
+    return qm_launch(c, QM_K_LORA_SET, (unsigned)std::max<int64_t>(1, std::min<int64_t>(work, 4ll * c->sm_count)), 1, 256, 0, &a, true);
+}
+
+// Rows of `width` bytes, `pitch` bytes apart: do two such sets of bytes (by their hulls) meet?
+static bool rows_meet(uint64_t p, int64_t pitch_p, int64_t width_p, uint64_t q, int64_t pitch_q, int64_t width_q, int64_t rows) {
+    return p && q && p < q + (uint64_t)((rows - 1) * pitch_q + width_q) && q < p + (uint64_t)((rows - 1) * pitch_p + width_p);
+}
+// base onto y: absent, the very same rows, or apart
+static bool base_ok(uint64_t base, int64_t ldb, uint64_t y, int64_t ldy, int64_t cols, int64_t rows) {
+    return !base || (base == y && ldb == ldy) || !rows_meet(base, ldb * 4, cols * 4, y, ldy * 4, cols * 4, rows);
+}
+
+static int32_t rows_check(const qm_lora *l, uint64_t x_dev, uint64_t x2_dev, int32_t m, int64_t ldx, uint64_t ids_dev,
+                          uint64_t base_dev, int64_t ldb, uint64_t y_dev, int64_t ldy, uint32_t flags) {
+    const uint32_t xop = flags & 0xFu;
+    if (m < 1 || m > 8 || ldx < l->cols || ldy < l->rows || (base_dev && ldb < l->rows)) return QM_ERR_SHAPE;
+    if (ldx > (1 << 30) || ldy > (1 << 30) || ldb > (1 << 30)) return QM_ERR_SHAPE;
+    if (xop > QM_XOP_SWIGLU || (flags & ~(0xFu | QM_FLAG_PDL))) return QM_ERR_ARG;
+    if (!x_dev || !y_dev || (x_dev & 15) || (ldx & 3) || ((ids_dev | base_dev | y_dev) & 3)) return QM_ERR_ARG;
+    const bool two = xop == QM_XOP_ADD_RMSNORM || xop == QM_XOP_SWIGLU;
+    if (two && (!x2_dev || (x2_dev & 15))) return QM_ERR_ARG;
+    if (!base_ok(base_dev, ldb, y_dev, ldy, l->rows, m) || rows_meet(x_dev, ldx * 4, l->cols * 4, y_dev, ldy * 4, l->rows * 4, m) ||
+        (two && rows_meet(x2_dev, ldx * 4, l->cols * 4, y_dev, ldy * 4, l->rows * 4, m)) ||
+        rows_meet(ids_dev, 4, 4, y_dev, ldy * 4, l->rows * 4, m))
+        return QM_ERR_ARG;
+    return QM_OK;
+}
+
+static int32_t rows_launch(qm_ctx *c, const qm_lora *l, uint64_t x_dev, uint64_t x2_dev, int32_t m, int64_t ldx, uint64_t ids_dev,
+                           uint64_t base_dev, int64_t ldb, uint64_t y_dev, int64_t ldy, uint32_t flags) {
+    QmLoraRowsArgs a;
+    memset(&a, 0, sizeof a);
+    a.x = (const float *)(uintptr_t)x_dev;
+    a.x2 = (const float *)(uintptr_t)x2_dev;
+    a.ids = (const int32_t *)(uintptr_t)ids_dev;
+    a.base = (const float *)(uintptr_t)base_dev;
+    a.y = (float *)(uintptr_t)y_dev;
+    a.a = (const uint16_t *)(uintptr_t)l->a;
+    a.b = (const uint16_t *)(uintptr_t)l->b;
+    a.scale = (const float *)(uintptr_t)l->scale;
+    a.rank = (const int32_t *)(uintptr_t)l->rank;
+    a.ldx = ldx;
+    a.ldb = ldb;
+    a.ldy = ldy;
+    a.rows = (int32_t)l->rows;
+    a.cols = (int32_t)l->cols;
+    a.np = (int32_t)l->np;
+    a.rpad = l->rpad;
+    a.slots = l->slots;
+    a.m = m;
+    a.xop = (int32_t)(flags & 0xFu);
+    a.eps = 1e-6f;
+    // clusters per row: no more than run at once, and none with less than a chunk of columns per CTA
+    const int64_t most = (l->np + QM_LORA_CLUSTER * QM_LORA_CHUNK - 1) / (QM_LORA_CLUSTER * QM_LORA_CHUNK);
+    a.nsplit = (int32_t)std::max<int64_t>(1, std::min<int64_t>(most, c->sm_count / (QM_LORA_CLUSTER * m)));
+    const int64_t ks = ((l->cols + QM_LORA_CLUSTER - 1) / QM_LORA_CLUSTER + 7) & ~(int64_t)7;
+    const int64_t chunk = (int64_t)l->rpad * QM_LORA_CHUNK * 2;
+    const int64_t smem = 16ll * l->rpad * 4 + 136 * 4 + chunk + std::max<int64_t>(8 * ks * 4, 32 * QM_LORA_CHUNK * 4 + chunk);
+    if (smem > QM_GEMV_SMEM_MAX) return QM_ERR_LIMIT;
+    return qm_launch_ex(c, QM_K_LORA_ROWS, (unsigned)(m * a.nsplit * QM_LORA_CLUSTER), 512, (unsigned)smem, &a, true, false, QM_LORA_CLUSTER);
+}
+
+extern "C" int32_t qm_lora_matvec(qm_ctx *c, qm_lora *l, uint64_t x_dev, uint64_t x2_dev, int32_t m, int64_t ldx, uint64_t ids_dev,
+                                  uint64_t base_dev, int64_t ldb, uint64_t y_dev, int64_t ldy, uint32_t flags) {
+    CHECK_CTX(c);
+    int32_t rc = lora_check(c, l);
+    if (!rc) rc = rows_check(l, x_dev, x2_dev, m, ldx, ids_dev, base_dev, ldb, y_dev, ldy, flags);
+    if (rc) return rc;
+    CtxGuard g(c);
+    DRV(g.rc);
+    return rows_launch(c, l, x_dev, x2_dev, m, ldx, ids_dev, base_dev, ldb, y_dev, ldy, flags);
+}
+
+extern "C" int32_t qm_matvec_lora(qm_ctx *c, qm_weight h, qm_lora *l, uint64_t x_dev, uint64_t x2_dev, int32_t m, int64_t ldx,
+                                  uint64_t ids_dev, uint64_t y_dev, int64_t ldy, uint32_t flags) {
+    CHECK_CTX(c);
+    QmWeight *w = qm_weight_from_handle(h);
+    int32_t rc = w ? lora_check(c, l) : QM_ERR_ARG;
+    if (!rc && (w->rows != l->rows || w->cols != l->cols)) rc = QM_ERR_SHAPE;
+    if (!rc) rc = rows_check(l, x_dev, x2_dev, m, ldx, ids_dev, y_dev, ldy, y_dev, ldy, flags);
+    if (rc) return rc;
+    CtxGuard g(c);
+    DRV(g.rc);
+    rc = qm_matvec_launch(c, w, x_dev, x2_dev, m, ldx, y_dev, ldy, flags, c->partials_dev, c->tickets_dev);
+    if (rc) return rc;
+    return rows_launch(c, l, x_dev, x2_dev, m, ldx, ids_dev, y_dev, ldy, y_dev, ldy, flags);
+}
+
+// ---- bf16 batches ----------------------------------------------------------------------------------
+static int rank_kernel(const qm_lora *l) { return l->rpad == 16 ? 0 : l->rpad == 32 ? 1 : l->rpad == 64 ? 2 : 3; }
+
+static int32_t lists_launch(qm_ctx *c, const qm_lora *l, uint64_t ids_dev, int32_t tokens) {
+    QmLoraListsArgs a;
+    memset(&a, 0, sizeof a);
+    a.ids = (const int32_t *)(uintptr_t)ids_dev;
+    a.rank = (const int32_t *)(uintptr_t)l->rank;
+    a.list = (int32_t *)(uintptr_t)l->list;
+    a.offsets = (int32_t *)(uintptr_t)l->offsets;
+    a.tiles = (int32_t *)(uintptr_t)l->tiles;
+    a.tokens = tokens;
+    a.slots = l->slots;
+    return qm_launch(c, QM_K_LORA_LISTS, 1, 1, 1024, (unsigned)((32 * (l->slots + 1) + 1024) * 4), &a, true);
+}
+
+static void batch_args(QmLoraBatchArgs *a, const qm_lora *l, uint64_t x, int64_t ldx, uint64_t dy, int64_t lddy, uint64_t ids_dev,
+                       int32_t tokens) {
+    memset(a, 0, sizeof *a);
+    const uint64_t in[2] = {x, dy}, w[2] = {l->a, l->b};
+    const int64_t ld[2] = {ldx, lddy}, pitch[2] = {l->cols, l->np}, cols[2] = {l->cols, l->rows};
+    for (int i = 0; i < 2; i++) {
+        QmLoraSide &s = a->side[i];
+        s.x = (const uint16_t *)(uintptr_t)in[i];
+        s.w = (const uint16_t *)(uintptr_t)w[i];
+        s.low = (uint16_t *)(uintptr_t)l->low[i];
+        s.ldx = ld[i];
+        s.pitch = pitch[i];
+        s.cols = (int32_t)cols[i];
+    }
+    a->list = ids_dev ? (const int32_t *)(uintptr_t)l->list : nullptr;
+    a->offsets = (const int32_t *)(uintptr_t)l->offsets;
+    a->tiles = (const int32_t *)(uintptr_t)l->tiles;
+    a->scale = (const float *)(uintptr_t)l->scale;
+    a->rank = (const int32_t *)(uintptr_t)l->rank;
+    a->plane = (int64_t)l->max_tokens * l->rpad;
+    a->tokens = tokens;
+    a->tiles_max = (int32_t)lora_tiles(l, tokens, ids_dev != 0);
+    a->rpad = l->rpad;
+    a->slots = l->slots;
+    a->max_rank = l->max_rank;
+}
+
+// CTAs that share one piece of work of `steps` steps: as many as leave each of them four steps, while all `units` pieces
+// together are at most two CTAs per SM.
+static int32_t share(const qm_ctx *c, int64_t units, int64_t steps) {
+    int32_t s = 1;
+    while (s < 8 && units * s * 2 <= 2 * c->sm_count && steps >= 8 * s) s *= 2;
+    return s;
+}
+
+static int32_t shrink_launch(qm_ctx *c, const qm_lora *l, QmLoraBatchArgs *a, int sides) {
+    const int64_t cols = sides == 2 ? std::max(l->cols, l->rows) : l->cols;
+    // (the tiles that are there for certain; those that short lists add come on top)
+    a->split = share(c, sides * (int64_t)((a->tokens + QM_LORA_TILE - 1) / QM_LORA_TILE), (cols + 63) / 64);
+    const int64_t smem = QM_LORA_SHRINK_STAGES * (64ll + l->rpad) * 128;
+    return qm_launch_ex(c, QM_K_LORA_SHRINK_R16 + rank_kernel(l), (unsigned)(sides * a->tiles_max * a->split), 128, (unsigned)smem, a, true,
+                        false, a->split);
+}
+
+static int32_t expand_launch(qm_ctx *c, const qm_lora *l, QmLoraBatchArgs *a, int out_side, uint64_t base, int64_t ldb, uint64_t y,
+                             int64_t ldy) {
+    a->out_side = out_side;
+    a->base = (const float *)(uintptr_t)base;
+    a->ldb = ldb;
+    a->y = (float *)(uintptr_t)y;
+    a->ldy = ldy;
+    a->vec = !((base | y) & 7) && !((ldb | ldy) & 1);
+    return qm_launch(c, QM_K_LORA_EXPAND_R16 + rank_kernel(l), (unsigned)a->tiles_max, (unsigned)((a->side[out_side].cols + 127) / 128), 256,
+                     (unsigned)(l->rpad * 256), a, true);
+}
+
+static int32_t batch_check(const qm_lora *l, uint64_t x, int64_t ldx, int32_t tokens, uint64_t ids_dev, uint64_t base, int64_t ldb,
+                           uint64_t y, int64_t ldy, int64_t in_cols, int64_t out_cols) {
+    if (tokens < 0 || ldx < in_cols || ldy < out_cols || (base && ldb < out_cols)) return QM_ERR_SHAPE;
+    if (ldx > (1 << 30) || ldy > (1 << 30) || ldb > (1 << 30)) return QM_ERR_SHAPE;
+    if (tokens > l->max_tokens) return QM_ERR_LIMIT;
+    if (tokens == 0) return QM_OK;
+    if (!x || !y || (x & 15) || (ldx & 7) || ((ids_dev | base | y) & 3)) return QM_ERR_ARG;
+    if (!base_ok(base, ldb, y, ldy, out_cols, tokens) || rows_meet(x, ldx * 2, in_cols * 2, y, ldy * 4, out_cols * 4, tokens) ||
+        rows_meet(ids_dev, 4, 4, y, ldy * 4, out_cols * 4, tokens))
+        return QM_ERR_ARG;
+    return QM_OK;
+}
+
+static int32_t batch_launch(qm_ctx *c, const qm_lora *l, uint64_t x, int32_t tokens, int64_t ldx, uint64_t ids_dev, uint64_t base,
+                            int64_t ldb, uint64_t y, int64_t ldy) {
+    if (ids_dev) {
+        int32_t rc = lists_launch(c, l, ids_dev, tokens);
+        if (rc) return rc;
+    }
+    QmLoraBatchArgs a;
+    batch_args(&a, l, x, ldx, 0, 0, ids_dev, tokens);
+    int32_t rc = shrink_launch(c, l, &a, 1);
+    if (rc) return rc;
+    return expand_launch(c, l, &a, 1, base, ldb, y, ldy);
+}
+
+extern "C" int32_t qm_lora_matmul_bf16(qm_ctx *c, qm_lora *l, uint64_t x_bf16_dev, int32_t tokens, int64_t ldx, uint64_t ids_dev,
+                                       uint64_t base_dev, int64_t ldb, uint64_t y_dev, int64_t ldy) {
+    CHECK_CTX(c);
+    int32_t rc = lora_check(c, l);
+    if (!rc) rc = batch_check(l, x_bf16_dev, ldx, tokens, ids_dev, base_dev, ldb, y_dev, ldy, l->cols, l->rows);
+    if (rc || tokens == 0) return rc;
+    CtxGuard g(c);
+    DRV(g.rc);
+    return batch_launch(c, l, x_bf16_dev, tokens, ldx, ids_dev, base_dev, ldb, y_dev, ldy);
+}
+
+extern "C" int32_t qm_matmul_bf16_lora(qm_ctx *c, qm_weight h, qm_lora *l, uint64_t a_dev, int32_t m, int64_t lda, uint64_t ids_dev,
+                                       uint64_t c_dev, int64_t ldc) {
+    CHECK_CTX(c);
+    QmWeight *w = qm_weight_from_handle(h);
+    int32_t rc = w ? lora_check(c, l) : QM_ERR_ARG;
+    if (!rc && (w->rows != l->rows || w->cols != l->cols)) rc = QM_ERR_SHAPE;
+    if (!rc) rc = batch_check(l, a_dev, lda, m, ids_dev, c_dev, ldc, c_dev, ldc, l->cols, l->rows);
+    if (!rc) rc = qm_matmul_bf16(c, h, a_dev, m, lda, c_dev, ldc);   // (no tokens: refused there)
+    if (rc) return rc;
+    CtxGuard g(c);
+    DRV(g.rc);
+    return batch_launch(c, l, a_dev, m, lda, ids_dev, c_dev, ldc, c_dev, ldc);
+}
+
+extern "C" int32_t qm_lora_backward(qm_ctx *c, qm_lora *l, uint64_t x_bf16_dev, int64_t ldx, uint64_t dy_bf16_dev, int64_t lddy,
+                                    int32_t tokens, uint64_t ids_dev, uint64_t base_dev, int64_t ldb, uint64_t dx_dev, int64_t lddx,
+                                    uint64_t da_dev, uint64_t db_dev) {
+    CHECK_CTX(c);
+    int32_t rc = lora_check(c, l);
+    if (rc) return rc;
+    if (!dx_dev && !da_dev && !db_dev) return QM_ERR_ARG;
+    if (tokens < 0 || ldx < l->cols || lddy < l->rows || ldx > (1 << 30) || lddy > (1 << 30)) return QM_ERR_SHAPE;
+    if (tokens > l->max_tokens) return QM_ERR_LIMIT;
+    if (tokens && (!x_bf16_dev || !dy_bf16_dev)) return QM_ERR_ARG;
+    if (((x_bf16_dev | dy_bf16_dev) & 15) || (ldx & 7) || (lddy & 7) || ((ids_dev | da_dev | db_dev) & 3)) return QM_ERR_ARG;
+    const int64_t na = (int64_t)l->slots * l->max_rank * l->cols, nb = (int64_t)l->slots * l->max_rank * l->rows;
+    if (dx_dev) {
+        rc = batch_check(l, x_bf16_dev, ldx, tokens, ids_dev, base_dev, ldb, dx_dev, lddx, l->cols, l->cols);
+        if (rc) return rc;
+        if (tokens && rows_meet(dy_bf16_dev, lddy * 2, l->rows * 2, dx_dev, lddx * 4, l->cols * 4, tokens)) return QM_ERR_ARG;
+    }
+    CtxGuard g(c);
+    DRV(g.rc);
+    if (tokens == 0) {
+        if (da_dev) DRV(c->drv->cuMemsetD8Async(da_dev, 0, (size_t)na * 4, c->stream));
+        if (db_dev) DRV(c->drv->cuMemsetD8Async(db_dev, 0, (size_t)nb * 4, c->stream));
+        return QM_OK;
+    }
+    if (ids_dev) {
+        rc = lists_launch(c, l, ids_dev, tokens);
+        if (rc) return rc;
+    }
+    QmLoraBatchArgs a;
+    batch_args(&a, l, x_bf16_dev, ldx, dy_bf16_dev, lddy, ids_dev, tokens);
+    rc = shrink_launch(c, l, &a, 2);
+    if (rc) return rc;
+    if (dx_dev) {
+        rc = expand_launch(c, l, &a, 0, base_dev, ldb, dx_dev, lddx);
+        if (rc) return rc;
+    }
+    if (!da_dev && !db_dev) return QM_OK;
+    a.side[0].grad = (float *)(uintptr_t)da_dev;
+    a.side[0].grad_slot = (int64_t)l->max_rank * l->cols;
+    a.side[0].grad_rank = l->cols;
+    a.side[0].grad_col = 1;
+    a.side[1].grad = (float *)(uintptr_t)db_dev;
+    a.side[1].grad_slot = (int64_t)l->max_rank * l->rows;
+    a.side[1].grad_rank = 1;
+    a.side[1].grad_col = l->max_rank;
+    const int64_t ba = (l->cols + 127) / 128, bb = (l->rows + 127) / 128;
+    const int64_t slots = ids_dev ? l->slots : 1;
+    a.outer_units = (int32_t)(std::max(ba, bb) * l->slots);
+    a.split = share(c, (ba + bb) * slots, (tokens / slots + 31) / 32);
+    const int64_t smem = std::max<int64_t>(QM_LORA_OUTER_STAGES * (32 * 256 + 3 * 32 * l->rpad * 2), (int64_t)l->rpad * 132 * 4);
+    if (2ll * a.outer_units * a.split > 0x7FFFFFFF) return QM_ERR_LIMIT;
+    return qm_launch_ex(c, QM_K_LORA_OUTER_R16 + rank_kernel(l), (unsigned)(2 * a.outer_units * a.split), 256, (unsigned)smem, &a, true, false,
+                        a.split);
+}
