@@ -409,17 +409,23 @@ struct QmGainSumArgs {
     int32_t ctas, dim;
 };
 
-// Low-rank adapters beside a stored projection (qm_lora.cu). A slot's A lies as [rpad][cols] and its B transposed as
-// [rpad][np], np = rows rounded up to 8, both bf16, ranks past the slot's own and columns past `rows` zero.
+// Low-rank adapters beside a stored projection (qm_lora.cu). A slot's A lies as [rpad][cols] and as [cols][rpad], its B as
+// [rpad][np], np = rows rounded up to 8, and as [rows][rpad], all bf16, ranks past the slot's own and columns past `rows`
+// zero.
 #define QM_LORA_TILE 64      // tokens of one tile: neighbours in the order by adapter
 #define QM_LORA_CLUSTER 8    // CTAs that share the rows of one adapter (qm_lora_rows)
 #define QM_LORA_CHUNK 256    // columns of B that a CTA of qm_lora_rows holds at a time
-#define QM_LORA_SHRINK_STAGES 4
-#define QM_LORA_OUTER_STAGES 3
+// Narrow products: stages in flight and groups of warps that share the ranks, by ranks / 16.
+#define QM_LORA_SHRINK_STAGES(rp) ((rp) == 4 ? 5 : 4)
+#define QM_LORA_SHRINK_GROUPS(rp) ((rp) == 1 ? 1 : (rp) <= 4 ? 2 : 4)
+// Gradients: tokens of a stage and stages in flight, by ranks / 16.
+#define QM_LORA_OUTER_TOKENS(rp) ((rp) <= 2 ? 64 : 32)
+#define QM_LORA_OUTER_STAGES(rp) ((rp) == 1 ? 4 : (rp) == 2 ? 3 : (rp) == 4 ? 4 : 5)
 
 struct QmLoraSetArgs {
     const void *a, *b;       // [rank][cols], [rows][rank]
-    uint16_t *da, *db;       // the slot's A and transposed B
+    uint16_t *da, *db;       // the slot's [rpad][cols] and [rpad][np]
+    uint16_t *dat, *dbt;     // the slot's [cols][rpad] and [rows][rpad]
     float *scale_out;
     int32_t *rank_out;
     int32_t rows, cols, np, rpad, rank, type;
@@ -459,7 +465,8 @@ struct QmLoraListsArgs {
 struct QmLoraSide {
     const uint16_t *x;       // [tokens][ldx] bf16
     const uint16_t *w;       // [slots][rpad][pitch] bf16
-    uint16_t *low;           // [3][max_tokens][rpad]: the products, split into three bf16 that add up to the float32 value
+    const uint16_t *wt;      // [slots][cols][rpad] bf16
+    uint16_t *low;           // [3][max_tokens + 64][rpad]: the products, split into three bf16 that add up to the float32 value
     float *grad;             // gradient of w, or null
     int64_t ldx, pitch;
     int64_t grad_slot, grad_rank, grad_col;   // its strides
@@ -476,11 +483,11 @@ struct QmLoraBatchArgs {
     const float *base;       // expand: [tokens][ldb] or null
     float *y;                // expand: [tokens][ldy]
     int64_t ldb, ldy;
-    int64_t plane;           // max_tokens * rpad
+    int64_t plane;           // (max_tokens + 64) * rpad: a tile's last rows may lie behind the last token
     int32_t tokens, tiles_max, rpad, slots, max_rank;
     int32_t split;           // CTAs of a cluster that share one tile's columns (shrink) or tokens (gradients)
     int32_t out_side;        // expand: the side whose w is multiplied by side[!out_side].low
-    int32_t vec;             // expand: base and y take float2
     int32_t outer_units;     // gradients: column blocks times slots of the wider side
+    int32_t first_side;      // shrink: the side of the first half of the grid
     int32_t pad_;
 };

@@ -15,8 +15,9 @@ struct qm_lora {
     int64_t rows, cols, np;
     int32_t slots, max_rank, rpad, max_tokens;
     CUdeviceptr a, b;            // [slots][rpad][cols], [slots][rpad][np] bf16
+    CUdeviceptr at, bt;          // [slots][cols][rpad], [slots][rows][rpad] bf16
     CUdeviceptr scale, rank;     // [slots]
-    CUdeviceptr low[2];          // [3][max_tokens][rpad] bf16: u, v
+    CUdeviceptr low[2];          // [3][max_tokens + 64][rpad] bf16: u, v
     CUdeviceptr list, offsets, tiles;
 };
 
@@ -29,7 +30,7 @@ static int64_t lora_tiles(const qm_lora *l, int64_t tokens, bool listed) {
 }
 
 static void lora_release(qm_ctx *c, qm_lora *l) {
-    CUdeviceptr all[] = {l->a, l->b, l->scale, l->rank, l->low[0], l->low[1], l->list, l->offsets, l->tiles};
+    CUdeviceptr all[] = {l->a, l->b, l->at, l->bt, l->scale, l->rank, l->low[0], l->low[1], l->list, l->offsets, l->tiles};
     for (CUdeviceptr p : all)
         if (p) c->drv->cuMemFree_v2(p);
     l->magic = 0;
@@ -57,11 +58,12 @@ extern "C" int32_t qm_lora_create(qm_ctx *c, int64_t rows, int64_t cols, int32_t
     l->max_tokens = max_tokens;
     CtxGuard g(c);
     CUresult r = g.rc;
-    const int64_t low = 3ll * max_tokens * l->rpad * 2;
+    const int64_t low = 3ll * (max_tokens + QM_LORA_TILE) * l->rpad * 2;
     struct {
         CUdeviceptr *p;
         int64_t bytes;
     } need[] = {{&l->a, (int64_t)adapters * l->rpad * cols * 2}, {&l->b, (int64_t)adapters * l->rpad * l->np * 2},
+                {&l->at, (int64_t)adapters * l->rpad * cols * 2}, {&l->bt, (int64_t)adapters * l->rpad * rows * 2},
                 {&l->scale, adapters * 4ll}, {&l->rank, adapters * 4ll}, {&l->low[0], low}, {&l->low[1], low},
                 {&l->list, max_tokens * 4ll}, {&l->offsets, (adapters + 2) * 4ll},
                 {&l->tiles, 16 + 16 * lora_tiles(l, max_tokens, true)}};
@@ -102,6 +104,8 @@ extern "C" int32_t qm_lora_set(qm_ctx *c, qm_lora *l, int32_t slot, int32_t rank
     a.b = (const void *)(uintptr_t)b_dev;
     a.da = (uint16_t *)(uintptr_t)l->a + (int64_t)slot * l->rpad * l->cols;
     a.db = (uint16_t *)(uintptr_t)l->b + (int64_t)slot * l->rpad * l->np;
+    a.dat = (uint16_t *)(uintptr_t)l->at + (int64_t)slot * l->rpad * l->cols;
+    a.dbt = (uint16_t *)(uintptr_t)l->bt + (int64_t)slot * l->rpad * l->rows;
     a.scale_out = (float *)(uintptr_t)l->scale + slot;
     a.rank_out = (int32_t *)(uintptr_t)l->rank + slot;
     a.rows = (int32_t)l->rows;
@@ -111,8 +115,8 @@ extern "C" int32_t qm_lora_set(qm_ctx *c, qm_lora *l, int32_t slot, int32_t rank
     a.rank = rank;
     a.type = type;
     a.scale = scale;
-    const int64_t work = rank ? (int64_t)l->rpad * std::max(l->cols, l->np) / 1024 : 1;
-    return qm_launch(c, QM_K_LORA_SET, (unsigned)std::max<int64_t>(1, std::min<int64_t>(work, 4ll * c->sm_count)), 1, 256, 0, &a, true);
+    const int64_t tiles = rank ? (l->rpad + 31) / 32 * ((l->cols + 63) / 64 + (l->np + 63) / 64) : 1;
+    return qm_launch(c, QM_K_LORA_SET, (unsigned)std::min<int64_t>(tiles, 8ll * c->sm_count), 1, 256, 0, &a, true);
 }
 
 // Rows of `width` bytes, `pitch` bytes apart: do two such sets of bytes (by their hulls) meet?
@@ -219,12 +223,13 @@ static int32_t lists_launch(qm_ctx *c, const qm_lora *l, uint64_t ids_dev, int32
 static void batch_args(QmLoraBatchArgs *a, const qm_lora *l, uint64_t x, int64_t ldx, uint64_t dy, int64_t lddy, uint64_t ids_dev,
                        int32_t tokens) {
     memset(a, 0, sizeof *a);
-    const uint64_t in[2] = {x, dy}, w[2] = {l->a, l->b};
+    const uint64_t in[2] = {x, dy}, w[2] = {l->a, l->b}, wt[2] = {l->at, l->bt};
     const int64_t ld[2] = {ldx, lddy}, pitch[2] = {l->cols, l->np}, cols[2] = {l->cols, l->rows};
     for (int i = 0; i < 2; i++) {
         QmLoraSide &s = a->side[i];
         s.x = (const uint16_t *)(uintptr_t)in[i];
         s.w = (const uint16_t *)(uintptr_t)w[i];
+        s.wt = (const uint16_t *)(uintptr_t)wt[i];
         s.low = (uint16_t *)(uintptr_t)l->low[i];
         s.ldx = ld[i];
         s.pitch = pitch[i];
@@ -235,7 +240,7 @@ static void batch_args(QmLoraBatchArgs *a, const qm_lora *l, uint64_t x, int64_t
     a->tiles = (const int32_t *)(uintptr_t)l->tiles;
     a->scale = (const float *)(uintptr_t)l->scale;
     a->rank = (const int32_t *)(uintptr_t)l->rank;
-    a->plane = (int64_t)l->max_tokens * l->rpad;
+    a->plane = (int64_t)(l->max_tokens + QM_LORA_TILE) * l->rpad;
     a->tokens = tokens;
     a->tiles_max = (int32_t)lora_tiles(l, tokens, ids_dev != 0);
     a->rpad = l->rpad;
@@ -243,20 +248,23 @@ static void batch_args(QmLoraBatchArgs *a, const qm_lora *l, uint64_t x, int64_t
     a->max_rank = l->max_rank;
 }
 
-// CTAs that share one piece of work of `steps` steps: as many as leave each of them four steps, while all `units` pieces
-// together are at most two CTAs per SM.
-static int32_t share(const qm_ctx *c, int64_t units, int64_t steps) {
+// CTAs that share one piece of work of `steps` steps: as many as leave each of them two steps, while all `units` pieces
+// together are at most `most` CTAs.
+static int32_t share(int64_t units, int64_t steps, int64_t most) {
     int32_t s = 1;
-    while (s < 8 && units * s * 2 <= 2 * c->sm_count && steps >= 8 * s) s *= 2;
+    while (s < 8 && units * s * 2 <= most && steps >= 4 * s) s *= 2;
     return s;
 }
 
 static int32_t shrink_launch(qm_ctx *c, const qm_lora *l, QmLoraBatchArgs *a, int sides) {
     const int64_t cols = sides == 2 ? std::max(l->cols, l->rows) : l->cols;
+    a->first_side = sides == 2 && l->rows > l->cols;   // the longer one first, the shorter one fills its last wave
     // (the tiles that are there for certain; those that short lists add come on top)
-    a->split = share(c, sides * (int64_t)((a->tokens + QM_LORA_TILE - 1) / QM_LORA_TILE), (cols + 63) / 64);
-    const int64_t smem = QM_LORA_SHRINK_STAGES * (64ll + l->rpad) * 128;
-    return qm_launch_ex(c, QM_K_LORA_SHRINK_R16 + rank_kernel(l), (unsigned)(sides * a->tiles_max * a->split), 128, (unsigned)smem, a, true,
+    a->split = share(sides * (int64_t)((a->tokens + QM_LORA_TILE - 1) / QM_LORA_TILE), (cols + 127) / 128, 4ll * c->sm_count);
+    const int rp = l->rpad / 16;
+    const int64_t stages = QM_LORA_SHRINK_STAGES(rp) * (64ll + l->rpad) * 256, sums = 8 / QM_LORA_SHRINK_GROUPS(rp) * 64ll * (l->rpad + 4) * 4;
+    const int64_t smem = std::max(stages, sums);
+    return qm_launch_ex(c, QM_K_LORA_SHRINK_R16 + rank_kernel(l), (unsigned)(sides * a->tiles_max * a->split), 256, (unsigned)smem, a, true,
                         false, a->split);
 }
 
@@ -267,9 +275,8 @@ static int32_t expand_launch(qm_ctx *c, const qm_lora *l, QmLoraBatchArgs *a, in
     a->ldb = ldb;
     a->y = (float *)(uintptr_t)y;
     a->ldy = ldy;
-    a->vec = !((base | y) & 7) && !((ldb | ldy) & 1);
-    return qm_launch(c, QM_K_LORA_EXPAND_R16 + rank_kernel(l), (unsigned)a->tiles_max, (unsigned)((a->side[out_side].cols + 127) / 128), 256,
-                     (unsigned)(l->rpad * 256), a, true);
+    const bool vec = !((base | y) & 15) && !((ldb | ldy) & 3) && a->side[out_side].cols % 4 == 0;
+    return qm_launch(c, (vec ? QM_K_LORA_EXPAND_R16 : QM_K_LORA_EXPAND_R16_S) + rank_kernel(l), (unsigned)a->tiles_max, (unsigned)((a->side[out_side].cols + 255) / 256), 256, 65536, a, true);
 }
 
 static int32_t batch_check(const qm_lora *l, uint64_t x, int64_t ldx, int32_t tokens, uint64_t ids_dev, uint64_t base, int64_t ldb,
@@ -371,8 +378,9 @@ extern "C" int32_t qm_lora_backward(qm_ctx *c, qm_lora *l, uint64_t x_bf16_dev, 
     const int64_t ba = (l->cols + 127) / 128, bb = (l->rows + 127) / 128;
     const int64_t slots = ids_dev ? l->slots : 1;
     a.outer_units = (int32_t)(std::max(ba, bb) * l->slots);
-    a.split = share(c, (ba + bb) * slots, (tokens / slots + 31) / 32);
-    const int64_t smem = std::max<int64_t>(QM_LORA_OUTER_STAGES * (32 * 256 + 3 * 32 * l->rpad * 2), (int64_t)l->rpad * 132 * 4);
+    const int rp = l->rpad / 16, tb = QM_LORA_OUTER_TOKENS(rp);
+    a.split = share(((da_dev ? ba : 0) + (db_dev ? bb : 0)) * slots, (tokens / slots + tb - 1) / tb, 4ll * c->sm_count);
+    const int64_t smem = std::max<int64_t>((int64_t)QM_LORA_OUTER_STAGES(rp) * (tb * 256 + 3 * tb * l->rpad * 2), (rp <= 2 ? 4 : rp == 4 ? 2 : 1) * (int64_t)l->rpad * 132 * 4);
     if (2ll * a.outer_units * a.split > 0x7FFFFFFF) return QM_ERR_LIMIT;
     return qm_launch_ex(c, QM_K_LORA_OUTER_R16 + rank_kernel(l), (unsigned)(2 * a.outer_units * a.split), 256, (unsigned)smem, &a, true, false,
                         a.split);

@@ -111,8 +111,9 @@ __device__ __forceinline__ float read_any(const void *p, int64_t i, int type) {
 
 }  // namespace
 
-// A slot's matrices into their place: A row by row, B transposed through 32 x 32 tiles; both rounded to bf16, the type the
-// products take (float32 and float16 adapters lose bits here, bf16 ones none). Zeros behind the rank and the rows.
+// A slot's matrices into their places, both rounded to bf16, the type the products take (float32 and float16 adapters lose
+// bits here, bf16 ones none): rank by rank for what sums over the wide side, column by column for what sums over the ranks.
+// Zeros behind the rank and the rows. A block takes 32 ranks x 64 columns of A or B through shared memory.
 extern "C" __global__ void __launch_bounds__(256) qm_lora_set(const __grid_constant__ QmLoraSetArgs a) {
     wait_for_inputs();
     if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -120,23 +121,38 @@ extern "C" __global__ void __launch_bounds__(256) qm_lora_set(const __grid_const
         *a.rank_out = a.rank;
     }
     if (a.rank == 0) return;
-    const int64_t na = (int64_t)a.rpad * a.cols / 2;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < na; i += (int64_t)gridDim.x * 256) {
-        const int r = (int)(2 * i / a.cols);
-        uint32_t w = 0;
-        if (r < a.rank) w = bf_bits(read_any(a.a, 2 * i, a.type)) | bf_bits(read_any(a.a, 2 * i + 1, a.type)) << 16;
-        reinterpret_cast<uint32_t *>(a.da)[i] = w;
-    }
-    __shared__ uint16_t tile[32][33];
-    const int tr = (a.rpad + 31) / 32, tc = (a.np + 31) / 32;
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    for (int t = blockIdx.x; t < tr * tc; t += gridDim.x) {
-        const int r0 = (t % tr) * 32, n0 = (t / tr) * 32;
-        for (int i = y; i < 32; i += 8)
-            tile[i][x] = n0 + i < a.rows && r0 + x < a.rank ? (uint16_t)bf_bits(read_any(a.b, (int64_t)(n0 + i) * a.rank + r0 + x, a.type)) : 0;
+    __shared__ uint16_t tile[32][66];
+    const int tr = (a.rpad + 31) / 32, ta = (a.cols + 63) / 64, tb = (a.np + 63) / 64;
+    for (int t = blockIdx.x; t < tr * (ta + tb); t += gridDim.x) {
+        const int r0 = (t % tr) * 32, w = t / tr;
+        const bool is_a = w < ta;
+        const int c0 = (is_a ? w : w - ta) * 64, cols = is_a ? a.cols : a.rows, pitch = is_a ? a.cols : a.np;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            // A lies rank by rank, B column by column: neighbouring threads read neighbours
+            const int e = threadIdx.x + 256 * i;
+            const int r = is_a ? e >> 6 : e & 31, c = is_a ? e & 63 : e >> 5;
+            uint32_t v = 0;
+            if (r0 + r < a.rank && c0 + c < cols)
+                v = bf_bits(is_a ? read_any(a.a, (int64_t)(r0 + r) * a.cols + c0 + c, a.type) : read_any(a.b, (int64_t)(c0 + c) * a.rank + r0 + r, a.type));
+            tile[r][c] = (uint16_t)v;
+        }
         __syncthreads();
-        for (int i = y; i < 32; i += 8)
-            if (r0 + i < a.rpad && n0 + x < a.np) a.db[(int64_t)(r0 + i) * a.np + n0 + x] = tile[x][i];
+        uint16_t *by_rank = is_a ? a.da : a.db, *by_col = is_a ? a.dat : a.dbt;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int e = threadIdx.x + 256 * i;
+            {
+                const int r = e >> 5, c = (e & 31) * 2;
+                if (r0 + r < a.rpad && c0 + c < pitch)
+                    *reinterpret_cast<uint32_t *>(by_rank + (int64_t)(r0 + r) * pitch + c0 + c) = *reinterpret_cast<const uint32_t *>(&tile[r][c]);
+            }
+            {
+                const int r = (e & 15) * 2, c = e >> 4;
+                if (r0 + r < a.rpad && c0 + c < cols)
+                    *reinterpret_cast<uint32_t *>(by_col + (int64_t)(c0 + c) * a.rpad + r0 + r) = tile[r][c] | (uint32_t)tile[r + 1][c] << 16;
+            }
+        }
         __syncthreads();
     }
 }
@@ -398,12 +414,13 @@ extern "C" __global__ void __launch_bounds__(1024) qm_lora_lists(const __grid_co
 }
 
 // ---- shrink --------------------------------------------------------------------------------------------------------------
-// A cluster of `split` CTAs takes one tile of 64 tokens of one adapter, each CTA a range of the columns: four warps of 16
-// tokens each, 64 columns per stage by cp.async, 16-byte pieces swizzled so that ldmatrix meets no bank twice. The sums meet
-// in distributed shared memory and are added in CTA order. An accumulator takes the 64 columns of a stage and is then added
-// to a float32 sum: tensor core accumulation truncates, and a chain over all of K would carry that.
+// A cluster of `split` CTAs takes one tile of 64 tokens of one adapter, each CTA a range of the columns, 128 per stage by
+// cp.async (16-byte pieces swizzled so that ldmatrix meets no bank twice). The eight warps share the columns of a stage, not
+// the tokens: every warp multiplies all 64 tokens with its 16 columns, so the tokens and the adapter are read from shared
+// memory once (from 32 ranks on the warps also share the ranks, and the tokens are read two or four times). The sums meet in
+// distributed shared memory and are added in a fixed order. An accumulator takes at most four products before it is added to
+// a float32 sum: tensor core accumulation truncates, and a chain over all of K would carry that.
 namespace {
-constexpr int SHRINK_STAGES = QM_LORA_SHRINK_STAGES;
 
 template <int RP>
 __device__ __forceinline__ void shrink(const QmLoraBatchArgs &a) {
@@ -412,16 +429,21 @@ __device__ __forceinline__ void shrink(const QmLoraBatchArgs &a) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int me = a.split > 1 ? (int)cluster_rank() : 0;
     const int unit = blockIdx.x / a.split;
-    const QmLoraSide &s = a.side[unit / a.tiles_max];
+    const QmLoraSide &s = a.side[unit < a.tiles_max ? a.first_side : 1 - a.first_side];
     Tile t;
-    if (!get_tile(a, unit % a.tiles_max, &t) || t.slot < 0) return;   // the whole cluster
-    constexpr int R = RP * 16, STAGE = (64 + R) * 128;
-    const int rank = a.rank[t.slot], r16 = (rank + 15) & ~15;
-    const int chunks = (s.cols + 63) / 64, per = (chunks + a.split - 1) / a.split;
+    if (!get_tile(a, unit < a.tiles_max ? unit : unit - a.tiles_max, &t) || t.slot < 0) return;   // the whole cluster
+    constexpr int R = RP * 16, STAGE = (64 + R) * 256, STAGES = QM_LORA_SHRINK_STAGES(RP);
+    constexpr int WN = QM_LORA_SHRINK_GROUPS(RP), WK = 8 / WN;   // warps by rank and by column
+    constexpr int NP = RP / WN;                             // pairs of n-tiles of a warp
+    constexpr int SL = 8 / WK;                              // slices of 16 columns of a warp and stage
+    const int wk = warp % WK, wn = warp / WK;
+    const int rank = a.rank[t.slot], r16 = (rank + 15) & ~15, mt = (t.count + 15) >> 4;
+    const int chunks = (s.cols + 127) / 128, per = (chunks + a.split - 1) / a.split;
     const int c0 = min(me * per, chunks), cn = min(per, chunks - c0);
     const uint32_t base = smem_u32(smem);
-    // thread: piece tid % 8 of rows tid / 8 + 16 i
-    const int piece = tid & 7, sub = tid >> 3;
+    // thread: piece tid % 16 of rows tid / 16 + 16 i
+    const int piece = tid & 15, sub = tid >> 4;
+    const uint32_t sw = (piece ^ (sub & 7)) * 16;
     const uint16_t *xrow[4];
     bool there[4];
 #pragma unroll
@@ -433,68 +455,97 @@ __device__ __forceinline__ void shrink(const QmLoraBatchArgs &a) {
     const uint16_t *w = s.w + ((int64_t)t.slot * a.rpad + sub) * s.pitch + piece * 8;
     auto fetch = [&](int chunk) {
         if (chunk < cn) {
-            const uint32_t st = base + (chunk % SHRINK_STAGES) * STAGE;
-            const int col = (c0 + chunk) * 64;
+            const uint32_t st = base + (chunk % STAGES) * STAGE;
+            const int col = (c0 + chunk) * 128;
             const int left = max(0, min(16, (s.cols - col - piece * 8) * 2));   // bytes of this piece inside the rows
-            const uint32_t sw = (piece ^ (sub & 7)) * 16;
             // a piece behind the rows' end reads nothing, from an address that is there
             const int at = left ? col : -piece * 8;
 #pragma unroll
-            for (int i = 0; i < 4; i++) copy16(st + (sub + 16 * i) * 128 + sw, xrow[i] + at, there[i] ? left : 0);
+            for (int i = 0; i < 4; i++)
+                if (i < mt) copy16(st + (sub + 16 * i) * 256 + sw, xrow[i] + at, there[i] ? left : 0);
 #pragma unroll
             for (int i = 0; i < RP; i++)
-                if (16 * i < r16) copy16(st + (64 + sub + 16 * i) * 128 + sw, w + (int64_t)16 * i * s.pitch + at, left);
+                if (16 * i < r16) copy16(st + (64 + sub + 16 * i) * 256 + sw, w + (int64_t)16 * i * s.pitch + at, left);
         }
         copy_commit();
     };
-    float sum[2 * RP][4];
+    float sum[4][2 * NP][4], acc[4][2 * NP][4];
 #pragma unroll
-    for (int n = 0; n < 2 * RP; n++)
+    for (int m = 0; m < 4; m++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) sum[n][k] = 0.f;
+        for (int n = 0; n < 2 * NP; n++)
 #pragma unroll
-    for (int i = 0; i < SHRINK_STAGES - 1; i++) fetch(i);
+            for (int k = 0; k < 4; k++) sum[m][n][k] = acc[m][n][k] = 0.f;
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; i++) fetch(i);
     for (int c = 0; c < cn; c++) {
-        copy_wait<SHRINK_STAGES - 2>();
+        copy_wait<STAGES - 2>();
         __syncthreads();
-        fetch(c + SHRINK_STAGES - 1);
-        const uint32_t st = base + (c % SHRINK_STAGES) * STAGE;
-        float acc[2 * RP][4];
+        fetch(c + STAGES - 1);
+        const uint32_t st = base + (c % STAGES) * STAGE;
 #pragma unroll
-        for (int n = 0; n < 2 * RP; n++)
+        for (int sl = 0; sl < SL; sl++) {
+            const int k = wk * SL + sl;
+            uint32_t fb[NP][4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) acc[n][k] = 0.f;
+            for (int n = 0; n < NP; n++) {
+                const int wr = 64 + (wn * NP + n) * 16 + (lane & 7) + ((lane >> 4) & 1) * 8;
+                ldsm4(st + wr * 256 + (((2 * k + ((lane >> 3) & 1)) ^ (wr & 7)) * 16), fb[n]);
+            }
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            uint32_t fa[4];
-            const int row = warp * 16 + (lane & 15);
-            ldsm4(st + row * 128 + (((2 * k + (lane >> 4)) ^ (row & 7)) * 16), fa);
+            for (int m = 0; m < 4; m++)
+                if (m < mt) {
+                    uint32_t fa[4];
+                    const int row = m * 16 + (lane & 15);
+                    ldsm4(st + row * 256 + (((2 * k + (lane >> 4)) ^ (row & 7)) * 16), fa);
 #pragma unroll
-            for (int n = 0; n < RP; n++)
-                if (16 * n < r16) {
-                    uint32_t fb[4];
-                    const int wr = n * 16 + (lane & 7) + ((lane >> 4) & 1) * 8;
-                    ldsm4(st + (64 + wr) * 128 + (((2 * k + ((lane >> 3) & 1)) ^ (wr & 7)) * 16), fb);
-                    mma(acc[2 * n], fa, fb[0], fb[1]);
-                    mma(acc[2 * n + 1], fa, fb[2], fb[3]);
+                    for (int n = 0; n < NP; n++)
+                        if ((wn * NP + n) * 16 < r16) {
+                            mma(acc[m][2 * n], fa, fb[n][0], fb[n][1]);
+                            mma(acc[m][2 * n + 1], fa, fb[n][2], fb[n][3]);
+                        }
                 }
         }
+        if ((c & (4 / SL - 1)) == 4 / SL - 1 || c == cn - 1)
 #pragma unroll
-        for (int n = 0; n < 2 * RP; n++)
+            for (int m = 0; m < 4; m++)
 #pragma unroll
-            for (int k = 0; k < 4; k++) sum[n][k] += acc[n][k];
+                for (int n = 0; n < 2 * NP; n++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        sum[m][n][k] += acc[m][n][k];
+                        acc[m][n][k] = 0.f;
+                    }
     }
     copy_wait<0>();
     __syncthreads();
-    float *part = reinterpret_cast<float *>(smem);   // [64][R + 4]
+    // [WK][64][R + 4] sums of the warps, added into the first
+    float *part = reinterpret_cast<float *>(smem);
     constexpr int LD = R + 4;
     {
         const int g = lane >> 2, q = (lane & 3) * 2;
+        float *p = part + wk * 64 * LD + wn * NP * 16;
 #pragma unroll
-        for (int n = 0; n < 2 * RP; n++) {
-            *reinterpret_cast<float2 *>(part + (warp * 16 + g) * LD + n * 8 + q) = make_float2(sum[n][0], sum[n][1]);
-            *reinterpret_cast<float2 *>(part + (warp * 16 + g + 8) * LD + n * 8 + q) = make_float2(sum[n][2], sum[n][3]);
+        for (int m = 0; m < 4; m++)
+            if (m < mt) {
+#pragma unroll
+                for (int n = 0; n < 2 * NP; n++) {
+                    *reinterpret_cast<float2 *>(p + (m * 16 + g) * LD + n * 8 + q) = make_float2(sum[m][n][0], sum[m][n][1]);
+                    *reinterpret_cast<float2 *>(p + (m * 16 + g + 8) * LD + n * 8 + q) = make_float2(sum[m][n][2], sum[m][n][3]);
+                }
+            }
+    }
+    __syncthreads();
+    for (int e = tid; e < t.count * (R / 2); e += 256) {
+        float *p = part + (e / (R / 2)) * LD + (e % (R / 2)) * 2;
+        float2 v = *reinterpret_cast<float2 *>(p);
+#pragma unroll
+        for (int k = 1; k < WK; k++) {
+            const float2 o = *reinterpret_cast<const float2 *>(p + k * 64 * LD);
+            v.x += o.x;
+            v.y += o.y;
         }
+        *reinterpret_cast<float2 *>(p) = v;
     }
     __syncthreads();
     if (a.split > 1) {
@@ -502,10 +553,9 @@ __device__ __forceinline__ void shrink(const QmLoraBatchArgs &a) {
         cluster_wait();
     }
     const float scale = a.scale[t.slot];
-    const int rows = 64 / a.split;
-    for (int e = tid; e < rows * (R / 2); e += 128) {
-        const int row = me * rows + e / (R / 2), r = (e % (R / 2)) * 2;
-        if (row >= t.count) continue;
+    // the CTAs take turns over the rows
+    for (int e = tid; e < ((t.count - me + a.split - 1) / a.split) * (R / 2); e += 256) {
+        const int row = me + (e / (R / 2)) * a.split, r = (e % (R / 2)) * 2;
         const uint32_t at = smem_u32(part + row * LD + r);
         float2 v = make_float2(0.f, 0.f);
         if (a.split > 1) {
@@ -531,105 +581,142 @@ __device__ __forceinline__ void shrink(const QmLoraBatchArgs &a) {
 }
 
 // ---- expand --------------------------------------------------------------------------------------------------------------
-// A CTA takes 64 tokens x 128 columns: eight warps of 16 x 64. The token side's fragments come straight from the workspace
-// (each is used by one warp), w's tile through shared memory; base is on its way while both arrive.
-template <int RP>
+// A CTA takes a tile's tokens x 256 columns, each of its eight warps 32 columns, without a barrier. All of base is asked for
+// at the start (cp.async into the warp's own shared memory, no registers held); the adapter's fragments of the columns stay
+// in registers while the warp goes through the tokens, 16 at a time. Both operands' fragments come straight from memory: the
+// order of the ranks inside a product is free, so a lane takes eight neighbouring ranks of its token and of its column as
+// one 16-byte load each. The products are added to base in shared memory and leave in rows of 128 bytes.
+__device__ __forceinline__ void copy4(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+template <int RP, bool VEC>
 __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
     wait_for_inputs();
-    extern __shared__ __align__(128) unsigned char smem[];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    extern __shared__ __align__(128) unsigned char smem[];   // [8 warps][4][16][32] floats, 16-byte pieces swizzled by the row
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Tile t;
     if (!get_tile(a, blockIdx.x, &t)) return;
     const QmLoraSide &s = a.side[a.out_side];
-    const int n0 = blockIdx.y * 128;
-    const int wm = (warp & 3) * 16, wn = (warp >> 2) * 64;
-    const int g = lane >> 2, q = (lane & 3) * 2;
-    int64_t row[2];
-    bool there[2];
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        there[h] = wm + g + 8 * h < t.count;
-        row[h] = token_at(a, t.first + (there[h] ? wm + g + 8 * h : 0));
-    }
-    const int rank = t.slot < 0 ? 0 : a.rank[t.slot], r16 = (rank + 15) & ~15;
+    const int c0 = blockIdx.y * 256 + warp * 32;
+    if (c0 >= s.cols) return;
+    const int rank = t.slot < 0 ? 0 : a.rank[t.slot];
     if (rank == 0 && a.base == a.y) return;
-    const uint32_t base = smem_u32(smem);
-    for (int i = tid; i < r16 * 16; i += 256) {
-        const int r = i >> 4, piece = i & 15;
-        const int left = max(0, min(16, (s.cols - n0 - piece * 8) * 2));
-        copy16(base + r * 256 + ((piece ^ (r & 7)) * 16), s.w + ((int64_t)t.slot * a.rpad + r) * s.pitch + (left ? n0 + piece * 8 : 0), left);
-    }
-    copy_commit();
-    float acc[8][4];
+    const int mt = (t.count + 15) >> 4;
+    const int g = lane >> 2, q = lane & 3;
+    float *own = reinterpret_cast<float *>(smem) + warp * 4 * 512;
+    // (tokens of the tile: lane holds two, row l and 32 + l)
+    const int tok0 = (int)token_at(a, t.first + min(lane, t.count - 1)), tok1 = (int)token_at(a, t.first + min(lane + 32, t.count - 1));
+    auto token = [&](int row) { return (int64_t)__shfl_sync(0xffffffffu, row < 32 ? tok0 : tok1, row & 31); };
 #pragma unroll
-    for (int n = 0; n < 8; n++)
+    for (int m = 0; m < 4; m++) {
+        if (m < mt) {
+            if constexpr (VEC) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int c = n0 + wn + n * 8 + q;
-            float2 v = make_float2(0.f, 0.f);
-            if (a.base && there[h]) {
-                const float *p = a.base + row[h] * a.ldb + c;
-                if (a.vec && c + 1 < s.cols) v = *reinterpret_cast<const float2 *>(p);
-                else {
-                    if (c < s.cols) v.x = p[0];
-                    if (c + 1 < s.cols) v.y = p[1];
+                for (int i = 0; i < 4; i++) {
+                    const int r = (lane >> 3) + 4 * i, piece = lane & 7, c = c0 + 4 * piece;
+                    // the four rows of this step lie in one half of the tile
+                    const int64_t row = __shfl_sync(0xffffffffu, m < 2 ? tok0 : tok1, (m & 1) * 16 + r);
+                    const bool in = a.base && m * 16 + r < t.count && c < s.cols;
+                    copy16(smem_u32(own + m * 512 + r * 32 + ((piece ^ (r & 7)) * 4)), in ? (const void *)(a.base + row * a.ldb + c) : (const void *)s.wt, in ? 16 : 0);
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int64_t row = token(m * 16 + r);
+                    const bool in = a.base && m * 16 + r < t.count && c0 + lane < s.cols;
+                    copy4(smem_u32(own + m * 512 + r * 32 + (((lane >> 2) ^ (r & 7)) * 4) + (lane & 3)),
+                          in ? (const void *)(a.base + row * a.ldb + c0 + lane) : (const void *)s.wt, in ? 4 : 0);
                 }
             }
-            acc[n][2 * h] = v.x;
-            acc[n][2 * h + 1] = v.y;
         }
-    float d[8][4];
+        copy_commit();
+    }
+    constexpr int KB = RP == 1 ? 1 : RP / 2;      // groups of 32 ranks (one of 16)
+    constexpr int W = RP == 1 ? 4 : 8;            // ranks of a lane
+    const int kb = RP == 1 ? (rank > 0) : (rank + 31) / 32;
+    auto load = [](const uint16_t *p, uint32_t (&f)[W / 2]) {
+        if constexpr (W == 8) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(p);
+            f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+        } else {
+            const uint2 v = *reinterpret_cast<const uint2 *>(p);
+            f[0] = v.x; f[1] = v.y;
+        }
+    };
+    uint32_t fb[KB][4][W / 2];
 #pragma unroll
-    for (int n = 0; n < 8; n++)
+    for (int k = 0; k < KB; k++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) d[n][k] = 0.f;
-    const uint16_t *low = a.side[1 - a.out_side].low;
-    copy_wait<0>();
-    __syncthreads();
+        for (int n = 0; n < 4; n++)   // (a column behind the last one: any other, the result is not stored)
+            if (k < kb) load(s.wt + ((int64_t)t.slot * s.cols + min(c0 + n * 8 + g, s.cols - 1)) * a.rpad + k * 32 + W * q, fb[k][n]);
+    const uint16_t *low = a.side[1 - a.out_side].low + ((int64_t)t.first + g) * a.rpad + W * q;
 #pragma unroll
-    for (int k = 0; k < RP; k++) {
-        if (16 * k >= r16) break;
-        uint32_t fa[3][4];
+    for (int m = 0; m < 4; m++) {
+        if (m >= mt) break;
+        float d[4][4];
 #pragma unroll
-        for (int p = 0; p < 3; p++)
+        for (int n = 0; n < 4; n++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int h = j & 1, r = k * 16 + (j >> 1) * 8 + q;
-                fa[p][j] = there[h] ? *reinterpret_cast<const uint32_t *>(low + p * a.plane + ((int64_t)t.first + wm + g + 8 * h) * a.rpad + r) : 0u;
+            for (int k = 0; k < 4; k++) d[n][k] = 0.f;
+        const uint16_t *lm = low + (int64_t)m * 16 * a.rpad;
+#pragma unroll
+        for (int k = 0; k < KB; k++)
+            if (k < kb) {
+#pragma unroll
+                for (int p = 2; p >= 0; p--) {   // the small parts first
+                    uint32_t u0[W / 2], u1[W / 2];
+                    load(lm + p * a.plane + k * 32, u0);
+                    load(lm + p * a.plane + 8 * a.rpad + k * 32, u1);
+#pragma unroll
+                    for (int j = 0; j < W / 4; j++) {
+                        const uint32_t fa[4] = {u0[2 * j], u1[2 * j], u0[2 * j + 1], u1[2 * j + 1]};
+#pragma unroll
+                        for (int n = 0; n < 4; n++) mma(d[n], fa, fb[k][n][2 * j], fb[k][n][2 * j + 1]);
+                    }
+                }
             }
+        if (m == 0) copy_wait<3>();
+        else if (m == 1) copy_wait<2>();
+        else if (m == 2) copy_wait<1>();
+        else copy_wait<0>();
+        __syncwarp();
+        float *st = own + m * 512;
 #pragma unroll
-        for (int n = 0; n < 4; n++) {
-            uint32_t fb[4];
-            const int wr = k * 16 + (lane & 15);
-            ldsm4_t(base + wr * 256 + ((((wn >> 3) + 2 * n + (lane >> 4)) ^ (wr & 7)) * 16), fb);
+        for (int n = 0; n < 4; n++)
 #pragma unroll
-            for (int p = 2; p >= 0; p--) {   // the small parts first
-                mma(d[2 * n], fa[p], fb[0], fb[1]);
-                mma(d[2 * n + 1], fa[p], fb[2], fb[3]);
+            for (int h = 0; h < 2; h++) {   // rows g and g + 8 share their swizzle
+                float2 *p = reinterpret_cast<float2 *>(st + (g + 8 * h) * 32 + (((2 * n + (q >> 1)) ^ g) * 4) + (q & 1) * 2);
+                float2 v = *p;
+                v.x += d[n][2 * h];
+                v.y += d[n][2 * h + 1];
+                *p = v;
+            }
+        __syncwarp();
+        if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int r = (lane >> 3) + 4 * i, piece = lane & 7, c = c0 + 4 * piece;
+                const int64_t row = __shfl_sync(0xffffffffu, m < 2 ? tok0 : tok1, (m & 1) * 16 + r);
+                const float4 v = *reinterpret_cast<const float4 *>(st + r * 32 + ((piece ^ (r & 7)) * 4));
+                if (m * 16 + r < t.count && c < s.cols) *reinterpret_cast<float4 *>(a.y + row * a.ldy + c) = v;
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int64_t row = token(m * 16 + r);
+                const float v = st[r * 32 + (((lane >> 2) ^ (r & 7)) * 4) + (lane & 3)];
+                if (m * 16 + r < t.count && c0 + lane < s.cols) a.y[row * a.ldy + c0 + lane] = v;
             }
         }
     }
-#pragma unroll
-    for (int n = 0; n < 8; n++)
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int c = n0 + wn + n * 8 + q;
-            if (!there[h]) continue;
-            float *p = a.y + row[h] * a.ldy + c;
-            const float2 v = make_float2(acc[n][2 * h] + d[n][2 * h], acc[n][2 * h + 1] + d[n][2 * h + 1]);
-            if (a.vec && c + 1 < s.cols) *reinterpret_cast<float2 *>(p) = v;
-            else {
-                if (c < s.cols) p[0] = v.x;
-                if (c + 1 < s.cols) p[1] = v.y;
-            }
-        }
 }
 
 // ---- outer ---------------------------------------------------------------------------------------------------------------
 // Gradient of one slot's A (or B): a cluster of `split` CTAs takes 128 columns, each CTA a range of the slot's tokens in
-// stages of 32; both operands lie token by token and enter through transposing ldmatrix. The CTAs' sums are added in order.
-constexpr int OUTER_STAGES = QM_LORA_OUTER_STAGES;
-
+// stages; both operands lie token by token and enter through transposing ldmatrix. Up to 32 ranks four groups of warps share
+// a stage's tokens, each with all ranks and half of the columns, so that little is read from shared memory twice; more ranks
+// share the groups. The sums of the groups and of the CTAs are added in a fixed order.
 template <int RP>
 __device__ __forceinline__ void outer(const QmLoraBatchArgs &a) {
     wait_for_inputs();
@@ -652,95 +739,126 @@ __device__ __forceinline__ void outer(const QmLoraBatchArgs &a) {
             count = a.tokens;
         }
     }
-    constexpr int R = RP * 16, XB = 32 * 256, STAGE = XB + 3 * 32 * R * 2;
-    constexpr int WM = RP, WN = 8 / RP, NT = 128 / WN / 8;   // warps by rank and by column, n-tiles of a warp
-    const int chunks = (count + 31) / 32, per = (chunks + a.split - 1) / a.split;
+    constexpr int R = RP * 16, TB = QM_LORA_OUTER_TOKENS(RP), STAGES = QM_LORA_OUTER_STAGES(RP);
+    constexpr int XB = TB * 256, STAGE = XB + 3 * TB * R * 2;
+    constexpr int WM = RP <= 2 ? 1 : RP / 2, WN = 2, WK = 4 / WM;   // warps by rank, by column and by token
+    constexpr int MT = RP / WM, NT = 8, SL = TB / 16 / WK;
+    const int chunks = (count + TB - 1) / TB, per = (chunks + a.split - 1) / a.split;
     const int c0 = min(me * per, chunks), cn = min(per, chunks - c0);
-    const int wm = warp % WM, wn = warp / WM;
+    const int wm = warp % WM, wn = warp / WM % WN, wk = warp / (WM * WN);
     const uint32_t base = smem_u32(smem);
+    // tokens of the stage that is fetched next: thread's rows tid / 16 + 16 i
+    int64_t tok[TB / 16];
+    auto tokens_of = [&](int chunk) {
+#pragma unroll
+        for (int i = 0; i < TB / 16; i++) {
+            const int p = (c0 + chunk) * TB + (tid >> 4) + 16 * i;
+            tok[i] = chunk < cn && p < count ? token_at(a, first + p) : -1;
+        }
+    };
     auto fetch = [&](int chunk) {
         if (chunk < cn) {
-            const uint32_t st = base + (chunk % OUTER_STAGES) * STAGE;
-            const int p0 = (c0 + chunk) * 32;
+            const uint32_t st = base + (chunk % STAGES) * STAGE;
+            const int p0 = (c0 + chunk) * TB;
+            const int piece = tid & 15;
 #pragma unroll
-            for (int i = 0; i < 2; i++) {   // 32 tokens x 16 pieces
-                const int e = tid + 256 * i, row = e >> 4, piece = e & 15;
-                const int left = p0 + row < count ? max(0, min(16, (s.cols - n0 - piece * 8) * 2)) : 0;
-                const int64_t tok = token_at(a, first + (p0 + row < count ? p0 + row : 0));
-                copy16(st + row * 256 + ((piece ^ (row & 7)) * 16), s.x + tok * s.ldx + (left ? n0 + piece * 8 : 0), left);
+            for (int i = 0; i < TB / 16; i++) {
+                const int row = (tid >> 4) + 16 * i;
+                const int left = tok[i] >= 0 ? max(0, min(16, (s.cols - n0 - piece * 8) * 2)) : 0;
+                copy16(st + row * 256 + ((piece ^ (row & 7)) * 16), s.x + (left ? tok[i] * s.ldx + n0 + piece * 8 : 0), left);
             }
             constexpr int PIECES = R / 8;   // of a row of one plane
-            for (int e = tid; e < 3 * 32 * PIECES; e += 256) {
-                const int plane = e / (32 * PIECES), row = (e / PIECES) % 32, piece = e % PIECES;
-                const bool in = p0 + row < count && piece * 8 < r16;
+#pragma unroll
+            for (int i = 0; i < (3 * TB * PIECES + 255) / 256; i++) {
+                const int e = tid + 256 * i;
+                if (3 * TB * PIECES % 256 && e >= 3 * TB * PIECES) break;
+                const int plane = e / (TB * PIECES), row = (e / PIECES) % TB, piece2 = e % PIECES;
+                const bool in = p0 + row < count && piece2 * 8 < r16;
                 // rows of 32, 64, 128 or 256 bytes: eight rows on eight bank groups
-                const int sw = PIECES >= 8 ? piece ^ (row & 7) : PIECES == 4 ? piece ^ ((row >> 1) & 3) : piece ^ ((row >> 2) & 1);
-                copy16(st + XB + (plane * 32 + row) * (R * 2) + sw * 16,
-                       low + plane * a.plane + ((int64_t)first + (in ? p0 + row : 0)) * a.rpad + (in ? piece * 8 : 0), in ? 16 : 0);
+                const int sw = PIECES >= 8 ? piece2 ^ (row & 7) : PIECES == 4 ? piece2 ^ ((row >> 1) & 3) : piece2 ^ ((row >> 2) & 1);
+                copy16(st + XB + (plane * TB + row) * (R * 2) + sw * 16,
+                       low + plane * a.plane + ((int64_t)first + (in ? p0 + row : 0)) * a.rpad + (in ? piece2 * 8 : 0), in ? 16 : 0);
             }
         }
         copy_commit();
     };
-    float sum[NT][4];
+    float acc[MT][NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+    for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) sum[n][k] = 0.f;
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-    for (int i = 0; i < OUTER_STAGES - 1; i++) fetch(i);
+            for (int k = 0; k < 4; k++) acc[m][n][k] = 0.f;
+    tokens_of(0);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; i++) {
+        fetch(i);
+        tokens_of(i + 1);
+    }
     for (int c = 0; c < cn; c++) {
-        copy_wait<OUTER_STAGES - 2>();
+        copy_wait<STAGES - 2>();
         __syncthreads();
-        fetch(c + OUTER_STAGES - 1);
-        const uint32_t st = base + (c % OUTER_STAGES) * STAGE;
-        if (wm * 16 < r16) {
-            float acc[NT][4];
+        fetch(c + STAGES - 1);
+        tokens_of(c + STAGES);
+        const uint32_t st = base + (c % STAGES) * STAGE;
+        if (wm * MT * 16 < r16) {
 #pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) acc[n][k] = 0.f;
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                uint32_t fa[3][4];
-#pragma unroll
-                for (int p = 0; p < 3; p++) {
-                    constexpr int PIECES = R / 8;
-                    const int row = k * 16 + (lane >> 4) * 8 + (lane & 7), piece = wm * 2 + ((lane >> 3) & 1);
-                    const int sw = PIECES >= 8 ? piece ^ (row & 7) : PIECES == 4 ? piece ^ ((row >> 1) & 3) : piece ^ ((row >> 2) & 1);
-                    ldsm4_t(st + XB + (p * 32 + row) * (R * 2) + sw * 16, fa[p]);
-                }
+            for (int sl = 0; sl < SL; sl++) {
+                const int t0 = (wk * SL + sl) * 16;
+                uint32_t fb[NT / 2][4];
 #pragma unroll
                 for (int n = 0; n < NT / 2; n++) {
-                    uint32_t fb[4];
-                    const int row = k * 16 + (lane & 15);
-                    ldsm4_t(st + row * 256 + ((wn * NT + 2 * n + (lane >> 4)) ^ (row & 7)) * 16, fb);
-#pragma unroll
-                    for (int p = 2; p >= 0; p--) {
-                        mma(acc[2 * n], fa[p], fb[0], fb[1]);
-                        mma(acc[2 * n + 1], fa[p], fb[2], fb[3]);
-                    }
+                    const int row = t0 + (lane & 15);
+                    ldsm4_t(st + row * 256 + ((wn * NT + 2 * n + (lane >> 4)) ^ (row & 7)) * 16, fb[n]);
                 }
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int p = 2; p >= 0; p--) {   // the small parts first
+                        constexpr int PIECES = R / 8;
+                        uint32_t fa[4];
+                        const int row = t0 + (lane >> 4) * 8 + (lane & 7), piece = (wm * MT + m) * 2 + ((lane >> 3) & 1);
+                        const int sw = PIECES >= 8 ? piece ^ (row & 7) : PIECES == 4 ? piece ^ ((row >> 1) & 3) : piece ^ ((row >> 2) & 1);
+                        ldsm4_t(st + XB + (p * TB + row) * (R * 2) + sw * 16, fa);
+#pragma unroll
+                        for (int n = 0; n < NT / 2; n++) {
+                            mma(acc[m][2 * n], fa, fb[n][0], fb[n][1]);
+                            mma(acc[m][2 * n + 1], fa, fb[n][2], fb[n][3]);
+                        }
+                    }
             }
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) sum[n][k] += acc[n][k];
         }
     }
     copy_wait<0>();
     __syncthreads();
-    float *part = reinterpret_cast<float *>(smem);   // [R][132]
+    float *part = reinterpret_cast<float *>(smem);   // [WK][R][132]
     constexpr int LD = 132;
     {
         const int g = lane >> 2, q = (lane & 3) * 2;
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int col = (wn * NT + n) * 8 + q;
-            *reinterpret_cast<float2 *>(part + (wm * 16 + g) * LD + col) = make_float2(sum[n][0], sum[n][1]);
-            *reinterpret_cast<float2 *>(part + (wm * 16 + g + 8) * LD + col) = make_float2(sum[n][2], sum[n][3]);
-        }
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                float *p = part + (wk * R + (wm * MT + m) * 16 + g) * LD + (wn * NT + n) * 8 + q;
+                *reinterpret_cast<float2 *>(p) = make_float2(acc[m][n][0], acc[m][n][1]);
+                *reinterpret_cast<float2 *>(p + 8 * LD) = make_float2(acc[m][n][2], acc[m][n][3]);
+            }
     }
     __syncthreads();
+    if (WK > 1) {
+        for (int e = tid; e < R * 64; e += 256) {
+            float *p = part + (e >> 6) * LD + (e & 63) * 2;
+            float2 v = *reinterpret_cast<float2 *>(p);
+#pragma unroll
+            for (int k = 1; k < WK; k++) {
+                const float2 o = *reinterpret_cast<const float2 *>(p + k * R * LD);
+                v.x += o.x;
+                v.y += o.y;
+            }
+            *reinterpret_cast<float2 *>(p) = v;
+        }
+        __syncthreads();
+    }
     if (a.split > 1) {
         cluster_arrive();
         cluster_wait();
@@ -770,15 +888,19 @@ __device__ __forceinline__ void outer(const QmLoraBatchArgs &a) {
 
 }  // namespace
 
-extern "C" __global__ void __launch_bounds__(128) qm_lora_shrink_r16(const __grid_constant__ QmLoraBatchArgs a) { shrink<1>(a); }
-extern "C" __global__ void __launch_bounds__(128) qm_lora_shrink_r32(const __grid_constant__ QmLoraBatchArgs a) { shrink<2>(a); }
-extern "C" __global__ void __launch_bounds__(128) qm_lora_shrink_r64(const __grid_constant__ QmLoraBatchArgs a) { shrink<4>(a); }
-extern "C" __global__ void __launch_bounds__(128) qm_lora_shrink_r128(const __grid_constant__ QmLoraBatchArgs a) { shrink<8>(a); }
-extern "C" __global__ void __launch_bounds__(256) qm_lora_expand_r16(const __grid_constant__ QmLoraBatchArgs a) { expand<1>(a); }
-extern "C" __global__ void __launch_bounds__(256) qm_lora_expand_r32(const __grid_constant__ QmLoraBatchArgs a) { expand<2>(a); }
-extern "C" __global__ void __launch_bounds__(256) qm_lora_expand_r64(const __grid_constant__ QmLoraBatchArgs a) { expand<4>(a); }
-extern "C" __global__ void __launch_bounds__(256) qm_lora_expand_r128(const __grid_constant__ QmLoraBatchArgs a) { expand<8>(a); }
-extern "C" __global__ void __launch_bounds__(256) qm_lora_outer_r16(const __grid_constant__ QmLoraBatchArgs a) { outer<1>(a); }
-extern "C" __global__ void __launch_bounds__(256) qm_lora_outer_r32(const __grid_constant__ QmLoraBatchArgs a) { outer<2>(a); }
-extern "C" __global__ void __launch_bounds__(256) qm_lora_outer_r64(const __grid_constant__ QmLoraBatchArgs a) { outer<4>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_shrink_r16(const __grid_constant__ QmLoraBatchArgs a) { shrink<1>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_shrink_r32(const __grid_constant__ QmLoraBatchArgs a) { shrink<2>(a); }
+extern "C" __global__ void __launch_bounds__(256) qm_lora_shrink_r64(const __grid_constant__ QmLoraBatchArgs a) { shrink<4>(a); }
+extern "C" __global__ void __launch_bounds__(256) qm_lora_shrink_r128(const __grid_constant__ QmLoraBatchArgs a) { shrink<8>(a); }
+extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r16(const __grid_constant__ QmLoraBatchArgs a) { expand<1, true>(a); }
+extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r16_s(const __grid_constant__ QmLoraBatchArgs a) { expand<1, false>(a); }
+extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r32(const __grid_constant__ QmLoraBatchArgs a) { expand<2, true>(a); }
+extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r32_s(const __grid_constant__ QmLoraBatchArgs a) { expand<2, false>(a); }
+extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r64(const __grid_constant__ QmLoraBatchArgs a) { expand<4, true>(a); }
+extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r64_s(const __grid_constant__ QmLoraBatchArgs a) { expand<4, false>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_expand_r128(const __grid_constant__ QmLoraBatchArgs a) { expand<8, true>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_expand_r128_s(const __grid_constant__ QmLoraBatchArgs a) { expand<8, false>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_outer_r16(const __grid_constant__ QmLoraBatchArgs a) { outer<1>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_outer_r32(const __grid_constant__ QmLoraBatchArgs a) { outer<2>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_outer_r64(const __grid_constant__ QmLoraBatchArgs a) { outer<4>(a); }
 extern "C" __global__ void __launch_bounds__(256) qm_lora_outer_r128(const __grid_constant__ QmLoraBatchArgs a) { outer<8>(a); }
