@@ -412,15 +412,18 @@ struct QmGainSumArgs {
 // Low-rank adapters beside a stored projection (qm_lora.cu). A slot's A lies as [rpad][cols] and as [cols][rpad], its B as
 // [rpad][np], np = rows rounded up to 8, and as [rows][rpad], all bf16, ranks past the slot's own and columns past `rows`
 // zero.
-#define QM_LORA_TILE 64      // tokens of one tile: neighbours in the order by adapter
+#define QM_LORA_TILE 128     // tokens of one tile: neighbours in the order by adapter
+#define QM_LORA_BLOCK 64     // a group of tokens starts at a multiple of this in the workspace
 #define QM_LORA_CLUSTER 8    // CTAs that share the rows of one adapter (qm_lora_rows)
 #define QM_LORA_CHUNK 256    // columns of B that a CTA of qm_lora_rows holds at a time
-// Narrow products: stages in flight and groups of warps that share the ranks, by ranks / 16.
-#define QM_LORA_SHRINK_STAGES(rp) ((rp) == 4 ? 5 : 4)
-#define QM_LORA_SHRINK_GROUPS(rp) ((rp) == 1 ? 1 : (rp) <= 4 ? 2 : 4)
-// Gradients: tokens of a stage and stages in flight, by ranks / 16.
-#define QM_LORA_OUTER_TOKENS(rp) ((rp) <= 2 ? 64 : 32)
-#define QM_LORA_OUTER_STAGES(rp) ((rp) == 1 ? 4 : (rp) == 2 ? 3 : (rp) == 4 ? 4 : 5)
+// By rp = ranks / 16 (1, 2, 4, 8): elements of a workspace row (three parts of 16 rp ranks, whole 128-byte pieces), stages in
+// flight of the narrow products and of the gradients, columns that one CTA of the gradients takes, warps of it that read the
+// accumulators.
+#define QM_LORA_PITCH(rp) ((48 * (rp) + 63) / 64 * 64)
+#define QM_LORA_SHRINK_STAGES(rp) ((rp) <= 2 ? 5 : (rp) == 4 ? 4 : 3)
+#define QM_LORA_OUTER_STAGES(rp) ((rp) == 8 ? 3 : (rp) == 4 ? 5 : 4)
+#define QM_LORA_OUTER_COLS(rp) ((rp) <= 2 ? 256 : 128)
+#define QM_LORA_OUTER_READERS(rp) ((rp) == 8 ? 12 : 8)
 
 struct QmLoraSetArgs {
     const void *a, *b;       // [rank][cols], [rows][rank]
@@ -456,19 +459,17 @@ struct QmLoraListsArgs {
     const int32_t *ids;
     const int32_t *rank;
     int32_t *list;           // [tokens]
-    int32_t *offsets;        // [slots + 2]
-    int32_t *tiles;          // [0] their number, then from [4] on four words each: slot or -1, first place in list, tokens, 0
-    int32_t tokens, slots;
+    int32_t *offsets;        // [2][slots + 2]: first places of the groups in list, and of their rows in the workspace
+    int32_t *tiles;          // [tiles_max][8]: slot or -1, first place in list, tokens (0: no tile), first workspace row,
+                             // rank, unused
+    int32_t tokens, slots, tiles_max, pad_;
 };
 
 // One product with a narrow matrix: a side of the adapters. Forward: x with A; backward also dy with B.
 struct QmLoraSide {
-    const uint16_t *x;       // [tokens][ldx] bf16
-    const uint16_t *w;       // [slots][rpad][pitch] bf16
     const uint16_t *wt;      // [slots][cols][rpad] bf16
-    uint16_t *low;           // [3][max_tokens + 64][rpad]: the products, split into three bf16 that add up to the float32 value
+    uint16_t *low;           // [workspace rows][pitch]: the narrow products, split into three bf16 that add up to the float32 value
     float *grad;             // gradient of w, or null
-    int64_t ldx, pitch;
     int64_t grad_slot, grad_rank, grad_col;   // its strides
     int32_t cols, pad_;
 };
@@ -482,12 +483,21 @@ struct QmLoraBatchArgs {
     const int32_t *rank;
     const float *base;       // expand: [tokens][ldb] or null
     float *y;                // expand: [tokens][ldy]
+    unsigned int *status;
     int64_t ldb, ldy;
-    int64_t plane;           // (max_tokens + 64) * rpad: a tile's last rows may lie behind the last token
     int32_t tokens, tiles_max, rpad, slots, max_rank;
     int32_t split;           // CTAs of a cluster that share one tile's columns (shrink) or tokens (gradients)
     int32_t out_side;        // expand: the side whose w is multiplied by side[!out_side].low
     int32_t outer_units;     // gradients: column blocks times slots of the wider side
     int32_t first_side;      // shrink: the side of the first half of the grid
     int32_t pad_;
+};
+
+// The same with the tensor maps of what the tensor cores read (qm_lora_shrink_*, qm_lora_outer_*).
+struct QmLoraTcArgs {
+    CUtensorMap gather[2];   // x, dy [tokens][cols]: 64 columns of one row
+    CUtensorMap rows[2];     // the same: 64 columns of 32 rows
+    CUtensorMap w[2];        // [slots * rpad][cols]: 64 columns of rpad rows
+    CUtensorMap low[2];      // [workspace rows][pitch]: 64 elements of 64 rows
+    QmLoraBatchArgs b;
 };

@@ -17,7 +17,9 @@ struct qm_lora {
     CUdeviceptr a, b;            // [slots][rpad][cols], [slots][rpad][np] bf16
     CUdeviceptr at, bt;          // [slots][cols][rpad], [slots][rows][rpad] bf16
     CUdeviceptr scale, rank;     // [slots]
-    CUdeviceptr low[2];          // [3][max_tokens + 64][rpad] bf16: u, v
+    CUdeviceptr low[2];          // [low_rows][pitch] bf16, three parts of rpad ranks: u, v
+    int64_t low_rows;
+    CUtensorMap w_map[2], low_map[2];
     CUdeviceptr list, offsets, tiles;
 };
 
@@ -35,6 +37,15 @@ static void lora_release(qm_ctx *c, qm_lora *l) {
         if (p) c->drv->cuMemFree_v2(p);
     l->magic = 0;
     delete l;
+}
+
+// A bf16 matrix [rows][pitch] of `cols` columns, read in boxes of 64 columns x `box` rows.
+static CUresult tensor_map(qm_ctx *c, CUtensorMap *map, uint64_t p, int64_t cols, int64_t rows, int64_t pitch, int box) {
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch * 2};
+    const cuuint32_t boxes[2] = {64, (cuuint32_t)box}, one[2] = {1, 1};
+    return c->drv->cuTensorMapEncodeTiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (void *)(uintptr_t)p, dims, strides, boxes, one,
+                                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 extern "C" int32_t qm_lora_create(qm_ctx *c, int64_t rows, int64_t cols, int32_t adapters, int32_t max_rank, int32_t max_tokens,
@@ -56,20 +67,28 @@ extern "C" int32_t qm_lora_create(qm_ctx *c, int64_t rows, int64_t cols, int32_t
     l->max_rank = max_rank;
     l->rpad = max_rank <= 16 ? 16 : max_rank <= 32 ? 32 : max_rank <= 64 ? 64 : 128;
     l->max_tokens = max_tokens;
+    const int64_t pitch = QM_LORA_PITCH(l->rpad / 16);
+    l->low_rows = ((int64_t)max_tokens + QM_LORA_TILE - 1) / QM_LORA_TILE * QM_LORA_TILE + (std::min(adapters, max_tokens) + 1) * (int64_t)QM_LORA_BLOCK;
     CtxGuard g(c);
     CUresult r = g.rc;
-    const int64_t low = 3ll * (max_tokens + QM_LORA_TILE) * l->rpad * 2;
+    const int64_t low = l->low_rows * pitch * 2;
     struct {
         CUdeviceptr *p;
         int64_t bytes;
     } need[] = {{&l->a, (int64_t)adapters * l->rpad * cols * 2}, {&l->b, (int64_t)adapters * l->rpad * l->np * 2},
                 {&l->at, (int64_t)adapters * l->rpad * cols * 2}, {&l->bt, (int64_t)adapters * l->rpad * rows * 2},
                 {&l->scale, adapters * 4ll}, {&l->rank, adapters * 4ll}, {&l->low[0], low}, {&l->low[1], low},
-                {&l->list, max_tokens * 4ll}, {&l->offsets, (adapters + 2) * 4ll},
-                {&l->tiles, 16 + 16 * lora_tiles(l, max_tokens, true)}};
+                {&l->list, max_tokens * 4ll}, {&l->offsets, (adapters + 2) * 8ll},
+                {&l->tiles, 32 * lora_tiles(l, max_tokens, true)}};
     for (auto &n : need)
         if (r == CUDA_SUCCESS) r = c->drv->cuMemAlloc_v2(n.p, (size_t)n.bytes);
     if (r == CUDA_SUCCESS) r = c->drv->cuMemsetD8Async(l->rank, 0, (size_t)adapters * 4, c->stream);
+    const int64_t wide[2] = {cols, rows}, w_pitch[2] = {cols, l->np};
+    const CUdeviceptr w[2] = {l->a, l->b};
+    for (int i = 0; i < 2; i++) {
+        if (r == CUDA_SUCCESS) r = tensor_map(c, &l->w_map[i], w[i], wide[i], (int64_t)adapters * l->rpad, w_pitch[i], l->rpad);
+        if (r == CUDA_SUCCESS) r = tensor_map(c, &l->low_map[i], l->low[i], pitch, l->low_rows, pitch, QM_LORA_BLOCK);
+    }
     if (r != CUDA_SUCCESS) {
         lora_release(c, l);
         return (int32_t)r;
@@ -217,54 +236,66 @@ static int32_t lists_launch(qm_ctx *c, const qm_lora *l, uint64_t ids_dev, int32
     a.tiles = (int32_t *)(uintptr_t)l->tiles;
     a.tokens = tokens;
     a.slots = l->slots;
-    return qm_launch(c, QM_K_LORA_LISTS, 1, 1, 1024, (unsigned)((32 * (l->slots + 1) + 1024) * 4), &a, true);
+    a.tiles_max = (int32_t)lora_tiles(l, tokens, true);
+    return qm_launch(c, QM_K_LORA_LISTS, 1, 1, 1024, (unsigned)((32 * (l->slots + 1) + 1536) * 4), &a, true);
 }
 
-static void batch_args(QmLoraBatchArgs *a, const qm_lora *l, uint64_t x, int64_t ldx, uint64_t dy, int64_t lddy, uint64_t ids_dev,
-                       int32_t tokens) {
-    memset(a, 0, sizeof *a);
-    const uint64_t in[2] = {x, dy}, w[2] = {l->a, l->b}, wt[2] = {l->at, l->bt};
-    const int64_t ld[2] = {ldx, lddy}, pitch[2] = {l->cols, l->np}, cols[2] = {l->cols, l->rows};
+static int32_t batch_args(qm_ctx *c, QmLoraTcArgs *ta, const qm_lora *l, uint64_t x, int64_t ldx, uint64_t dy, int64_t lddy, uint64_t ids_dev,
+                          int32_t tokens) {
+    memset(ta, 0, sizeof *ta);
+    QmLoraBatchArgs *a = &ta->b;
+    const uint64_t in[2] = {x, dy}, wt[2] = {l->at, l->bt};
+    const int64_t ld[2] = {ldx, lddy}, cols[2] = {l->cols, l->rows};
     for (int i = 0; i < 2; i++) {
         QmLoraSide &s = a->side[i];
-        s.x = (const uint16_t *)(uintptr_t)in[i];
-        s.w = (const uint16_t *)(uintptr_t)w[i];
         s.wt = (const uint16_t *)(uintptr_t)wt[i];
         s.low = (uint16_t *)(uintptr_t)l->low[i];
-        s.ldx = ld[i];
-        s.pitch = pitch[i];
         s.cols = (int32_t)cols[i];
+        ta->w[i] = l->w_map[i];
+        ta->low[i] = l->low_map[i];
+        if (in[i]) {
+            DRV(tensor_map(c, &ta->gather[i], in[i], cols[i], tokens, ld[i], 1));
+            DRV(tensor_map(c, &ta->rows[i], in[i], cols[i], tokens, ld[i], 32));
+        }
     }
     a->list = ids_dev ? (const int32_t *)(uintptr_t)l->list : nullptr;
     a->offsets = (const int32_t *)(uintptr_t)l->offsets;
     a->tiles = (const int32_t *)(uintptr_t)l->tiles;
     a->scale = (const float *)(uintptr_t)l->scale;
     a->rank = (const int32_t *)(uintptr_t)l->rank;
-    a->plane = (int64_t)(l->max_tokens + QM_LORA_TILE) * l->rpad;
+    a->status = (unsigned int *)(uintptr_t)c->status_dev;
     a->tokens = tokens;
     a->tiles_max = (int32_t)lora_tiles(l, tokens, ids_dev != 0);
     a->rpad = l->rpad;
     a->slots = l->slots;
     a->max_rank = l->max_rank;
+    return QM_OK;
 }
 
-// CTAs that share one piece of work of `steps` steps: as many as leave each of them two steps, while all `units` pieces
-// together are at most `most` CTAs.
-static int32_t share(int64_t units, int64_t steps, int64_t most) {
-    int32_t s = 1;
-    while (s < 8 && units * s * 2 <= most && steps >= 4 * s) s *= 2;
-    return s;
+// CTAs that share one piece of work of `steps` steps, `at_once` CTAs running at a time: 1, 2, 4 or 8, whichever takes the
+// fewest steps in all, a CTA's start and end counted as eight.
+static int32_t share(int64_t units, int64_t steps, int64_t at_once) {
+    int32_t best = 1;
+    int64_t least = INT64_MAX;
+    for (int32_t s = 1; s <= 8; s *= 2) {
+        const int64_t cost = (units * s + at_once - 1) / at_once * ((steps + s - 1) / s + 8);
+        if (cost < least) {
+            least = cost;
+            best = s;
+        }
+    }
+    return best;
 }
 
-static int32_t shrink_launch(qm_ctx *c, const qm_lora *l, QmLoraBatchArgs *a, int sides) {
+static int32_t shrink_launch(qm_ctx *c, const qm_lora *l, QmLoraTcArgs *ta, int sides) {
+    QmLoraBatchArgs *a = &ta->b;
     const int64_t cols = sides == 2 ? std::max(l->cols, l->rows) : l->cols;
     a->first_side = sides == 2 && l->rows > l->cols;   // the longer one first, the shorter one fills its last wave
     // (the tiles that are there for certain; those that short lists add come on top)
-    a->split = share(sides * (int64_t)((a->tokens + QM_LORA_TILE - 1) / QM_LORA_TILE), (cols + 127) / 128, 4ll * c->sm_count);
+    a->split = share(sides * (int64_t)((a->tokens + QM_LORA_TILE - 1) / QM_LORA_TILE), (cols + 63) / 64, 2ll * c->sm_count);
     const int rp = l->rpad / 16;
-    const int64_t stages = QM_LORA_SHRINK_STAGES(rp) * (64ll + l->rpad) * 256, sums = 8 / QM_LORA_SHRINK_GROUPS(rp) * 64ll * (l->rpad + 4) * 4;
-    const int64_t smem = std::max(stages, sums);
-    return qm_launch_ex(c, QM_K_LORA_SHRINK_R16 + rank_kernel(l), (unsigned)(sides * a->tiles_max * a->split), 256, (unsigned)smem, a, true,
+    const int64_t smem = 1024 + QM_LORA_SHRINK_STAGES(rp) * (16384 + l->rpad * 128ll) + 128;
+    return qm_launch_ex(c, QM_K_LORA_SHRINK_R16 + rank_kernel(l), (unsigned)(sides * a->tiles_max * a->split), 192, (unsigned)smem, ta, true,
                         false, a->split);
 }
 
@@ -276,7 +307,8 @@ static int32_t expand_launch(qm_ctx *c, const qm_lora *l, QmLoraBatchArgs *a, in
     a->y = (float *)(uintptr_t)y;
     a->ldy = ldy;
     const bool vec = !((base | y) & 15) && !((ldb | ldy) & 3) && a->side[out_side].cols % 4 == 0;
-    return qm_launch(c, (vec ? QM_K_LORA_EXPAND_R16 : QM_K_LORA_EXPAND_R16_S) + rank_kernel(l), (unsigned)a->tiles_max, (unsigned)((a->side[out_side].cols + 255) / 256), 256, 65536, a, true);
+    return qm_launch(c, (vec ? QM_K_LORA_EXPAND_R16 : QM_K_LORA_EXPAND_R16_S) + rank_kernel(l), (unsigned)(2 * a->tiles_max),
+                     (unsigned)((a->side[out_side].cols + 255) / 256), 256, 65536, a, true);
 }
 
 static int32_t batch_check(const qm_lora *l, uint64_t x, int64_t ldx, int32_t tokens, uint64_t ids_dev, uint64_t base, int64_t ldb,
@@ -298,11 +330,11 @@ static int32_t batch_launch(qm_ctx *c, const qm_lora *l, uint64_t x, int32_t tok
         int32_t rc = lists_launch(c, l, ids_dev, tokens);
         if (rc) return rc;
     }
-    QmLoraBatchArgs a;
-    batch_args(&a, l, x, ldx, 0, 0, ids_dev, tokens);
-    int32_t rc = shrink_launch(c, l, &a, 1);
+    QmLoraTcArgs a;
+    int32_t rc = batch_args(c, &a, l, x, ldx, 0, 0, ids_dev, tokens);
+    if (!rc) rc = shrink_launch(c, l, &a, 1);
     if (rc) return rc;
-    return expand_launch(c, l, &a, 1, base, ldb, y, ldy);
+    return expand_launch(c, l, &a.b, 1, base, ldb, y, ldy);
 }
 
 extern "C" int32_t qm_lora_matmul_bf16(qm_ctx *c, qm_lora *l, uint64_t x_bf16_dev, int32_t tokens, int64_t ldx, uint64_t ids_dev,
@@ -358,10 +390,11 @@ extern "C" int32_t qm_lora_backward(qm_ctx *c, qm_lora *l, uint64_t x_bf16_dev, 
         rc = lists_launch(c, l, ids_dev, tokens);
         if (rc) return rc;
     }
-    QmLoraBatchArgs a;
-    batch_args(&a, l, x_bf16_dev, ldx, dy_bf16_dev, lddy, ids_dev, tokens);
-    rc = shrink_launch(c, l, &a, 2);
+    QmLoraTcArgs ta;
+    rc = batch_args(c, &ta, l, x_bf16_dev, ldx, dy_bf16_dev, lddy, ids_dev, tokens);
+    if (!rc) rc = shrink_launch(c, l, &ta, 2);
     if (rc) return rc;
+    QmLoraBatchArgs &a = ta.b;
     if (dx_dev) {
         rc = expand_launch(c, l, &a, 0, base_dev, ldb, dx_dev, lddx);
         if (rc) return rc;
@@ -375,13 +408,14 @@ extern "C" int32_t qm_lora_backward(qm_ctx *c, qm_lora *l, uint64_t x_bf16_dev, 
     a.side[1].grad_slot = (int64_t)l->max_rank * l->rows;
     a.side[1].grad_rank = 1;
     a.side[1].grad_col = l->max_rank;
-    const int64_t ba = (l->cols + 127) / 128, bb = (l->rows + 127) / 128;
-    const int64_t slots = ids_dev ? l->slots : 1;
+    const int rp = l->rpad / 16, bn = QM_LORA_OUTER_COLS(rp);
+    const int64_t ba = (l->cols + bn - 1) / bn, bb = (l->rows + bn - 1) / bn;
+    const int64_t slots = ids_dev ? std::min(l->slots, tokens) : 1;
     a.outer_units = (int32_t)(std::max(ba, bb) * l->slots);
-    const int rp = l->rpad / 16, tb = QM_LORA_OUTER_TOKENS(rp);
-    a.split = share(((da_dev ? ba : 0) + (db_dev ? bb : 0)) * slots, (tokens / slots + tb - 1) / tb, 4ll * c->sm_count);
-    const int64_t smem = std::max<int64_t>((int64_t)QM_LORA_OUTER_STAGES(rp) * (tb * 256 + 3 * tb * l->rpad * 2), (rp <= 2 ? 4 : rp == 4 ? 2 : 1) * (int64_t)l->rpad * 132 * 4);
+    a.split = share(((da_dev ? ba : 0) + (db_dev ? bb : 0)) * slots, (tokens / slots + 63) / 64, c->sm_count);
+    const int64_t smem = 1024 + QM_LORA_OUTER_STAGES(rp) * 8192ll * (QM_LORA_PITCH(rp) / 64 + bn / 64) + 128;
     if (2ll * a.outer_units * a.split > 0x7FFFFFFF) return QM_ERR_LIMIT;
-    return qm_launch_ex(c, QM_K_LORA_OUTER_R16 + rank_kernel(l), (unsigned)(2 * a.outer_units * a.split), 256, (unsigned)smem, &a, true, false,
+    return qm_launch_ex(c, QM_K_LORA_OUTER_R16 + rank_kernel(l), (unsigned)(2 * a.outer_units * a.split), (QM_LORA_OUTER_READERS(rp) + 2) * 32,
+                        (unsigned)smem, &ta, true, false,
                         a.split);
 }

@@ -10,6 +10,7 @@
 //   outer   grad[r][c] = sum_t low[t][r] x[t][c]
 // The 16-bit operands are multiplied as they are. low is a float32 sum; where it is an operand it is taken as the sum of
 // three bf16 (8 bits each: all 24 bits of the value), one mma for each, so no rounding to 16 bits enters a result.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -56,14 +57,6 @@ template <int N>
 __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -83,25 +76,27 @@ __device__ __forceinline__ void split3(float v, uint32_t (&p)[3]) {
 }
 
 struct Tile {
-    int slot, first, count;   // slot -1: no adapter
+    int slot, first, count, row, rank;   // slot -1: no adapter; count 0: no tile
 };
 
-// False behind the last tile.
-__device__ __forceinline__ bool get_tile(const QmLoraBatchArgs &a, int i, Tile *t) {
+__device__ __forceinline__ Tile get_tile(const QmLoraBatchArgs &a, int i) {
+    Tile t;
     if (a.list) {
-        if (i >= a.tiles[0]) return false;
-        const int4 w = *reinterpret_cast<const int4 *>(a.tiles + 4 + 4 * i);
-        t->slot = w.x;
-        t->first = w.y;
-        t->count = w.z;
-        return true;
+        const int4 w = *reinterpret_cast<const int4 *>(a.tiles + 8 * i);
+        t.slot = w.x;
+        t.first = w.y;
+        t.count = w.z;
+        t.row = w.w;
+        t.rank = a.tiles[8 * i + 4];
+    } else {
+        t.rank = a.rank[0];
+        t.slot = t.rank > 0 ? 0 : -1;
+        t.first = t.row = i * QM_LORA_TILE;
+        t.count = min(QM_LORA_TILE, a.tokens - t.first);
     }
-    t->first = i * QM_LORA_TILE;
-    t->count = min(QM_LORA_TILE, a.tokens - t->first);
-    t->slot = a.rank[0] > 0 ? 0 : -1;
-    return t->count > 0;
+    return t;
 }
-__device__ __forceinline__ int64_t token_at(const QmLoraBatchArgs &a, int place) { return a.list ? a.list[place] : place; }
+__device__ __forceinline__ int token_at(const QmLoraBatchArgs &a, int place) { return a.list ? a.list[place] : place; }
 
 __device__ __forceinline__ float read_any(const void *p, int64_t i, int type) {
     if (type == 0) return reinterpret_cast<const float *>(p)[i];
@@ -341,9 +336,9 @@ extern "C" __global__ void __launch_bounds__(512) qm_lora_rows(const __grid_cons
 // each token its place, so tokens keep their order inside a group, in every run.
 extern "C" __global__ void __launch_bounds__(1024) qm_lora_lists(const __grid_constant__ QmLoraListsArgs a) {
     wait_for_inputs();
-    extern __shared__ int32_t hist[];   // [32][groups], [512] tokens before, [512] tiles before
+    extern __shared__ int32_t hist[];   // [32][groups], then [512] tokens, tiles and workspace blocks up to and with the group
     const int groups = a.slots + 1, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    int32_t *before = hist + 32 * groups, *tiles = before + 512;
+    int32_t *before = hist + 32 * groups, *tiles = before + 512, *blocks = tiles + 512;
     for (int i = tid; i < 32 * groups; i += 1024) hist[i] = 0;
     __syncthreads();
     const int per = ((a.tokens + 31) / 32 + 31) & ~31;
@@ -366,38 +361,30 @@ extern "C" __global__ void __launch_bounds__(1024) qm_lora_lists(const __grid_co
             hist[w * groups + tid] = total;
             total += n;
         }
-    const int mine = (total + QM_LORA_TILE - 1) / QM_LORA_TILE;
     if (tid < 512) {
         before[tid] = total;
-        tiles[tid] = mine;
+        tiles[tid] = (total + QM_LORA_TILE - 1) / QM_LORA_TILE;
+        blocks[tid] = (total + QM_LORA_BLOCK - 1) / QM_LORA_BLOCK;
     }
     __syncthreads();
-    for (int o = 1; o < 512; o <<= 1) {
-        int p = 0, q = 0;
-        if (tid < 512 && tid >= o) {
+    for (int o = 1; o < groups; o <<= 1) {
+        int p = 0, q = 0, r = 0;
+        if (tid < groups && tid >= o) {
             p = before[tid - o];
             q = tiles[tid - o];
+            r = blocks[tid - o];
         }
         __syncthreads();
-        if (tid < 512) {
+        if (tid < groups) {
             before[tid] += p;
             tiles[tid] += q;
+            blocks[tid] += r;
         }
         __syncthreads();
     }
-    // both are now sums up to and with the group
-    const int ntiles = tiles[groups - 1];
-    if (tid <= groups) a.offsets[tid] = tid ? before[tid - 1] : 0;
-    if (tid == 0) a.tiles[0] = ntiles;
-    for (int i = tid; i < ntiles; i += 1024) {
-        int lo = 0, hi = groups - 1;   // the first group whose sum is above i
-        while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (tiles[mid] > i) hi = mid;
-            else lo = mid + 1;
-        }
-        const int first = (lo ? before[lo - 1] : 0) + (i - (lo ? tiles[lo - 1] : 0)) * QM_LORA_TILE;
-        *reinterpret_cast<int4 *>(a.tiles + 4 + 4 * i) = make_int4(lo < a.slots ? lo : -1, first, min(QM_LORA_TILE, before[lo] - first), 0);
+    if (tid <= groups) {
+        a.offsets[tid] = tid ? before[tid - 1] : 0;
+        a.offsets[a.slots + 2 + tid] = tid ? blocks[tid - 1] * QM_LORA_BLOCK : 0;
     }
     for (int t = t0; t < t1; t += 32) {
         const int g = t + lane < t1 ? group_of(t + lane) : -1;
@@ -411,177 +398,291 @@ extern "C" __global__ void __launch_bounds__(1024) qm_lora_lists(const __grid_co
         }
         __syncwarp();
     }
+    const int ntiles = tiles[groups - 1];
+    for (int i = tid; i < a.tiles_max; i += 1024) {
+        int4 w = make_int4(-1, 0, 0, 0);
+        int rank = 0;
+        if (i < ntiles) {
+            int lo = 0, hi = groups - 1;   // the first group whose sum is above i
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (tiles[mid] > i) hi = mid;
+                else lo = mid + 1;
+            }
+            const int in = (i - (lo ? tiles[lo - 1] : 0)) * QM_LORA_TILE;
+            w.y = (lo ? before[lo - 1] : 0) + in;
+            w.z = min(QM_LORA_TILE, before[lo] - w.y);
+            w.w = (lo ? blocks[lo - 1] * QM_LORA_BLOCK : 0) + in;
+            if (lo < a.slots) {
+                w.x = lo;
+                rank = a.rank[lo];
+            }
+        }
+        reinterpret_cast<int4 *>(a.tiles)[2 * i] = w;
+        a.tiles[8 * i + 4] = rank;
+    }
+}
+
+// ---- tcgen05 plumbing ----------------------------------------------------------------------------------------------------
+namespace {
+
+
+// Operand tiles as 128-byte rows, 16-byte pieces swizzled by the row (the 128-byte swizzle of the tensor maps). Rows along K
+// (`group` is not used: the row groups lie 1024 bytes apart), or rows along M or N with 64 elements of it each, the next 64
+// `group` bytes further.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t group) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(group >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// bf16 operands, float32 accumulators, M = 128.
+__device__ constexpr uint32_t tc_idesc(int n, bool along_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (along_mn ? 3u << 15 : 0u) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_load16(uint32_t addr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr)
+        : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map),
+                 "r"(bar), "r"(x), "r"(y)
+                 : "memory");
+}
+// Four rows by their numbers into four consecutive rows; a number behind the last row brings zeros.
+__device__ __forceinline__ void tma_rows4(uint32_t dst, const CUtensorMap *map, int x, const int (&y)[4], uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3])
+        : "memory");
+}
+
+// Tensor core accumulation truncates: a chain of n additions was seen 3e-8 n off. So an accumulator takes PERIOD stages (16
+// additions) and is then added to float32 registers while the next stages go into a second one (where tensor memory holds
+// two).
+constexpr int PERIOD = 4;
+
+// A CTA's barriers, behind its stages: full and empty per stage and per accumulator; the accumulators' address.
+struct Pipe {
+    uint32_t full, empty, acc_full, acc_empty, tmem;
+};
+// Everything that needs no input: barriers, and tensor memory. The next kernel may start only after the tensor memory of all
+// CTAs is in their hands, so that none of its CTAs can hold what one of these still asks for.
+template <int STAGES>
+__device__ __forceinline__ Pipe pipe_open(unsigned char *bars, uint32_t cols, int readers) {
+    Pipe p;
+    p.full = smem_u32(bars);
+    p.empty = p.full + 8 * STAGES;
+    p.acc_full = p.empty + 8 * STAGES;
+    p.acc_empty = p.acc_full + 16;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 2 * STAGES + 2; s++) qm::mbar_init(p.full + 8 * s, 1);
+        for (int s = 0; s < 2; s++) qm::mbar_init(p.acc_empty + 8 * s, readers);
+        qm::fence_barrier_init();
+    }
+    if (threadIdx.x < 32) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(p.acc_empty + 16), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    p.tmem = *reinterpret_cast<volatile uint32_t *>(bars + 8 * (2 * STAGES + 4));
+    wait_for_inputs();
+    return p;
+}
+__device__ __forceinline__ void pipe_close(const Pipe &p, uint32_t cols) {
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(p.tmem), "r"(cols) : "memory");
+    }
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// The multiplying thread: stage by stage, `issue(stage address, accumulator, first of a period)`.
+template <int STAGES, int NACC, class F>
+__device__ __forceinline__ void pipe_multiply(const Pipe &p, uint32_t base, uint32_t stage_bytes, int cn, unsigned int *status, F issue) {
+    for (int c = 0; c < cn; c++) {
+        const int st = c % STAGES, period = c / PERIOD, acc = period % NACC;
+        bool ok = true;
+        if (c % PERIOD == 0 && period >= NACC) ok = qm::mbar_wait_bounded(p.acc_empty + 8 * acc, (uint32_t)(period / NACC - 1) & 1u);
+        if (!ok || !qm::mbar_wait_bounded(p.full + 8 * st, (uint32_t)(c / STAGES) & 1u)) {
+            atomicOr(status, QM_STATUS_TIMEOUT);
+            return;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        issue(base + st * stage_bytes, acc, c % PERIOD == 0);
+        tc_commit(p.empty + 8 * st);
+        if (c % PERIOD == PERIOD - 1 || c == cn - 1) tc_commit(p.acc_full + 8 * acc);
+    }
+}
+// A reading warp: adds each period's accumulator columns `first`.. to v.
+template <int N, int NACC>
+__device__ __forceinline__ void pipe_read(const Pipe &p, uint32_t acc_cols, uint32_t first, int cn, unsigned int *status, float (&v)[N]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = 0.f;
+    for (int period = 0; period * PERIOD < cn; period++) {
+        const int acc = period % NACC;
+        if (!qm::mbar_wait_bounded(p.acc_full + 8 * acc, (uint32_t)(period / NACC) & 1u)) {
+            if (lane == 0) atomicOr(status, QM_STATUS_TIMEOUT);
+            return;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < N; j += 16) {
+            float o[16];
+            tc_load16(p.tmem + ((uint32_t)((warp & 3) * 32) << 16) + acc * acc_cols + first + j, o);
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[j + i] += o[i];
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p.acc_empty + 8 * acc);
+    }
+}
+// The loading warp's view of 32 rows: lane l holds the numbers of rows 4 l .. 4 l + 3 of the tile, `there` of them exist. Its
+// group of eight lanes holds 32 rows; are those that exist neighbours?
+__device__ __forceinline__ bool neighbours(const int (&rows)[4], int there) {
+    const int lane = threadIdx.x & 31;
+    const int first = __shfl_sync(0xffffffffu, rows[0], lane & 24);
+    bool ok = true;
+#pragma unroll
+    for (int i = 0; i < 4; i++) ok = ok && (i >= there || rows[i] == first + 4 * (lane & 7) + i);
+    const uint32_t all = __ballot_sync(0xffffffffu, ok);
+    return ((all >> (lane & 24)) & 0xFFu) == 0xFFu;
 }
 
 // ---- shrink --------------------------------------------------------------------------------------------------------------
-// A cluster of `split` CTAs takes one tile of 64 tokens of one adapter, each CTA a range of the columns, 128 per stage by
-// cp.async (16-byte pieces swizzled so that ldmatrix meets no bank twice). The eight warps share the columns of a stage, not
-// the tokens: every warp multiplies all 64 tokens with its 16 columns, so the tokens and the adapter are read from shared
-// memory once (from 32 ranks on the warps also share the ranks, and the tokens are read two or four times). The sums meet in
-// distributed shared memory and are added in a fixed order. An accumulator takes at most four products before it is added to
-// a float32 sum: tensor core accumulation truncates, and a chain over all of K would carry that.
-namespace {
+// A cluster of `split` CTAs takes one tile of 128 tokens of one adapter, the CTAs taking turns over its columns, 64 per
+// stage: the adapter's ranks and the tokens by TMA, 32 tokens that are neighbours as one box, others by their numbers. One
+// thread issues the products (M = the tokens, N = the ranks) into tensor memory. What a CTA reads from memory is all that
+// bounds it. The CTAs' sums meet in distributed shared memory and are added in a fixed order.
+constexpr int SHRINK_THREADS = 192;   // four warps that read the accumulators, one that loads, one that multiplies
 
 template <int RP>
-__device__ __forceinline__ void shrink(const QmLoraBatchArgs &a) {
-    wait_for_inputs();
-    extern __shared__ __align__(128) unsigned char smem[];
+__device__ __forceinline__ void shrink(const QmLoraTcArgs &ta) {
+    const QmLoraBatchArgs &a = ta.b;
+    extern __shared__ unsigned char smem_raw[];
+    constexpr int R = RP * 16, XB = 128 * 128, STAGE = XB + R * 128, STAGES = QM_LORA_SHRINK_STAGES(RP);
+    constexpr int TCOLS = 2 * R;
+    unsigned char *smem = reinterpret_cast<unsigned char *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const Pipe pipe = pipe_open<STAGES>(smem + STAGES * STAGE, TCOLS, 4);
     const int me = a.split > 1 ? (int)cluster_rank() : 0;
     const int unit = blockIdx.x / a.split;
-    const QmLoraSide &s = a.side[unit < a.tiles_max ? a.first_side : 1 - a.first_side];
-    Tile t;
-    if (!get_tile(a, unit < a.tiles_max ? unit : unit - a.tiles_max, &t) || t.slot < 0) return;   // the whole cluster
-    constexpr int R = RP * 16, STAGE = (64 + R) * 256, STAGES = QM_LORA_SHRINK_STAGES(RP);
-    constexpr int WN = QM_LORA_SHRINK_GROUPS(RP), WK = 8 / WN;   // warps by rank and by column
-    constexpr int NP = RP / WN;                             // pairs of n-tiles of a warp
-    constexpr int SL = 8 / WK;                              // slices of 16 columns of a warp and stage
-    const int wk = warp % WK, wn = warp / WK;
-    const int rank = a.rank[t.slot], r16 = (rank + 15) & ~15, mt = (t.count + 15) >> 4;
-    const int chunks = (s.cols + 127) / 128, per = (chunks + a.split - 1) / a.split;
-    const int c0 = min(me * per, chunks), cn = min(per, chunks - c0);
-    const uint32_t base = smem_u32(smem);
-    // thread: piece tid % 16 of rows tid / 16 + 16 i
-    const int piece = tid & 15, sub = tid >> 4;
-    const uint32_t sw = (piece ^ (sub & 7)) * 16;
-    const uint16_t *xrow[4];
-    bool there[4];
+    const int side = unit < a.tiles_max ? a.first_side : 1 - a.first_side;
+    const QmLoraSide &s = a.side[side];
+    const Tile t = get_tile(a, unit < a.tiles_max ? unit : unit - a.tiles_max);
+    if (t.count > 0 && t.slot >= 0) {   // the same for the whole cluster
+        const int chunks = (s.cols + 63) / 64, cn = max(0, (chunks - me + a.split - 1) / a.split);
+        const uint32_t base = smem_u32(smem);
+        float *part = reinterpret_cast<float *>(smem);   // [128][R + 4], over the stages once they are done
+        constexpr int LD = R + 4;
+        float v[R];
+        if (warp == 4) {
+            const int there = min(4, t.count - 4 * lane);
+            int rows[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int row = sub + 16 * i;
-        there[i] = row < t.count;
-        xrow[i] = s.x + token_at(a, t.first + (there[i] ? row : 0)) * s.ldx + piece * 8;
-    }
-    const uint16_t *w = s.w + ((int64_t)t.slot * a.rpad + sub) * s.pitch + piece * 8;
-    auto fetch = [&](int chunk) {
-        if (chunk < cn) {
-            const uint32_t st = base + (chunk % STAGES) * STAGE;
-            const int col = (c0 + chunk) * 128;
-            const int left = max(0, min(16, (s.cols - col - piece * 8) * 2));   // bytes of this piece inside the rows
-            // a piece behind the rows' end reads nothing, from an address that is there
-            const int at = left ? col : -piece * 8;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (i < mt) copy16(st + (sub + 16 * i) * 256 + sw, xrow[i] + at, there[i] ? left : 0);
-#pragma unroll
-            for (int i = 0; i < RP; i++)
-                if (16 * i < r16) copy16(st + (64 + sub + 16 * i) * 256 + sw, w + (int64_t)16 * i * s.pitch + at, left);
-        }
-        copy_commit();
-    };
-    float sum[4][2 * NP][4], acc[4][2 * NP][4];
-#pragma unroll
-    for (int m = 0; m < 4; m++)
-#pragma unroll
-        for (int n = 0; n < 2 * NP; n++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) sum[m][n][k] = acc[m][n][k] = 0.f;
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; i++) fetch(i);
-    for (int c = 0; c < cn; c++) {
-        copy_wait<STAGES - 2>();
-        __syncthreads();
-        fetch(c + STAGES - 1);
-        const uint32_t st = base + (c % STAGES) * STAGE;
-#pragma unroll
-        for (int sl = 0; sl < SL; sl++) {
-            const int k = wk * SL + sl;
-            uint32_t fb[NP][4];
-#pragma unroll
-            for (int n = 0; n < NP; n++) {
-                const int wr = 64 + (wn * NP + n) * 16 + (lane & 7) + ((lane >> 4) & 1) * 8;
-                ldsm4(st + wr * 256 + (((2 * k + ((lane >> 3) & 1)) ^ (wr & 7)) * 16), fb[n]);
-            }
-#pragma unroll
-            for (int m = 0; m < 4; m++)
-                if (m < mt) {
-                    uint32_t fa[4];
-                    const int row = m * 16 + (lane & 15);
-                    ldsm4(st + row * 256 + (((2 * k + (lane >> 4)) ^ (row & 7)) * 16), fa);
-#pragma unroll
-                    for (int n = 0; n < NP; n++)
-                        if ((wn * NP + n) * 16 < r16) {
-                            mma(acc[m][2 * n], fa, fb[n][0], fb[n][1]);
-                            mma(acc[m][2 * n + 1], fa, fb[n][2], fb[n][3]);
-                        }
+            for (int i = 0; i < 4; i++) rows[i] = i < there ? token_at(a, t.first + 4 * lane + i) : a.tokens;
+            // (a box may bring rows behind the tile's last token: rows of the product that are not read)
+            const bool box = neighbours(rows, there);
+            const bool one = box ? (lane & 7) == 0 && there > 0 : there > 0;
+            const uint32_t bytes = __reduce_add_sync(0xffffffffu, one ? (box ? 4096u : 512u) : 0u) + R * 128;
+            for (int c = 0; c < cn; c++) {
+                const int st = c % STAGES;
+                if (c >= STAGES && !qm::mbar_wait_bounded(pipe.empty + 8 * st, (uint32_t)(c / STAGES - 1) & 1u)) {
+                    if (lane == 0) atomicOr(a.status, QM_STATUS_TIMEOUT);
+                    break;
                 }
-        }
-        if ((c & (4 / SL - 1)) == 4 / SL - 1 || c == cn - 1)
-#pragma unroll
-            for (int m = 0; m < 4; m++)
-#pragma unroll
-                for (int n = 0; n < 2 * NP; n++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        sum[m][n][k] += acc[m][n][k];
-                        acc[m][n][k] = 0.f;
-                    }
-    }
-    copy_wait<0>();
-    __syncthreads();
-    // [WK][64][R + 4] sums of the warps, added into the first
-    float *part = reinterpret_cast<float *>(smem);
-    constexpr int LD = R + 4;
-    {
-        const int g = lane >> 2, q = (lane & 3) * 2;
-        float *p = part + wk * 64 * LD + wn * NP * 16;
-#pragma unroll
-        for (int m = 0; m < 4; m++)
-            if (m < mt) {
-#pragma unroll
-                for (int n = 0; n < 2 * NP; n++) {
-                    *reinterpret_cast<float2 *>(p + (m * 16 + g) * LD + n * 8 + q) = make_float2(sum[m][n][0], sum[m][n][1]);
-                    *reinterpret_cast<float2 *>(p + (m * 16 + g + 8) * LD + n * 8 + q) = make_float2(sum[m][n][2], sum[m][n][3]);
+                const uint32_t at = base + st * STAGE, bar = pipe.full + 8 * st;
+                const int x = (c * a.split + me) * 64;
+                if (lane == 0) {
+                    qm::mbar_expect_tx(bar, bytes);
+                    tma_box(at + XB, &ta.w[side], x, t.slot * a.rpad, bar);
+                }
+                __syncwarp();
+                if (one) {
+                    if (box) tma_box(at + lane * 512, &ta.rows[side], x, rows[0], bar);
+                    else tma_rows4(at + lane * 512, &ta.gather[side], x, rows, bar);
                 }
             }
-    }
-    __syncthreads();
-    for (int e = tid; e < t.count * (R / 2); e += 256) {
-        float *p = part + (e / (R / 2)) * LD + (e % (R / 2)) * 2;
-        float2 v = *reinterpret_cast<float2 *>(p);
+        } else if (warp == 5) {
+            if (lane == 0)
+                pipe_multiply<STAGES, 2>(pipe, base, STAGE, cn, a.status, [&](uint32_t at, int acc, bool first) {
+                    const uint64_t x = tile_desc(at, 16), w = tile_desc(at + XB, 16);
 #pragma unroll
-        for (int k = 1; k < WK; k++) {
-            const float2 o = *reinterpret_cast<const float2 *>(p + k * 64 * LD);
-            v.x += o.x;
-            v.y += o.y;
-        }
-        *reinterpret_cast<float2 *>(p) = v;
-    }
-    __syncthreads();
-    if (a.split > 1) {
-        cluster_arrive();
-        cluster_wait();
-    }
-    const float scale = a.scale[t.slot];
-    // the CTAs take turns over the rows
-    for (int e = tid; e < ((t.count - me + a.split - 1) / a.split) * (R / 2); e += 256) {
-        const int row = me + (e / (R / 2)) * a.split, r = (e % (R / 2)) * 2;
-        const uint32_t at = smem_u32(part + row * LD + r);
-        float2 v = make_float2(0.f, 0.f);
-        if (a.split > 1) {
-            for (int k = 0; k < a.split; k++) {
-                const float2 p = peer_f32x2(peer_addr(at, k));
-                v.x += p.x;
-                v.y += p.y;
-            }
+                    for (int k = 0; k < 4; k++)   // 16 columns = 32 bytes = 2 descriptor units
+                        tc_mma(pipe.tmem + acc * R, x + 2 * k, w + 2 * k, tc_idesc(R, false), !first || k > 0);
+                });
         } else {
-            v = *reinterpret_cast<const float2 *>(part + row * LD + r);
+            pipe_read<R, 2>(pipe, R, 0, cn, a.status, v);
         }
-        uint32_t p[3], q[3];
-        split3(r < rank ? v.x * scale : 0.f, p);
-        split3(r + 1 < rank ? v.y * scale : 0.f, q);
-        uint16_t *out = s.low + ((int64_t)t.first + row) * a.rpad + r;
+        __syncthreads();   // nothing uses the stages any more
+        if (warp < 4) {
 #pragma unroll
-        for (int k = 0; k < 3; k++) *reinterpret_cast<uint32_t *>(out + k * a.plane) = p[k] | q[k] << 16;
+            for (int i = 0; i < R; i += 4)
+                *reinterpret_cast<float4 *>(part + tid * LD + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
+        __syncthreads();
+        if (a.split > 1) {
+            cluster_arrive();
+            cluster_wait();
+        }
+        const float scale = a.scale[t.slot];
+        const int rows = (t.count + QM_LORA_BLOCK - 1) / QM_LORA_BLOCK * QM_LORA_BLOCK;   // zeros behind the tokens
+        constexpr int LP = QM_LORA_PITCH(RP);
+        // the CTAs take turns over the rows
+        for (int e = tid; e < ((rows - me + a.split - 1) / a.split) * (R / 2); e += SHRINK_THREADS) {
+            const int row = me + (e / (R / 2)) * a.split, r = (e % (R / 2)) * 2;
+            float2 w = make_float2(0.f, 0.f);
+            if (row < t.count) {
+                const uint32_t at = smem_u32(part + row * LD + r);
+                if (a.split > 1) {
+                    for (int k = 0; k < a.split; k++) {
+                        const float2 p = peer_f32x2(peer_addr(at, k));
+                        w.x += p.x;
+                        w.y += p.y;
+                    }
+                } else {
+                    w = *reinterpret_cast<const float2 *>(part + row * LD + r);
+                }
+            }
+            uint32_t p[3], q[3];
+            split3(r < t.rank ? w.x * scale : 0.f, p);
+            split3(r + 1 < t.rank ? w.y * scale : 0.f, q);
+            uint16_t *out = s.low + ((int64_t)t.row + row) * LP + r;
+#pragma unroll
+            for (int k = 0; k < 3; k++) *reinterpret_cast<uint32_t *>(out + k * R) = p[k] | q[k] << 16;
+        }
+        if (a.split > 1) {
+            cluster_arrive();
+            cluster_wait();
+        }
     }
-    if (a.split > 1) {
-        cluster_arrive();
-        cluster_wait();
-    }
+    pipe_close(pipe, TCOLS);
 }
 
 // ---- expand --------------------------------------------------------------------------------------------------------------
-// A CTA takes a tile's tokens x 256 columns, each of its eight warps 32 columns, without a barrier. All of base is asked for
+// A CTA takes half a tile's tokens x 256 columns, each of its eight warps 32 columns, without a barrier. All of base is asked for
 // at the start (cp.async into the warp's own shared memory, no registers held); the adapter's fragments of the columns stay
 // in registers while the warp goes through the tokens, 16 at a time. Both operands' fragments come straight from memory: the
 // order of the ranks inside a product is free, so a lane takes eight neighbouring ranks of its token and of its column as
@@ -595,18 +696,24 @@ __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
     wait_for_inputs();
     extern __shared__ __align__(128) unsigned char smem[];   // [8 warps][4][16][32] floats, 16-byte pieces swizzled by the row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    Tile t;
-    if (!get_tile(a, blockIdx.x, &t)) return;
+    Tile t = get_tile(a, blockIdx.x >> 1);
+    if (blockIdx.x & 1) {
+        t.first += 64;
+        t.row += 64;
+        t.count -= 64;
+    }
+    t.count = min(t.count, 64);
+    if (t.count <= 0) return;
     const QmLoraSide &s = a.side[a.out_side];
     const int c0 = blockIdx.y * 256 + warp * 32;
     if (c0 >= s.cols) return;
-    const int rank = t.slot < 0 ? 0 : a.rank[t.slot];
+    const int rank = t.slot < 0 ? 0 : t.rank;
     if (rank == 0 && a.base == a.y) return;
     const int mt = (t.count + 15) >> 4;
     const int g = lane >> 2, q = lane & 3;
     float *own = reinterpret_cast<float *>(smem) + warp * 4 * 512;
     // (tokens of the tile: lane holds two, row l and 32 + l)
-    const int tok0 = (int)token_at(a, t.first + min(lane, t.count - 1)), tok1 = (int)token_at(a, t.first + min(lane + 32, t.count - 1));
+    const int tok0 = token_at(a, t.first + min(lane, t.count - 1)), tok1 = token_at(a, t.first + min(lane + 32, t.count - 1));
     auto token = [&](int row) { return (int64_t)__shfl_sync(0xffffffffu, row < 32 ? tok0 : tok1, row & 31); };
 #pragma unroll
     for (int m = 0; m < 4; m++) {
@@ -634,6 +741,7 @@ __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
     }
     constexpr int KB = RP == 1 ? 1 : RP / 2;      // groups of 32 ranks (one of 16)
     constexpr int W = RP == 1 ? 4 : 8;            // ranks of a lane
+    constexpr int LP = QM_LORA_PITCH(RP);
     const int kb = RP == 1 ? (rank > 0) : (rank + 31) / 32;
     auto load = [](const uint16_t *p, uint32_t (&f)[W / 2]) {
         if constexpr (W == 8) {
@@ -650,7 +758,7 @@ __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
 #pragma unroll
         for (int n = 0; n < 4; n++)   // (a column behind the last one: any other, the result is not stored)
             if (k < kb) load(s.wt + ((int64_t)t.slot * s.cols + min(c0 + n * 8 + g, s.cols - 1)) * a.rpad + k * 32 + W * q, fb[k][n]);
-    const uint16_t *low = a.side[1 - a.out_side].low + ((int64_t)t.first + g) * a.rpad + W * q;
+    const uint16_t *low = a.side[1 - a.out_side].low + ((int64_t)t.row + g) * LP + W * q;
 #pragma unroll
     for (int m = 0; m < 4; m++) {
         if (m >= mt) break;
@@ -659,15 +767,15 @@ __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
         for (int n = 0; n < 4; n++)
 #pragma unroll
             for (int k = 0; k < 4; k++) d[n][k] = 0.f;
-        const uint16_t *lm = low + (int64_t)m * 16 * a.rpad;
+        const uint16_t *lm = low + m * 16 * LP;
 #pragma unroll
         for (int k = 0; k < KB; k++)
             if (k < kb) {
 #pragma unroll
                 for (int p = 2; p >= 0; p--) {   // the small parts first
                     uint32_t u0[W / 2], u1[W / 2];
-                    load(lm + p * a.plane + k * 32, u0);
-                    load(lm + p * a.plane + 8 * a.rpad + k * 32, u1);
+                    load(lm + p * RP * 16 + k * 32, u0);
+                    load(lm + p * RP * 16 + 8 * LP + k * 32, u1);
 #pragma unroll
                     for (int j = 0; j < W / 4; j++) {
                         const uint32_t fa[4] = {u0[2 * j], u1[2 * j], u0[2 * j + 1], u1[2 * j + 1]};
@@ -713,185 +821,156 @@ __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
 }
 
 // ---- outer ---------------------------------------------------------------------------------------------------------------
-// Gradient of one slot's A (or B): a cluster of `split` CTAs takes 128 columns, each CTA a range of the slot's tokens in
-// stages; both operands lie token by token and enter through transposing ldmatrix. Up to 32 ranks four groups of warps share
-// a stage's tokens, each with all ranks and half of the columns, so that little is read from shared memory twice; more ranks
-// share the groups. The sums of the groups and of the CTAs are added in a fixed order.
+// Gradient of one slot's A (or B): a cluster of `split` CTAs takes a block of columns, the CTAs taking turns over the slot's
+// tokens, 64 per stage. Both operands lie token by token, which is along M and N: M = the three parts of the ranks side by
+// side, as they lie in the workspace, so one product takes all of them, N = the columns. 32 tokens that are neighbours come
+// as boxes, others by their numbers; behind the slot's last token come zeros. The parts, and the CTAs' sums, are added in a
+// fixed order.
 template <int RP>
-__device__ __forceinline__ void outer(const QmLoraBatchArgs &a) {
-    wait_for_inputs();
-    extern __shared__ __align__(128) unsigned char smem[];
+__device__ __forceinline__ void outer(const QmLoraTcArgs &ta) {
+    const QmLoraBatchArgs &a = ta.b;
+    extern __shared__ unsigned char smem_raw[];
+    constexpr int R = RP * 16, G = QM_LORA_PITCH(RP) / 64, BN = QM_LORA_OUTER_COLS(RP), NG = BN / 64;
+    constexpr int AB = G * 8192, STAGE = AB + NG * 8192, STAGES = QM_LORA_OUTER_STAGES(RP);
+    constexpr int MM = (G + 1) / 2;                       // products of M = 128
+    constexpr int NACC = 2 * MM * BN <= 512 ? 2 : 1;
+    constexpr int READERS = QM_LORA_OUTER_READERS(RP), THREADS = (READERS + 2) * 32;
+    constexpr int MINE = MM * BN / (READERS / 4);         // columns of the accumulators that a reading warp adds up
+    constexpr int TCOLS = 512;
+    unsigned char *smem = reinterpret_cast<unsigned char *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const Pipe pipe = pipe_open<STAGES>(smem + STAGES * STAGE, TCOLS, READERS);
     const int me = a.split > 1 ? (int)cluster_rank() : 0;
     const int which = blockIdx.x / (a.outer_units * a.split), unit = blockIdx.x / a.split - which * a.outer_units;
     const QmLoraSide &s = a.side[which];
-    const int blocks = (s.cols + 127) / 128;
-    if (!s.grad || unit >= blocks * a.slots) return;   // the whole cluster
-    const int slot = unit / blocks, n0 = (unit % blocks) * 128;
-    const uint16_t *low = a.side[1 - which].low;
-    const int rank = a.rank[slot], r16 = (rank + 15) & ~15;
-    int first = 0, count = 0;
-    if (rank > 0) {
-        if (a.list) {
-            first = a.offsets[slot];
-            count = a.offsets[slot + 1] - first;
-        } else if (slot == 0) {
-            count = a.tokens;
-        }
-    }
-    constexpr int R = RP * 16, TB = QM_LORA_OUTER_TOKENS(RP), STAGES = QM_LORA_OUTER_STAGES(RP);
-    constexpr int XB = TB * 256, STAGE = XB + 3 * TB * R * 2;
-    constexpr int WM = RP <= 2 ? 1 : RP / 2, WN = 2, WK = 4 / WM;   // warps by rank, by column and by token
-    constexpr int MT = RP / WM, NT = 8, SL = TB / 16 / WK;
-    const int chunks = (count + TB - 1) / TB, per = (chunks + a.split - 1) / a.split;
-    const int c0 = min(me * per, chunks), cn = min(per, chunks - c0);
-    const int wm = warp % WM, wn = warp / WM % WN, wk = warp / (WM * WN);
-    const uint32_t base = smem_u32(smem);
-    // tokens of the stage that is fetched next: thread's rows tid / 16 + 16 i
-    int64_t tok[TB / 16];
-    auto tokens_of = [&](int chunk) {
-#pragma unroll
-        for (int i = 0; i < TB / 16; i++) {
-            const int p = (c0 + chunk) * TB + (tid >> 4) + 16 * i;
-            tok[i] = chunk < cn && p < count ? token_at(a, first + p) : -1;
-        }
-    };
-    auto fetch = [&](int chunk) {
-        if (chunk < cn) {
-            const uint32_t st = base + (chunk % STAGES) * STAGE;
-            const int p0 = (c0 + chunk) * TB;
-            const int piece = tid & 15;
-#pragma unroll
-            for (int i = 0; i < TB / 16; i++) {
-                const int row = (tid >> 4) + 16 * i;
-                const int left = tok[i] >= 0 ? max(0, min(16, (s.cols - n0 - piece * 8) * 2)) : 0;
-                copy16(st + row * 256 + ((piece ^ (row & 7)) * 16), s.x + (left ? tok[i] * s.ldx + n0 + piece * 8 : 0), left);
-            }
-            constexpr int PIECES = R / 8;   // of a row of one plane
-#pragma unroll
-            for (int i = 0; i < (3 * TB * PIECES + 255) / 256; i++) {
-                const int e = tid + 256 * i;
-                if (3 * TB * PIECES % 256 && e >= 3 * TB * PIECES) break;
-                const int plane = e / (TB * PIECES), row = (e / PIECES) % TB, piece2 = e % PIECES;
-                const bool in = p0 + row < count && piece2 * 8 < r16;
-                // rows of 32, 64, 128 or 256 bytes: eight rows on eight bank groups
-                const int sw = PIECES >= 8 ? piece2 ^ (row & 7) : PIECES == 4 ? piece2 ^ ((row >> 1) & 3) : piece2 ^ ((row >> 2) & 1);
-                copy16(st + XB + (plane * TB + row) * (R * 2) + sw * 16,
-                       low + plane * a.plane + ((int64_t)first + (in ? p0 + row : 0)) * a.rpad + (in ? piece2 * 8 : 0), in ? 16 : 0);
+    const int blocks = (s.cols + BN - 1) / BN;
+    if (s.grad && unit < blocks * a.slots) {   // the same for the whole cluster
+        const int slot = unit / blocks, n0 = (unit % blocks) * BN;
+        const int rank = a.rank[slot];
+        int first = 0, count = 0, row = 0;
+        if (rank > 0) {
+            if (a.list) {
+                first = a.offsets[slot];
+                count = a.offsets[slot + 1] - first;
+                row = a.offsets[a.slots + 2 + slot];
+            } else if (slot == 0) {
+                count = a.tokens;
             }
         }
-        copy_commit();
-    };
-    float acc[MT][NT][4];
+        const int chunks = (count + 63) / 64, cn = max(0, (chunks - me + a.split - 1) / a.split);
+        const uint32_t base = smem_u32(smem);
+        float *part = reinterpret_cast<float *>(smem);   // [R][BN + 4], over the stages once they are done
+        constexpr int LD = BN + 4;
+        float v[MINE];
+        if (warp == READERS) {
+            // lanes 0..15: the tokens of four rows of a block; asked for four blocks ahead
+            constexpr int AHEAD = 4;
+            int rows[AHEAD][4];
+            auto ask = [&](int c, int (&r)[4]) {
+                const int p = (c * a.split + me) * 64 + 4 * (lane & 15);
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+                for (int i = 0; i < 4; i++) r[i] = c < cn && p + i < count ? token_at(a, first + p + i) : a.tokens;
+            };
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+            for (int u = 0; u < AHEAD; u++) ask(u, rows[u]);
+            bool ok = true;
+            for (int c4 = 0; c4 < cn && ok; c4 += AHEAD)
 #pragma unroll
-            for (int k = 0; k < 4; k++) acc[m][n][k] = 0.f;
-    tokens_of(0);
+                for (int u = 0; u < AHEAD; u++) {
+                    const int c = c4 + u, st = c % STAGES;
+                    if (c >= cn || !ok) break;
+                    const bool box = neighbours(rows[u], 4);
+                    if (c >= STAGES && !qm::mbar_wait_bounded(pipe.empty + 8 * st, (uint32_t)(c / STAGES - 1) & 1u)) {
+                        if (lane == 0) atomicOr(a.status, QM_STATUS_TIMEOUT);
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t at = base + st * STAGE, bar = pipe.full + 8 * st;
+                    if (lane == 0) qm::mbar_expect_tx(bar, STAGE);
+                    __syncwarp();
+                    if (lane >= 16 && lane < 16 + G) tma_box(at + (lane - 16) * 8192, &ta.low[1 - which], 64 * (lane - 16), row + (c * a.split + me) * 64, bar);
+                    if (lane < 16) {
+                        if (!box) {
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; i++) {
-        fetch(i);
-        tokens_of(i + 1);
-    }
-    for (int c = 0; c < cn; c++) {
-        copy_wait<STAGES - 2>();
-        __syncthreads();
-        fetch(c + STAGES - 1);
-        tokens_of(c + STAGES);
-        const uint32_t st = base + (c % STAGES) * STAGE;
-        if (wm * MT * 16 < r16) {
+                            for (int j = 0; j < NG; j++) tma_rows4(at + AB + j * 8192 + lane * 512, &ta.gather[which], n0 + 64 * j, rows[u], bar);
+                        } else if ((lane & 7) == 0) {
 #pragma unroll
-            for (int sl = 0; sl < SL; sl++) {
-                const int t0 = (wk * SL + sl) * 16;
-                uint32_t fb[NT / 2][4];
-#pragma unroll
-                for (int n = 0; n < NT / 2; n++) {
-                    const int row = t0 + (lane & 15);
-                    ldsm4_t(st + row * 256 + ((wn * NT + 2 * n + (lane >> 4)) ^ (row & 7)) * 16, fb[n]);
-                }
-#pragma unroll
-                for (int m = 0; m < MT; m++)
-#pragma unroll
-                    for (int p = 2; p >= 0; p--) {   // the small parts first
-                        constexpr int PIECES = R / 8;
-                        uint32_t fa[4];
-                        const int row = t0 + (lane >> 4) * 8 + (lane & 7), piece = (wm * MT + m) * 2 + ((lane >> 3) & 1);
-                        const int sw = PIECES >= 8 ? piece ^ (row & 7) : PIECES == 4 ? piece ^ ((row >> 1) & 3) : piece ^ ((row >> 2) & 1);
-                        ldsm4_t(st + XB + (p * TB + row) * (R * 2) + sw * 16, fa);
-#pragma unroll
-                        for (int n = 0; n < NT / 2; n++) {
-                            mma(acc[m][2 * n], fa, fb[n][0], fb[n][1]);
-                            mma(acc[m][2 * n + 1], fa, fb[n][2], fb[n][3]);
+                            for (int j = 0; j < NG; j++) tma_box(at + AB + j * 8192 + lane * 512, &ta.rows[which], n0 + 64 * j, rows[u][0], bar);
                         }
                     }
-            }
+                    __syncwarp();
+                    ask(c + AHEAD, rows[u]);
+                }
+        } else if (warp == READERS + 1) {
+            if (lane == 0)
+                pipe_multiply<STAGES, NACC>(pipe, base, STAGE, cn, a.status, [&](uint32_t at, int acc, bool begin) {
+                    const uint64_t x = tile_desc(at + AB, 8192);
+#pragma unroll
+                    for (int m = 0; m < MM; m++) {
+                        // (a half without a partner is taken twice; the second half of the result is not read)
+                        const uint64_t l = tile_desc(at + m * 16384, 2 * m + 1 < G ? 8192 : 0);
+#pragma unroll
+                        for (int k = 0; k < 4; k++)   // 16 tokens = 2048 bytes = 128 descriptor units
+                            tc_mma(pipe.tmem + acc * MM * BN + m * BN, l + 128 * k, x + 128 * k, tc_idesc(BN, true), !begin || k > 0);
+                    }
+                });
+        } else {
+            pipe_read<MINE, NACC>(pipe, MM * BN, (warp >> 2) * MINE, cn, a.status, v);
         }
-    }
-    copy_wait<0>();
-    __syncthreads();
-    float *part = reinterpret_cast<float *>(smem);   // [WK][R][132]
-    constexpr int LD = 132;
-    {
-        const int g = lane >> 2, q = (lane & 3) * 2;
+        // row m of the accumulators is rank m % R of part m / R: the smallest part first, the others onto it
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+        for (int p = 2; p >= 0; p--) {
+            __syncthreads();   // before the first: nothing uses the stages any more
+            if (warp < READERS) {
+                const int c = (warp >> 2) * MINE, m = c / BN, j = c % BN;   // this warp's columns lie in one product
+                const int at = m * 128 + (warp & 3) * 32 + lane - p * R;    // this lane's rank, if it holds one of this part
+                if (at >= 0 && at < R) {
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                float *p = part + (wk * R + (wm * MT + m) * 16 + g) * LD + (wn * NT + n) * 8 + q;
-                *reinterpret_cast<float2 *>(p) = make_float2(acc[m][n][0], acc[m][n][1]);
-                *reinterpret_cast<float2 *>(p + 8 * LD) = make_float2(acc[m][n][2], acc[m][n][3]);
+                    for (int i = 0; i < MINE; i += 4) {
+                        float4 *q = reinterpret_cast<float4 *>(part + at * LD + j + i);
+                        float4 z = p == 2 ? make_float4(0.f, 0.f, 0.f, 0.f) : *q;
+                        z.x += v[i]; z.y += v[i + 1]; z.z += v[i + 2]; z.w += v[i + 3];
+                        *q = z;
+                    }
+                }
             }
-    }
-    __syncthreads();
-    if (WK > 1) {
-        for (int e = tid; e < R * 64; e += 256) {
-            float *p = part + (e >> 6) * LD + (e & 63) * 2;
-            float2 v = *reinterpret_cast<float2 *>(p);
-#pragma unroll
-            for (int k = 1; k < WK; k++) {
-                const float2 o = *reinterpret_cast<const float2 *>(p + k * R * LD);
-                v.x += o.x;
-                v.y += o.y;
-            }
-            *reinterpret_cast<float2 *>(p) = v;
         }
         __syncthreads();
-    }
-    if (a.split > 1) {
-        cluster_arrive();
-        cluster_wait();
-    }
-    // neighbouring threads take neighbours of the gradient's inner axis: columns of A, ranks of B
-    float *grad = s.grad + slot * s.grad_slot;
-    const int total = a.max_rank * 128, share = (total + a.split - 1) / a.split;
-    for (int e = me * share + tid; e < min(total, (me + 1) * share); e += 256) {
-        const int r = s.grad_col == 1 ? e >> 7 : e % a.max_rank, col = s.grad_col == 1 ? e & 127 : e / a.max_rank;
-        if (n0 + col >= s.cols) continue;
-        float v = 0.f;
-        if (r < rank && count > 0) {
-            const uint32_t at = smem_u32(part + r * LD + col);
-            if (a.split > 1) {
-                for (int k = 0; k < a.split; k++) v += peer_f32(peer_addr(at, k));
-            } else {
-                v = part[r * LD + col];
-            }
+        if (a.split > 1) {
+            cluster_arrive();
+            cluster_wait();
         }
-        grad[r * s.grad_rank + (n0 + col) * s.grad_col] = v;
+        // neighbouring threads take neighbours of the gradient's inner axis: columns of A, ranks of B
+        float *grad = s.grad + slot * s.grad_slot;
+        const int total = a.max_rank * BN, share = (total + a.split - 1) / a.split;
+        for (int e = me * share + tid; e < min(total, (me + 1) * share); e += THREADS) {
+            const int r = s.grad_col == 1 ? e / BN : e % a.max_rank, col = s.grad_col == 1 ? e % BN : e / a.max_rank;
+            if (n0 + col >= s.cols) continue;
+            float w = 0.f;
+            if (r < rank && count > 0) {
+                const uint32_t at = smem_u32(part + r * LD + col);
+                if (a.split > 1) {
+                    for (int k = 0; k < a.split; k++) w += peer_f32(peer_addr(at, k));
+                } else {
+                    w = part[r * LD + col];
+                }
+            }
+            grad[r * s.grad_rank + (n0 + col) * s.grad_col] = w;
+        }
+        if (a.split > 1) {
+            cluster_arrive();
+            cluster_wait();
+        }
     }
-    if (a.split > 1) {
-        cluster_arrive();
-        cluster_wait();
-    }
+    pipe_close(pipe, TCOLS);
 }
 
 }  // namespace
 
-extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_shrink_r16(const __grid_constant__ QmLoraBatchArgs a) { shrink<1>(a); }
-extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_shrink_r32(const __grid_constant__ QmLoraBatchArgs a) { shrink<2>(a); }
-extern "C" __global__ void __launch_bounds__(256) qm_lora_shrink_r64(const __grid_constant__ QmLoraBatchArgs a) { shrink<4>(a); }
-extern "C" __global__ void __launch_bounds__(256) qm_lora_shrink_r128(const __grid_constant__ QmLoraBatchArgs a) { shrink<8>(a); }
+extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r16(const __grid_constant__ QmLoraTcArgs a) { shrink<1>(a); }
+extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r32(const __grid_constant__ QmLoraTcArgs a) { shrink<2>(a); }
+extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r64(const __grid_constant__ QmLoraTcArgs a) { shrink<4>(a); }
+extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r128(const __grid_constant__ QmLoraTcArgs a) { shrink<8>(a); }
 extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r16(const __grid_constant__ QmLoraBatchArgs a) { expand<1, true>(a); }
 extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r16_s(const __grid_constant__ QmLoraBatchArgs a) { expand<1, false>(a); }
 extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r32(const __grid_constant__ QmLoraBatchArgs a) { expand<2, true>(a); }
@@ -900,7 +979,7 @@ extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r64(const __
 extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r64_s(const __grid_constant__ QmLoraBatchArgs a) { expand<4, false>(a); }
 extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_expand_r128(const __grid_constant__ QmLoraBatchArgs a) { expand<8, true>(a); }
 extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_expand_r128_s(const __grid_constant__ QmLoraBatchArgs a) { expand<8, false>(a); }
-extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_outer_r16(const __grid_constant__ QmLoraBatchArgs a) { outer<1>(a); }
-extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_outer_r32(const __grid_constant__ QmLoraBatchArgs a) { outer<2>(a); }
-extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_outer_r64(const __grid_constant__ QmLoraBatchArgs a) { outer<4>(a); }
-extern "C" __global__ void __launch_bounds__(256) qm_lora_outer_r128(const __grid_constant__ QmLoraBatchArgs a) { outer<8>(a); }
+extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(1) + 2) * 32) qm_lora_outer_r16(const __grid_constant__ QmLoraTcArgs a) { outer<1>(a); }
+extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(2) + 2) * 32) qm_lora_outer_r32(const __grid_constant__ QmLoraTcArgs a) { outer<2>(a); }
+extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(4) + 2) * 32) qm_lora_outer_r64(const __grid_constant__ QmLoraTcArgs a) { outer<4>(a); }
+extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(8) + 2) * 32) qm_lora_outer_r128(const __grid_constant__ QmLoraTcArgs a) { outer<8>(a); }
