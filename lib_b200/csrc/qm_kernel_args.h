@@ -411,7 +411,7 @@ struct QmGainSumArgs {
 
 // Low-rank adapters beside a stored projection (qm_lora.cu). A slot's A lies as [rpad][cols] and as [cols][rpad], its B as
 // [rpad][np], np = rows rounded up to 8, and as [rows][rpad], all bf16, ranks past the slot's own and columns past `rows`
-// zero.
+// zero; the [..][rpad] forms have their ranks in the order of the fragments that are read from them (qm_lora_set).
 #define QM_LORA_TILE 128     // tokens of one tile: neighbours in the order by adapter
 #define QM_LORA_BLOCK 64     // a group of tokens starts at a multiple of this in the workspace
 #define QM_LORA_CLUSTER 8    // CTAs that share the rows of one adapter (qm_lora_rows)
@@ -422,6 +422,7 @@ struct QmGainSumArgs {
 #define QM_LORA_PITCH(rp) ((48 * (rp) + 63) / 64 * 64)
 #define QM_LORA_SHRINK_STAGES(rp) ((rp) <= 2 ? 5 : (rp) == 4 ? 4 : 3)
 #define QM_LORA_OUTER_STAGES(rp) ((rp) == 8 ? 3 : (rp) == 4 ? 5 : 4)
+#define QM_LORA_EXPAND_ROW(rp) (96 * (rp) + 16)   // bytes of a token's narrow products in expand's shared memory
 #define QM_LORA_OUTER_COLS(rp) ((rp) <= 2 ? 256 : 128)
 #define QM_LORA_OUTER_READERS(rp) ((rp) == 8 ? 12 : 8)
 

@@ -237,7 +237,7 @@ static int32_t lists_launch(qm_ctx *c, const qm_lora *l, uint64_t ids_dev, int32
     a.tokens = tokens;
     a.slots = l->slots;
     a.tiles_max = (int32_t)lora_tiles(l, tokens, true);
-    return qm_launch(c, QM_K_LORA_LISTS, 1, 1, 1024, (unsigned)((32 * (l->slots + 1) + 1536) * 4), &a, true);
+    return qm_launch(c, QM_K_LORA_LISTS, 1, 1, 1024, (unsigned)((32 * (l->slots + 1) + 1536) * 4 + 256), &a, true);
 }
 
 static int32_t batch_args(qm_ctx *c, QmLoraTcArgs *ta, const qm_lora *l, uint64_t x, int64_t ldx, uint64_t dy, int64_t lddy, uint64_t ids_dev,
@@ -308,7 +308,7 @@ static int32_t expand_launch(qm_ctx *c, const qm_lora *l, QmLoraBatchArgs *a, in
     a->ldy = ldy;
     const bool vec = !((base | y) & 15) && !((ldb | ldy) & 3) && a->side[out_side].cols % 4 == 0;
     return qm_launch(c, (vec ? QM_K_LORA_EXPAND_R16 : QM_K_LORA_EXPAND_R16_S) + rank_kernel(l), (unsigned)(2 * a->tiles_max),
-                     (unsigned)((a->side[out_side].cols + 255) / 256), 256, 65536, a, true);
+                     (unsigned)((a->side[out_side].cols + 255) / 256), 256, (unsigned)(65536 + 64 * QM_LORA_EXPAND_ROW(l->rpad / 16)), a, true);
 }
 
 static int32_t batch_check(const qm_lora *l, uint64_t x, int64_t ldx, int32_t tokens, uint64_t ids_dev, uint64_t base, int64_t ldb,

@@ -57,6 +57,10 @@ template <int N>
 __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -143,9 +147,11 @@ extern "C" __global__ void __launch_bounds__(256) qm_lora_set(const __grid_const
                     *reinterpret_cast<uint32_t *>(by_rank + (int64_t)(r0 + r) * pitch + c0 + c) = *reinterpret_cast<const uint32_t *>(&tile[r][c]);
             }
             {
-                const int r = (e & 15) * 2, c = e >> 4;
-                if (r0 + r < a.rpad && c0 + c < cols)
-                    *reinterpret_cast<uint32_t *>(by_col + (int64_t)(c0 + c) * a.rpad + r0 + r) = tile[r][c] | (uint32_t)tile[r + 1][c] << 16;
+                // pairs of ranks in the order that expand's lanes take them: of 32 ranks (of 16, where there are no more)
+                // lane q reads the pairs q, q + 4, q + 8, ... as one piece
+                const int i2 = e & 15, c = e >> 4, groups = min(4, a.rpad / 8), r = (i2 % groups * 4 + i2 / groups) * 2;
+                if (r0 + 2 * i2 < a.rpad && c0 + c < cols)
+                    *reinterpret_cast<uint32_t *>(by_col + (int64_t)(c0 + c) * a.rpad + r0 + 2 * i2) = tile[r][c] | (uint32_t)tile[r + 1][c] << 16;
             }
         }
         __syncthreads();
@@ -339,20 +345,38 @@ extern "C" __global__ void __launch_bounds__(1024) qm_lora_lists(const __grid_co
     extern __shared__ int32_t hist[];   // [32][groups], then [512] tokens, tiles and workspace blocks up to and with the group
     const int groups = a.slots + 1, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int32_t *before = hist + 32 * groups, *tiles = before + 512, *blocks = tiles + 512;
-    for (int i = tid; i < 32 * groups; i += 1024) hist[i] = 0;
-    __syncthreads();
+    uint8_t *known = reinterpret_cast<uint8_t *>(blocks + 512);   // [256] slots that hold an adapter
     const int per = ((a.tokens + 31) / 32 + 31) & ~31;
     const int t0 = warp * per, t1 = min(t0 + per, a.tokens);
-    auto group_of = [&](int t) {
-        const int id = a.ids[t];
-        return id >= 0 && id < a.slots && a.rank[id] > 0 ? id : a.slots;
+    constexpr int AHEAD = 8;   // ids that a lane asks for at a time; the first ones stay in registers
+    int ids[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) ids[i] = t0 + 32 * i + lane < t1 ? a.ids[t0 + 32 * i + lane] : -1;
+    if (tid < a.slots) known[tid] = a.rank[tid] > 0;
+    for (int i = tid; i < 32 * groups; i += 1024) hist[i] = 0;
+    __syncthreads();
+    auto group_of = [&](int id) { return id >= 0 && id < a.slots && known[id] ? id : a.slots; };
+    // f(token of this lane, its group or -1, lanes of the same group), 32 tokens at a time
+    auto walk = [&](auto f) {
+        for (int t = t0; t < t1; t += 32 * AHEAD) {
+            int more[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                const int u = t + 32 * i + lane;
+                more[i] = t == t0 ? ids[i] : u < t1 ? a.ids[u] : -1;
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                if (t + 32 * i >= t1) break;
+                const int u = t + 32 * i + lane, g = u < t1 ? group_of(more[i]) : -1;
+                f(u, g, __match_any_sync(0xffffffffu, g));
+            }
+        }
     };
-    for (int t = t0; t < t1; t += 32) {
-        const int g = t + lane < t1 ? group_of(t + lane) : -1;
-        const uint32_t same = __match_any_sync(0xffffffffu, g);
+    walk([&](int, int g, uint32_t same) {
         if (g >= 0 && lane == __ffs(same) - 1) hist[warp * groups + g] += __popc(same);
         __syncwarp();
-    }
+    });
     __syncthreads();
     int total = 0;
     if (tid < groups)
@@ -386,18 +410,16 @@ extern "C" __global__ void __launch_bounds__(1024) qm_lora_lists(const __grid_co
         a.offsets[tid] = tid ? before[tid - 1] : 0;
         a.offsets[a.slots + 2 + tid] = tid ? blocks[tid - 1] * QM_LORA_BLOCK : 0;
     }
-    for (int t = t0; t < t1; t += 32) {
-        const int g = t + lane < t1 ? group_of(t + lane) : -1;
-        const uint32_t same = __match_any_sync(0xffffffffu, g);
+    walk([&](int u, int g, uint32_t same) {
         int at = 0;
         if (g >= 0) at = hist[warp * groups + g] + (g ? before[g - 1] : 0) + __popc(same & ((1u << lane) - 1));
         __syncwarp();
         if (g >= 0) {
-            a.list[at] = t + lane;
+            a.list[at] = u;
             if (lane == __ffs(same) - 1) hist[warp * groups + g] += __popc(same);
         }
         __syncwarp();
-    }
+    });
     const int ntiles = tiles[groups - 1];
     for (int i = tid; i < a.tiles_max; i += 1024) {
         int4 w = make_int4(-1, 0, 0, 0);
@@ -682,20 +704,24 @@ __device__ __forceinline__ void shrink(const QmLoraTcArgs &ta) {
 }
 
 // ---- expand --------------------------------------------------------------------------------------------------------------
-// A CTA takes half a tile's tokens x 256 columns, each of its eight warps 32 columns, without a barrier. All of base is asked for
-// at the start (cp.async into the warp's own shared memory, no registers held); the adapter's fragments of the columns stay
-// in registers while the warp goes through the tokens, 16 at a time. Both operands' fragments come straight from memory: the
-// order of the ranks inside a product is free, so a lane takes eight neighbouring ranks of its token and of its column as
-// one 16-byte load each. The products are added to base in shared memory and leave in rows of 128 bytes.
+// A CTA takes half a tile's tokens x 256 columns, each of its eight warps 32 columns. All of base is asked for at the start
+// (cp.async into the warp's own shared memory, no registers held), the tokens' narrow products once for the CTA; the
+// adapter's fragments of the columns stay in registers while the warp goes through the tokens, 16 at a time. The products
+// are added to base in shared memory and leave in rows of 128 bytes. Legacy mma on purpose: 16 to 128 ranks x 3 parts are too
+// little work to bound anything, and its fragments need neither tensor memory nor a second pass over the results.
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+// Place of column c (0..31) of row r in a warp's [16][32] floats: 16-byte pieces moved in pairs by the row, so that neither
+// the fragments' accesses (four rows x 32 bytes at a time) nor whole rows meet a bank twice.
+__device__ __forceinline__ int staged(int r, int c) { return r * 32 + (((c >> 2) ^ (2 * (r & 3))) << 2) + (c & 3); }
 
 template <int RP, bool VEC>
 __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
     wait_for_inputs();
-    extern __shared__ __align__(128) unsigned char smem[];   // [8 warps][4][16][32] floats, 16-byte pieces swizzled by the row
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    extern __shared__ __align__(128) unsigned char smem[];   // [8 warps][4][16][32] floats, then [64] rows of narrow products
+    constexpr int R = RP * 16, LP = QM_LORA_PITCH(RP), UB = QM_LORA_EXPAND_ROW(RP);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     Tile t = get_tile(a, blockIdx.x >> 1);
     if (blockIdx.x & 1) {
         t.first += 64;
@@ -706,34 +732,40 @@ __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
     if (t.count <= 0) return;
     const QmLoraSide &s = a.side[a.out_side];
     const int c0 = blockIdx.y * 256 + warp * 32;
-    if (c0 >= s.cols) return;
     const int rank = t.slot < 0 ? 0 : t.rank;
     if (rank == 0 && a.base == a.y) return;
     const int mt = (t.count + 15) >> 4;
     const int g = lane >> 2, q = lane & 3;
     float *own = reinterpret_cast<float *>(smem) + warp * 4 * 512;
-    // (tokens of the tile: lane holds two, row l and 32 + l)
+    const uint32_t low = smem_u32(smem) + 65536;
+    // the tokens' numbers: lane holds rows l and 32 + l
     const int tok0 = token_at(a, t.first + min(lane, t.count - 1)), tok1 = token_at(a, t.first + min(lane + 32, t.count - 1));
-    auto token = [&](int row) { return (int64_t)__shfl_sync(0xffffffffu, row < 32 ? tok0 : tok1, row & 31); };
+    if (rank > 0) {
+        const uint16_t *src = a.side[1 - a.out_side].low + (int64_t)t.row * LP;
+        for (int e = tid; e < mt * 16 * (6 * RP); e += 256) {   // rows of 3 R ranks: 6 RP pieces of 16 bytes
+            const int row = e / (6 * RP), piece = e % (6 * RP);
+            copy16(low + row * UB + piece * 16, src + row * LP + piece * 8, 16);
+        }
+    }
+    copy_commit();
+    const bool mine = c0 < s.cols;
 #pragma unroll
     for (int m = 0; m < 4; m++) {
-        if (m < mt) {
+        if (m < mt && mine) {
             if constexpr (VEC) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int r = (lane >> 3) + 4 * i, piece = lane & 7, c = c0 + 4 * piece;
-                    // the four rows of this step lie in one half of the tile
+                    const int r = (lane >> 3) + 4 * i, c = 4 * (lane & 7);
                     const int64_t row = __shfl_sync(0xffffffffu, m < 2 ? tok0 : tok1, (m & 1) * 16 + r);
-                    const bool in = a.base && m * 16 + r < t.count && c < s.cols;
-                    copy16(smem_u32(own + m * 512 + r * 32 + ((piece ^ (r & 7)) * 4)), in ? (const void *)(a.base + row * a.ldb + c) : (const void *)s.wt, in ? 16 : 0);
+                    const bool in = a.base && m * 16 + r < t.count && c0 + c < s.cols;
+                    copy16(smem_u32(own + m * 512 + staged(r, c)), in ? (const void *)(a.base + row * a.ldb + c0 + c) : (const void *)s.wt, in ? 16 : 0);
                 }
             } else {
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    const int64_t row = token(m * 16 + r);
+                    const int64_t row = __shfl_sync(0xffffffffu, m < 2 ? tok0 : tok1, (m & 1) * 16 + r);
                     const bool in = a.base && m * 16 + r < t.count && c0 + lane < s.cols;
-                    copy4(smem_u32(own + m * 512 + r * 32 + (((lane >> 2) ^ (r & 7)) * 4) + (lane & 3)),
-                          in ? (const void *)(a.base + row * a.ldb + c0 + lane) : (const void *)s.wt, in ? 4 : 0);
+                    copy4(smem_u32(own + m * 512 + staged(r, lane)), in ? (const void *)(a.base + row * a.ldb + c0 + lane) : (const void *)s.wt, in ? 4 : 0);
                 }
             }
         }
@@ -741,24 +773,25 @@ __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
     }
     constexpr int KB = RP == 1 ? 1 : RP / 2;      // groups of 32 ranks (one of 16)
     constexpr int W = RP == 1 ? 4 : 8;            // ranks of a lane
-    constexpr int LP = QM_LORA_PITCH(RP);
     const int kb = RP == 1 ? (rank > 0) : (rank + 31) / 32;
-    auto load = [](const uint16_t *p, uint32_t (&f)[W / 2]) {
-        if constexpr (W == 8) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(p);
-            f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
-        } else {
-            const uint2 v = *reinterpret_cast<const uint2 *>(p);
-            f[0] = v.x; f[1] = v.y;
-        }
-    };
     uint32_t fb[KB][4][W / 2];
 #pragma unroll
     for (int k = 0; k < KB; k++)
 #pragma unroll
         for (int n = 0; n < 4; n++)   // (a column behind the last one: any other, the result is not stored)
-            if (k < kb) load(s.wt + ((int64_t)t.slot * s.cols + min(c0 + n * 8 + g, s.cols - 1)) * a.rpad + k * 32 + W * q, fb[k][n]);
-    const uint16_t *low = a.side[1 - a.out_side].low + ((int64_t)t.row + g) * LP + W * q;
+            if (k < kb) {
+                const uint16_t *p = s.wt + ((int64_t)t.slot * s.cols + min(c0 + n * 8 + g, s.cols - 1)) * R + k * 32 + W * q;
+                if constexpr (W == 8) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+                    fb[k][n][0] = v.x; fb[k][n][1] = v.y; fb[k][n][2] = v.z; fb[k][n][3] = v.w;
+                } else {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+                    fb[k][n][0] = v.x; fb[k][n][1] = v.y;
+                }
+            }
+    copy_wait<4>();
+    __syncthreads();
+    if (!mine) return;
 #pragma unroll
     for (int m = 0; m < 4; m++) {
         if (m >= mt) break;
@@ -767,22 +800,19 @@ __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
         for (int n = 0; n < 4; n++)
 #pragma unroll
             for (int k = 0; k < 4; k++) d[n][k] = 0.f;
-        const uint16_t *lm = low + m * 16 * LP;
+        const uint32_t lm = low + (m * 16 + (lane & 15)) * UB + (lane >> 4) * 16;
 #pragma unroll
         for (int k = 0; k < KB; k++)
             if (k < kb) {
 #pragma unroll
-                for (int p = 2; p >= 0; p--) {   // the small parts first
-                    uint32_t u0[W / 2], u1[W / 2];
-                    load(lm + p * RP * 16 + k * 32, u0);
-                    load(lm + p * RP * 16 + 8 * LP + k * 32, u1);
+                for (int p = 2; p >= 0; p--)   // the small parts first
 #pragma unroll
                     for (int j = 0; j < W / 4; j++) {
-                        const uint32_t fa[4] = {u0[2 * j], u1[2 * j], u0[2 * j + 1], u1[2 * j + 1]};
+                        uint32_t fa[4];
+                        ldsm4(lm + (p * R + k * 32 + j * 16) * 2, fa);
 #pragma unroll
                         for (int n = 0; n < 4; n++) mma(d[n], fa, fb[k][n][2 * j], fb[k][n][2 * j + 1]);
                     }
-                }
             }
         if (m == 0) copy_wait<3>();
         else if (m == 1) copy_wait<2>();
@@ -793,8 +823,8 @@ __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
 #pragma unroll
         for (int n = 0; n < 4; n++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {   // rows g and g + 8 share their swizzle
-                float2 *p = reinterpret_cast<float2 *>(st + (g + 8 * h) * 32 + (((2 * n + (q >> 1)) ^ g) * 4) + (q & 1) * 2);
+            for (int h = 0; h < 2; h++) {
+                float2 *p = reinterpret_cast<float2 *>(st + staged(g + 8 * h, n * 8 + 2 * q));
                 float2 v = *p;
                 v.x += d[n][2 * h];
                 v.y += d[n][2 * h + 1];
@@ -804,16 +834,16 @@ __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
         if constexpr (VEC) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int r = (lane >> 3) + 4 * i, piece = lane & 7, c = c0 + 4 * piece;
+                const int r = (lane >> 3) + 4 * i, c = 4 * (lane & 7);
                 const int64_t row = __shfl_sync(0xffffffffu, m < 2 ? tok0 : tok1, (m & 1) * 16 + r);
-                const float4 v = *reinterpret_cast<const float4 *>(st + r * 32 + ((piece ^ (r & 7)) * 4));
-                if (m * 16 + r < t.count && c < s.cols) *reinterpret_cast<float4 *>(a.y + row * a.ldy + c) = v;
+                const float4 v = *reinterpret_cast<const float4 *>(st + staged(r, c));
+                if (m * 16 + r < t.count && c0 + c < s.cols) *reinterpret_cast<float4 *>(a.y + row * a.ldy + c0 + c) = v;
             }
         } else {
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                const int64_t row = token(m * 16 + r);
-                const float v = st[r * 32 + (((lane >> 2) ^ (r & 7)) * 4) + (lane & 3)];
+                const int64_t row = __shfl_sync(0xffffffffu, m < 2 ? tok0 : tok1, (m & 1) * 16 + r);
+                const float v = st[staged(r, lane)];
                 if (m * 16 + r < t.count && c0 + lane < s.cols) a.y[row * a.ldy + c0 + lane] = v;
             }
         }
@@ -975,8 +1005,8 @@ extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r16(const __
 extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r16_s(const __grid_constant__ QmLoraBatchArgs a) { expand<1, false>(a); }
 extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r32(const __grid_constant__ QmLoraBatchArgs a) { expand<2, true>(a); }
 extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r32_s(const __grid_constant__ QmLoraBatchArgs a) { expand<2, false>(a); }
-extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r64(const __grid_constant__ QmLoraBatchArgs a) { expand<4, true>(a); }
-extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r64_s(const __grid_constant__ QmLoraBatchArgs a) { expand<4, false>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_expand_r64(const __grid_constant__ QmLoraBatchArgs a) { expand<4, true>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_expand_r64_s(const __grid_constant__ QmLoraBatchArgs a) { expand<4, false>(a); }
 extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_expand_r128(const __grid_constant__ QmLoraBatchArgs a) { expand<8, true>(a); }
 extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_expand_r128_s(const __grid_constant__ QmLoraBatchArgs a) { expand<8, false>(a); }
 extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(1) + 2) * 32) qm_lora_outer_r16(const __grid_constant__ QmLoraTcArgs a) { outer<1>(a); }
