@@ -131,9 +131,11 @@ static const KernelName kKernels[QM_K_COUNT] = {
     {QM_MOD_LORA, "qm_lora_expand_r32"}, {QM_MOD_LORA, "qm_lora_expand_r64"}, {QM_MOD_LORA, "qm_lora_expand_r128"},
     {QM_MOD_LORA, "qm_lora_expand_r16_s"}, {QM_MOD_LORA, "qm_lora_expand_r32_s"}, {QM_MOD_LORA, "qm_lora_expand_r64_s"},
     {QM_MOD_LORA, "qm_lora_expand_r128_s"},
-    {QM_MOD_ROPE, "qm_qk_norm_w1"},    {QM_MOD_ROPE, "qm_qk_norm_w2"},    {QM_MOD_ROPE, "qm_qk_norm_w4"},
-    {QM_MOD_ROPE, "qm_qk_norm_s8"},    {QM_MOD_ROPE, "qm_qk_grad_w1"},    {QM_MOD_ROPE, "qm_qk_grad_w2"},
-    {QM_MOD_ROPE, "qm_qk_grad_w4"},    {QM_MOD_ROPE, "qm_qk_grad_s8"},    {QM_MOD_ROPE, "qm_qk_gain_sum"},
+    {QM_MOD_ROPE, "qm_qk_norm_w1"}, {QM_MOD_ROPE, "qm_qk_norm_w2"}, {QM_MOD_ROPE, "qm_qk_norm_w4"}, {QM_MOD_ROPE, "qm_qk_norm_s8"},
+    {QM_MOD_ROPE, "qm_qk_norm_w1_b"}, {QM_MOD_ROPE, "qm_qk_norm_w2_b"}, {QM_MOD_ROPE, "qm_qk_norm_w4_b"}, {QM_MOD_ROPE, "qm_qk_norm_s8_b"},
+    {QM_MOD_ROPE, "qm_qk_grad_w1"}, {QM_MOD_ROPE, "qm_qk_grad_w2"}, {QM_MOD_ROPE, "qm_qk_grad_w4"}, {QM_MOD_ROPE, "qm_qk_grad_s8"},
+    {QM_MOD_ROPE, "qm_qk_grad_w1_b"}, {QM_MOD_ROPE, "qm_qk_grad_w2_b"}, {QM_MOD_ROPE, "qm_qk_grad_w4_b"}, {QM_MOD_ROPE, "qm_qk_grad_s8_b"},
+    {QM_MOD_ROPE, "qm_qk_gain_sum"},
 };
 
 // ---- errors --------------------------------------------------------------------------

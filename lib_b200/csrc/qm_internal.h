@@ -38,8 +38,10 @@ enum {
     QM_K_LORA_SHRINK_R128, QM_K_LORA_OUTER_R16, QM_K_LORA_OUTER_R32, QM_K_LORA_OUTER_R64, QM_K_LORA_OUTER_R128,
     QM_K_LORA_EXPAND_R16, QM_K_LORA_EXPAND_R32, QM_K_LORA_EXPAND_R64, QM_K_LORA_EXPAND_R128,
     QM_K_LORA_EXPAND_R16_S, QM_K_LORA_EXPAND_R32_S, QM_K_LORA_EXPAND_R64_S, QM_K_LORA_EXPAND_R128_S,
-    QM_K_QK_NORM_W1, QM_K_QK_NORM_W2, QM_K_QK_NORM_W4, QM_K_QK_NORM_S8, QM_K_QK_GRAD_W1, QM_K_QK_GRAD_W2, QM_K_QK_GRAD_W4,
-    QM_K_QK_GRAD_S8, QM_K_QK_GAIN_SUM, QM_K_COUNT
+    QM_K_QK_NORM_W1, QM_K_QK_NORM_W2, QM_K_QK_NORM_W4, QM_K_QK_NORM_S8,
+    QM_K_QK_NORM_W1_B, QM_K_QK_NORM_W2_B, QM_K_QK_NORM_W4_B, QM_K_QK_NORM_S8_B,
+    QM_K_QK_GRAD_W1, QM_K_QK_GRAD_W2, QM_K_QK_GRAD_W4, QM_K_QK_GRAD_S8,
+    QM_K_QK_GRAD_W1_B, QM_K_QK_GRAD_W2_B, QM_K_QK_GRAD_W4_B, QM_K_QK_GRAD_S8_B, QM_K_QK_GAIN_SUM, QM_K_COUNT
 };
 
 #define QM_GEMV_SMEM_MAX (227 * 1024)

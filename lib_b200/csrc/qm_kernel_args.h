@@ -396,10 +396,9 @@ struct QmQkArgs {
     float *partial;          // backward: [CTAs][2][dim] sums of the gains' gradients, or null
     int64_t ldx, ldq, ldk, lddx;
     int32_t tokens, hq, hk, dim, rot;
-    int32_t interleaved, norm, bf16;
-    int32_t chunk, chunks;   // heads of one warp, and how many such groups a token has
+    int32_t interleaved, norm;
+    int32_t chunk, chunks, q_chunks;   // heads of one warp; how many such groups a token has, and its query heads
     float eps;
-    int32_t pad_;
 };
 
 // The gains' gradients from the CTAs' sums (qm_qk_gain_sum).

@@ -192,7 +192,7 @@ static int32_t rows_launch(qm_ctx *c, const qm_lora *l, uint64_t x_dev, uint64_t
     a.nsplit = (int32_t)std::max<int64_t>(1, std::min<int64_t>(most, c->sm_count / (QM_LORA_CLUSTER * m)));
     const int64_t ks = ((l->cols + QM_LORA_CLUSTER - 1) / QM_LORA_CLUSTER + 7) & ~(int64_t)7;
     const int64_t chunk = (int64_t)l->rpad * QM_LORA_CHUNK * 2;
-    const int64_t smem = 16ll * l->rpad * 4 + 136 * 4 + chunk + std::max<int64_t>(8 * ks * 4, 32 * QM_LORA_CHUNK * 4 + chunk);
+    const int64_t smem = 16ll * l->rpad * 4 + 8 * 4 + chunk + std::max<int64_t>(8 * ks * 4, 32 * QM_LORA_CHUNK * 4 + chunk);
     if (smem > QM_GEMV_SMEM_MAX) return QM_ERR_LIMIT;
     return qm_launch_ex(c, QM_K_LORA_ROWS, (unsigned)(m * a.nsplit * QM_LORA_CLUSTER), 512, (unsigned)smem, &a, true, false, QM_LORA_CLUSTER);
 }

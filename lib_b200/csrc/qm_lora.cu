@@ -161,8 +161,97 @@ extern "C" __global__ void __launch_bounds__(256) qm_lora_set(const __grid_const
 // ---- 1..8 float32 rows ---------------------------------------------------------------------------------------------------
 // One launch: a cluster of eight CTAs takes the rows of one adapter (the cluster of the first such row; the others leave at
 // once). Each CTA multiplies an eighth of x with its columns of A, the partial sums meet in distributed shared memory, and
-// each CTA then adds its own columns of B. `nsplit` clusters share the columns and repeat the first half. The first columns
-// of B are on their way to shared memory while A is read.
+// each CTA then adds its own columns of B. `nsplit` clusters share the columns and repeat the first half. At these sizes only
+// trips to memory count: the first columns of B and of base are on their way before A is read, and a warp asks for up to four
+// ranks of A at a time.
+namespace {
+
+struct RowsShared {
+    float *part;     // [8][rpad] this CTA's sums
+    float *u;        // [rpad][8]
+    float *ssq;      // [8]
+    uint16_t *b0, *b1;   // [rpad][CHUNK]
+    float *xs;       // [8][ks]; later the sums, then the second chunk of B
+    float *sums;     // [4][8][CHUNK]
+};
+
+// This CTA's columns of A with NR rows of x: a warp takes ranks warp, warp + 16, ..., four of them at a time.
+template <int NR>
+__device__ __forceinline__ void rows_narrow(const QmLoraRowsArgs &a, const RowsShared &sh, const uint16_t *w, int r, int nr, int ks, int kn) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int r0 = warp; r0 < r; r0 += 64) {
+        float acc[4][NR];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int i = 0; i < NR; i++) acc[j][i] = 0.f;
+#pragma unroll 2
+        for (int c = 8 * lane; c < kn; c += 256) {
+            uint4 q[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (r0 + 16 * j < r) q[j] = *reinterpret_cast<const uint4 *>(w + (int64_t)(r0 + 16 * j) * a.cols + c);
+#pragma unroll
+            for (int i = 0; i < NR; i++)
+                if (i < nr) {
+                    const float4 v = *reinterpret_cast<const float4 *>(sh.xs + i * ks + c), z = *reinterpret_cast<const float4 *>(sh.xs + i * ks + c + 4);
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (r0 + 16 * j < r)
+                            acc[j][i] += bf_lo(q[j].x) * v.x + bf_hi(q[j].x) * v.y + bf_lo(q[j].y) * v.z + bf_hi(q[j].y) * v.w + bf_lo(q[j].z) * z.x +
+                                         bf_hi(q[j].z) * z.y + bf_lo(q[j].w) * z.z + bf_hi(q[j].w) * z.w;
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (r0 + 16 * j < r) {
+#pragma unroll
+                for (int i = 0; i < NR; i++)
+                    if (i < nr) {
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) acc[j][i] += __shfl_xor_sync(0xffffffffu, acc[j][i], o);
+                        if (lane == 0) sh.part[i * a.rpad + r0 + 16 * j] = acc[j][i];
+                    }
+            }
+    }
+}
+
+// Sums over the ranks for one chunk of columns: four groups of 128 threads share the ranks, a thread has two columns.
+template <int NR>
+__device__ __forceinline__ void rows_wide(const RowsShared &sh, const uint16_t *b, int r, int nr) {
+    const int group = threadIdx.x >> 7, col2 = (threadIdx.x & 127) * 2;
+    float acc[NR][2];
+#pragma unroll
+    for (int i = 0; i < NR; i++) acc[i][0] = acc[i][1] = 0.f;
+#pragma unroll 4
+    for (int rr = group; rr < r; rr += 4) {
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(b + rr * QM_LORA_CHUNK + col2);
+        const float lo = bf_lo(w), hi = bf_hi(w);
+        float v[NR];
+        if constexpr (NR == 1) {
+            v[0] = sh.u[rr * 8];
+        } else {
+#pragma unroll
+            for (int i = 0; i < NR; i += 2) {
+                const float2 p = *reinterpret_cast<const float2 *>(sh.u + rr * 8 + i);
+                v[i] = p.x;
+                v[i + 1] = p.y;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NR; i++)
+            if (i < nr) {
+                acc[i][0] += v[i] * lo;
+                acc[i][1] += v[i] * hi;
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < NR; i++)
+        if (i < nr) *reinterpret_cast<float2 *>(sh.sums + (group * 8 + i) * QM_LORA_CHUNK + col2) = make_float2(acc[i][0], acc[i][1]);
+}
+
+}  // namespace
+
 extern "C" __global__ void __launch_bounds__(512) qm_lora_rows(const __grid_constant__ QmLoraRowsArgs a) {
     wait_for_inputs();
     extern __shared__ __align__(16) unsigned char smem[];
@@ -171,168 +260,140 @@ extern "C" __global__ void __launch_bounds__(512) qm_lora_rows(const __grid_cons
     const int row = cluster / a.nsplit, part = cluster % a.nsplit;
     const int np_cta = (((a.np + a.nsplit * QM_LORA_CLUSTER - 1) / (a.nsplit * QM_LORA_CLUSTER)) + 7) & ~7;
     const int n0 = min((part * QM_LORA_CLUSTER + me) * np_cta, a.rows), nn = min(np_cta, a.rows - n0);
-    int slot = a.ids ? a.ids[row] : 0;
-    const int r = slot >= 0 && slot < a.slots ? a.rank[slot] : 0;
+    const int id = a.ids && lane < a.m ? a.ids[lane] : 0;
+    const int slot = __shfl_sync(0xffffffffu, id, row);
+    const uint32_t same = __ballot_sync(0xffffffffu, lane < a.m && id == slot);   // the rows of this adapter
+    const bool named = slot >= 0 && slot < a.slots;
+    const int r = named ? a.rank[slot] : 0;
     if (r == 0) {   // no adapter
         if (a.base != a.y)
             for (int c = tid; c < nn; c += 512) a.y[row * a.ldy + n0 + c] = a.base ? a.base[row * a.ldb + n0 + c] : 0.f;
         return;
     }
-    int mine[8], nr = 0;   // the rows of this adapter
+    if (__ffs(same) - 1 < row) return;   // an earlier row's cluster has this one
+    const int nr = __popc(same);
+    auto row_of = [&](int i) {   // the i-th row of this adapter
+        uint32_t left = same;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const bool same = i < a.m && (a.ids ? a.ids[i] : 0) == slot;
-        if (same && i < row) return;   // an earlier row's cluster has this one
-        mine[i] = 0;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (i < a.m && (a.ids ? a.ids[i] : 0) == slot) {
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-                if (k == nr) mine[k] = i;
-            nr++;
-        }
+        for (int k = 0; k < 7; k++)
+            if (k < i) left &= left - 1;
+        return __ffs(left) - 1;
+    };
+    const float scale = a.scale[slot];
     const int ks = ((a.cols + QM_LORA_CLUSTER - 1) / QM_LORA_CLUSTER + 7) & ~7;
     const int k0 = min(me * ks, a.cols), kn = min(ks, a.cols - k0);
-    float *part_u = reinterpret_cast<float *>(smem);                 // [8][rpad]
-    float *u = part_u + 8 * a.rpad;                                  // [rpad][8]
-    float *ssq = u + 8 * a.rpad;                                     // [8] of this CTA, then [8][16] of the warps
-    uint16_t *b0 = reinterpret_cast<uint16_t *>(ssq + 8 + 128);      // [rpad][CHUNK]
-    float *xs = reinterpret_cast<float *>(b0 + a.rpad * QM_LORA_CHUNK);   // [8][ks]; later the sums, then the second chunk
-    float *sums = xs;                                                // [4][8][CHUNK]
-    uint16_t *b1 = reinterpret_cast<uint16_t *>(xs + 32 * QM_LORA_CHUNK);
+    RowsShared sh;
+    sh.part = reinterpret_cast<float *>(smem);
+    sh.u = sh.part + 8 * a.rpad;
+    sh.ssq = sh.u + 8 * a.rpad;
+    sh.b0 = reinterpret_cast<uint16_t *>(sh.ssq + 8);
+    sh.xs = sh.sums = reinterpret_cast<float *>(sh.b0 + a.rpad * QM_LORA_CHUNK);
+    sh.b1 = reinterpret_cast<uint16_t *>(sh.xs + 32 * QM_LORA_CHUNK);
     const uint16_t *wb = a.b + (int64_t)slot * a.rpad * a.np;
     auto fetch_b = [&](int chunk) {
         const int c0 = chunk * QM_LORA_CHUNK, units = (min(QM_LORA_CHUNK, nn - c0) + 7) / 8;
-        const uint32_t dst = smem_u32(chunk & 1 ? b1 : b0);
+        const uint32_t dst = smem_u32(chunk & 1 ? sh.b1 : sh.b0);
         for (int i = tid; i < r * (QM_LORA_CHUNK / 8); i += 512) {
             const int rr = i / (QM_LORA_CHUNK / 8), q = i % (QM_LORA_CHUNK / 8);
             if (q < units) copy16(dst + (rr * QM_LORA_CHUNK + q * 8) * 2, wb + (int64_t)rr * a.np + n0 + c0 + q * 8, 16);
         }
         copy_commit();
     };
+    // this thread's outputs of a chunk: rows tid / 256 + 2 i of the adapter's, column tid % 256
+    float base[4];
+    const int out_col = tid % QM_LORA_CHUNK, out_row = tid / QM_LORA_CHUNK;
+    auto fetch_base = [&](int chunk) {
+        const int c = chunk * QM_LORA_CHUNK + out_col;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            base[i] = 0.f;
+            if (a.base && out_row + 2 * i < nr && c < nn) base[i] = a.base[row_of(out_row + 2 * i) * a.ldb + n0 + c];
+        }
+    };
     if (nn > 0) fetch_b(0);
     // x, transformed as qm_matvec stages it; the scale of a norm is one factor per row and comes in at the end
     const bool norm = a.xop == 1 || a.xop == 2;
-    for (int i = 0; i < nr; i++) {
-        int xr = mine[0];
-#pragma unroll
-        for (int k = 1; k < 8; k++) xr = k == i ? mine[k] : xr;
-        const float *x = a.x + xr * a.ldx + k0, *x2 = a.x2 ? a.x2 + xr * a.ldx + k0 : nullptr;
-        float ss = 0.f;
-        for (int c = 4 * tid; c < kn; c += 2048) {
-            float4 v = *reinterpret_cast<const float4 *>(x + c);
-            if (a.xop >= 2) {
-                const float4 w = *reinterpret_cast<const float4 *>(x2 + c);
-                if (a.xop == 2) {
-                    v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
-                } else {
-                    v.x = v.x / (1.f + expf(-v.x)) * w.x;
-                    v.y = v.y / (1.f + expf(-v.y)) * w.y;
-                    v.z = v.z / (1.f + expf(-v.z)) * w.z;
-                    v.w = v.w / (1.f + expf(-v.w)) * w.w;
-                }
-            }
-            ss += v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
-            *reinterpret_cast<float4 *>(xs + i * ks + c) = v;
-        }
-        if (norm) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (lane == 0) ssq[8 + i * 16 + warp] = ss;
-        }
-    }
-    __syncthreads();
-    if (norm && tid < nr) {
-        float s = 0.f;
-        for (int w = 0; w < 16; w++) s += ssq[8 + tid * 16 + w];
-        ssq[tid] = s;
-    }
-    // a warp per rank: this CTA's columns of one row of A with every activation row
-    for (int rr = warp; rr < r; rr += 16) {
-        const uint16_t *w = a.a + ((int64_t)slot * a.rpad + rr) * a.cols + k0;
-        float acc[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) acc[i] = 0.f;
 #pragma unroll 2
-        for (int c = 8 * lane; c < kn; c += 256) {
-            const uint4 q = *reinterpret_cast<const uint4 *>(w + c);
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (i < nr) {
-                    const float4 v = *reinterpret_cast<const float4 *>(xs + i * ks + c), z = *reinterpret_cast<const float4 *>(xs + i * ks + c + 4);
-                    acc[i] += bf_lo(q.x) * v.x + bf_hi(q.x) * v.y + bf_lo(q.y) * v.z + bf_hi(q.y) * v.w + bf_lo(q.z) * z.x +
-                              bf_hi(q.z) * z.y + bf_lo(q.w) * z.z + bf_hi(q.w) * z.w;
-                }
+    for (int e = tid; e < nr * (kn / 4); e += 512) {
+        const int i = e / (kn / 4), c = (e - i * (kn / 4)) * 4;
+        const int64_t at = row_of(i) * a.ldx + k0 + c;
+        float4 v = *reinterpret_cast<const float4 *>(a.x + at);
+        if (a.xop >= 2) {
+            const float4 w = *reinterpret_cast<const float4 *>(a.x2 + at);
+            if (a.xop == 2) {
+                v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+            } else {
+                v.x = v.x / (1.f + expf(-v.x)) * w.x;
+                v.y = v.y / (1.f + expf(-v.y)) * w.y;
+                v.z = v.z / (1.f + expf(-v.z)) * w.z;
+                v.w = v.w / (1.f + expf(-v.w)) * w.w;
+            }
+        }
+        *reinterpret_cast<float4 *>(sh.xs + i * ks + c) = v;
+    }
+    if (nn > 0) fetch_base(0);
+    __syncthreads();
+    const uint16_t *wa = a.a + (int64_t)slot * a.rpad * a.cols + k0;
+    if (nr == 1) rows_narrow<1>(a, sh, wa, r, nr, ks, kn);
+    else if (nr == 2) rows_narrow<2>(a, sh, wa, r, nr, ks, kn);
+    else if (nr <= 4) rows_narrow<4>(a, sh, wa, r, nr, ks, kn);
+    else rows_narrow<8>(a, sh, wa, r, nr, ks, kn);
+    if (norm && 15 - warp < nr) {   // the warps with the fewest ranks add the squares
+        const int i = 15 - warp;
+        float ss = 0.f;
+        for (int c = 4 * lane; c < kn; c += 128) {
+            const float4 v = *reinterpret_cast<const float4 *>(sh.xs + i * ks + c);
+            ss += v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
         }
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (i < nr) {
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-                if (lane == 0) part_u[i * a.rpad + rr] = acc[i];
-            }
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (lane == 0) sh.ssq[i] = ss;
     }
     __syncthreads();
     cluster_arrive();
     cluster_wait();
     // every CTA adds the eight partial sums in the same order
-    const float scale = a.scale[slot];
     for (int e = tid; e < nr * r; e += 512) {
         const int i = e / r, rr = e - i * r;
-        const uint32_t at = smem_u32(part_u + i * a.rpad + rr);
-        float s = 0.f;
+        const uint32_t at = smem_u32(sh.part + i * a.rpad + rr), sa = smem_u32(sh.ssq + i);
+        float p[QM_LORA_CLUSTER], q[QM_LORA_CLUSTER];
 #pragma unroll
-        for (int k = 0; k < QM_LORA_CLUSTER; k++) s += peer_f32(peer_addr(at, k));
-        if (norm) {
-            const uint32_t sa = smem_u32(ssq + i);
-            float q = 0.f;
-#pragma unroll
-            for (int k = 0; k < QM_LORA_CLUSTER; k++) q += peer_f32(peer_addr(sa, k));
-            s *= rsqrtf(q / (float)a.cols + a.eps);
+        for (int k = 0; k < QM_LORA_CLUSTER; k++) {
+            p[k] = peer_f32(peer_addr(at, k));
+            q[k] = norm ? peer_f32(peer_addr(sa, k)) : 0.f;
         }
-        u[rr * 8 + i] = s * scale;
+        float s = 0.f, ss = 0.f;
+#pragma unroll
+        for (int k = 0; k < QM_LORA_CLUSTER; k++) {
+            s += p[k];
+            ss += q[k];
+        }
+        if (norm) s *= rsqrtf(ss / (float)a.cols + a.eps);
+        sh.u[rr * 8 + i] = s * scale;
     }
     cluster_arrive();   // done with the others' memory; waited for before leaving
-    const int group = tid >> 7, col2 = (tid & 127) * 2;
     const int chunks = (nn + QM_LORA_CHUNK - 1) / QM_LORA_CHUNK;
     for (int k = 0; k < chunks; k++) {
         copy_wait<0>();
         __syncthreads();
         if (k + 1 < chunks) fetch_b(k + 1);
-        const uint16_t *b = k & 1 ? b1 : b0;
-        float acc[8][2];
-#pragma unroll
-        for (int i = 0; i < 8; i++) acc[i][0] = acc[i][1] = 0.f;
-        for (int rr = group; rr < r; rr += 4) {
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(b + rr * QM_LORA_CHUNK + col2);
-            const float lo = bf_lo(w), hi = bf_hi(w);
-            const float4 p = *reinterpret_cast<const float4 *>(u + rr * 8), q = *reinterpret_cast<const float4 *>(u + rr * 8 + 4);
-            const float v[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (i < nr) {
-                    acc[i][0] += v[i] * lo;
-                    acc[i][1] += v[i] * hi;
-                }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (i < nr) *reinterpret_cast<float2 *>(sums + (group * 8 + i) * QM_LORA_CHUNK + col2) = make_float2(acc[i][0], acc[i][1]);
+        const uint16_t *b = k & 1 ? sh.b1 : sh.b0;
+        if (nr == 1) rows_wide<1>(sh, b, r, nr);
+        else if (nr == 2) rows_wide<2>(sh, b, r, nr);
+        else if (nr <= 4) rows_wide<4>(sh, b, r, nr);
+        else rows_wide<8>(sh, b, r, nr);
         __syncthreads();
-        const int width = min(QM_LORA_CHUNK, nn - k * QM_LORA_CHUNK);
-        for (int e = tid; e < nr * QM_LORA_CHUNK; e += 512) {
-            const int i = e / QM_LORA_CHUNK, c = e % QM_LORA_CHUNK;
-            if (c >= width) continue;
-            int yr = mine[0];
+        const int c = k * QM_LORA_CHUNK + out_col;
 #pragma unroll
-            for (int q = 1; q < 8; q++) yr = q == i ? mine[q] : yr;
-            const float *s = sums + i * QM_LORA_CHUNK + c;
-            const int64_t at = n0 + k * QM_LORA_CHUNK + c;
-            const float d = (s[0] + s[8 * QM_LORA_CHUNK]) + (s[16 * QM_LORA_CHUNK] + s[24 * QM_LORA_CHUNK]);
-            a.y[yr * a.ldy + at] = (a.base ? a.base[yr * a.ldb + at] : 0.f) + d;
+        for (int i = 0; i < 4; i++) {
+            const int yr = out_row + 2 * i;
+            if (yr < nr && c < nn) {
+                const float *s = sh.sums + yr * QM_LORA_CHUNK + out_col;
+                const float d = (s[0] + s[8 * QM_LORA_CHUNK]) + (s[16 * QM_LORA_CHUNK] + s[24 * QM_LORA_CHUNK]);
+                a.y[row_of(yr) * a.ldy + n0 + c] = base[i] + d;
+            }
         }
+        if (k + 1 < chunks) fetch_base(k + 1);
     }
     cluster_wait();
 }

@@ -124,19 +124,30 @@ static void fill(QmQkArgs *a, const qm_rope *r, uint64_t x, int64_t ldx, int32_t
     a->rot = r->rot;
     a->interleaved = r->interleaved;
     a->norm = (flags & QM_QK_NO_NORM) ? 0 : 1;
-    a->bf16 = (flags & QM_QK_BF16) ? 1 : 0;
     a->eps = eps;
 }
 
 // Two neighbouring pairs per lane: whole vectors of two elements everywhere. Otherwise one.
-static bool vectors(const QmQkArgs &a, uint64_t f32_ptrs, int64_t f32_lds) {
-    const uint64_t part = a.bf16 ? 3 : 7;
+static bool vectors(const QmQkArgs &a, bool bf16, uint64_t f32_ptrs, int64_t f32_lds) {
+    const uint64_t part = bf16 ? 3 : 7;
     const uint64_t qk = (a.hq ? (uint64_t)(uintptr_t)a.q : 0) | (a.hk ? (uint64_t)(uintptr_t)a.k : 0);
     const int64_t lds = f32_lds | (a.hq ? a.ldq : 0) | (a.hk ? a.ldk : 0);
     return a.dim % 4 == 0 && a.rot % 4 == 0 && !(f32_ptrs & 7) && !(qk & part) && !(lds & 1);
 }
 
-static int slots(const QmQkArgs &a, bool vec) { return !vec ? 3 : a.dim <= 128 ? 0 : a.dim <= 256 ? 1 : 2; }
+// The kernel of a direction: by element type, then by slots of a lane.
+static int kernel(const QmQkArgs &a, int first, bool bf16, bool vec) {
+    return first + (bf16 ? 4 : 0) + (!vec ? 3 : a.dim <= 128 ? 0 : a.dim <= 256 ? 1 : 2);
+}
+
+// As many warps as the device holds before a warp gets a second head of its token; then up to 16 heads share the angles
+// (8192 tokens x 40 heads of 128: QK_CHUNK_FIGURES).
+static void deal(const qm_ctx *c, QmQkArgs *a) {
+    const int64_t heads = (int64_t)a->hq + a->hk;
+    a->chunk = (int32_t)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, heads), a->tokens * heads / (64ll * c->sm_count)));
+    a->q_chunks = (a->hq + a->chunk - 1) / a->chunk;
+    a->chunks = a->q_chunks + (a->hk + a->chunk - 1) / a->chunk;
+}
 
 extern "C" int32_t qm_qk_norm_rope(qm_ctx *c, qm_rope *r, uint64_t x_dev, int64_t ldx, int32_t tokens, int32_t q_heads,
                                    int32_t k_heads, uint64_t q_gain_dev, uint64_t k_gain_dev, float eps, uint64_t pos_dev,
@@ -146,12 +157,13 @@ extern "C" int32_t qm_qk_norm_rope(qm_ctx *c, qm_rope *r, uint64_t x_dev, int64_
     if (rc || tokens == 0) return rc;
     QmQkArgs a;
     fill(&a, r, x_dev, ldx, tokens, q_heads, k_heads, q_gain_dev, k_gain_dev, eps, pos_dev, q_out, ldq, k_out, ldk, flags);
-    const int64_t dim = r->dim, size = a.bf16 ? 2 : 4;
+    const bool bf16 = (flags & QM_QK_BF16) != 0;
+    const int64_t dim = r->dim, size = bf16 ? 2 : 4;
     const Span x = span_of(x_dev, tokens, ldx * 4, (q_heads + (int64_t)k_heads) * dim * 4);
     const Span q = q_heads ? span_of(q_out, tokens, ldq * size, q_heads * dim * size) : Span{0, 0};
     const Span k = k_heads ? span_of(k_out, tokens, ldk * size, k_heads * dim * size) : Span{0, 0};
-    const bool q_on = !a.bf16 && q_out == x_dev && ldq == ldx;
-    const bool k_on = !a.bf16 && k_out == x_dev + (uint64_t)q_heads * dim * 4 && ldk == ldx;
+    const bool q_on = !bf16 && q_out == x_dev && ldq == ldx;
+    const bool k_on = !bf16 && k_out == x_dev + (uint64_t)q_heads * dim * 4 && ldk == ldx;
     if (q_heads && overlap(q, x) && !q_on) return QM_ERR_ARG;
     if (k_heads && overlap(k, x) && !k_on) return QM_ERR_ARG;
     // side by side in one buffer of rows (q_on and k_on among them) the two do not meet
@@ -160,17 +172,12 @@ extern "C" int32_t qm_qk_norm_rope(qm_ctx *c, qm_rope *r, uint64_t x_dev, int64_
         const int64_t in = ((gap % row) + row) % row;
         if (ldq != ldk || in < q_heads * dim * size || in + k_heads * dim * size > row) return QM_ERR_ARG;
     }
-    const int64_t heads = (int64_t)q_heads + k_heads;
-    // As many warps as the device holds before a warp gets a second head of its token; then up to eight heads share the
-    // angles.
-    a.chunk = (int32_t)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, heads), tokens * heads / (64ll * c->sm_count)));
-    a.chunks = (int32_t)((heads + a.chunk - 1) / a.chunk);
+    deal(c, &a);
     const int64_t grid = ((int64_t)tokens * a.chunks + 7) / 8;
     if (grid > 0x7FFFFFFF) return QM_ERR_SHAPE;
     CtxGuard g(c);
     DRV(g.rc);
-    const bool vec = vectors(a, x_dev | q_gain_dev | k_gain_dev, ldx);
-    return qm_launch(c, QM_K_QK_NORM_W1 + slots(a, vec), (unsigned)grid, 1, 256, 0, &a, true);
+    return qm_launch(c, kernel(a, QM_K_QK_NORM_W1, bf16, vectors(a, bf16, x_dev | q_gain_dev | k_gain_dev, ldx)), (unsigned)grid, 1, 256, 0, &a, true);
 }
 
 extern "C" int32_t qm_qk_norm_rope_backward(qm_ctx *c, qm_rope *r, uint64_t x_dev, int64_t ldx, int32_t tokens, int32_t q_heads,
@@ -195,7 +202,8 @@ extern "C" int32_t qm_qk_norm_rope_backward(qm_ctx *c, qm_rope *r, uint64_t x_de
     }
     QmQkArgs a;
     fill(&a, r, x_dev, ldx, tokens, q_heads, k_heads, q_gain_dev, k_gain_dev, eps, pos_dev, dq_dev, lddq, dk_dev, lddk, flags);
-    const int64_t size = a.bf16 ? 2 : 4;
+    const bool bf16 = (flags & QM_QK_BF16) != 0;
+    const int64_t size = bf16 ? 2 : 4;
     const Span dx = span_of(dx_dev, tokens, lddx * 4, heads * dim * 4);
     if (overlap(dx, span_of(x_dev, tokens, ldx * 4, heads * dim * 4)) && !(dx_dev == x_dev && lddx == ldx)) return QM_ERR_ARG;
     if (q_heads && overlap(dx, span_of(dq_dev, tokens, lddq * size, q_heads * dim * size)) && !(size == 4 && dq_dev == dx_dev && lddq == lddx))
@@ -206,12 +214,11 @@ extern "C" int32_t qm_qk_norm_rope_backward(qm_ctx *c, qm_rope *r, uint64_t x_de
     a.dx = (float *)(uintptr_t)dx_dev;
     a.lddx = lddx;
     a.partial = gains ? (float *)(uintptr_t)r->partial : nullptr;
-    a.chunk = (int32_t)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, heads), tokens * heads / (64ll * c->sm_count)));
-    a.chunks = (int32_t)((heads + a.chunk - 1) / a.chunk);
+    deal(c, &a);
     const int64_t tasks = (int64_t)tokens * a.chunks;
     const unsigned grid = (unsigned)std::min<int64_t>((tasks + 7) / 8, r->grad_ctas);
-    const bool vec = vectors(a, x_dev | q_gain_dev | k_gain_dev | dx_dev, ldx | lddx);
-    rc = qm_launch(c, QM_K_QK_GRAD_W1 + slots(a, vec), grid, 1, 256, gains ? (unsigned)(8 * 2 * dim * 4) : 0, &a, true);
+    rc = qm_launch(c, kernel(a, QM_K_QK_GRAD_W1, bf16, vectors(a, bf16, x_dev | q_gain_dev | k_gain_dev | dx_dev, ldx | lddx)), grid, 1, 256,
+                   gains ? (unsigned)(8 * 2 * dim * 4) : 0, &a, true);
     if (rc || !gains) return rc;
     QmGainSumArgs s;
     memset(&s, 0, sizeof s);
@@ -220,5 +227,5 @@ extern "C" int32_t qm_qk_norm_rope_backward(qm_ctx *c, qm_rope *r, uint64_t x_de
     s.dk = (float *)(uintptr_t)dk_gain_dev;
     s.ctas = (int32_t)grid;
     s.dim = (int32_t)dim;
-    return qm_launch(c, QM_K_QK_GAIN_SUM, (unsigned)((2 * dim + 7) / 8), 1, 256, 0, &s, true);
+    return qm_launch(c, QM_K_QK_GAIN_SUM, (unsigned)((2 * dim + 31) / 32), 1, 1024, 0, &s, true);
 }

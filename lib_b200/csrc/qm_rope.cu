@@ -7,10 +7,12 @@
 //   dx = r * (dz * gain - n * mean(dz * gain * n)), r = 1 / sqrt(mean(x^2) + eps).
 //
 // Nothing is read twice and nothing is written that is not a result, so both are bound by memory for a batch of tokens and
-// by launch latency for one. A warp takes `chunk` heads of one token: the angles are computed once for all of them, up to
-// four heads are in flight at a time, and a head lies in the warp's registers between its load and its store. A lane owns
-// V neighbouring pairs per slot; with V = 2 every access is 8 bytes wide (4 for bf16) and a warp's accesses are contiguous,
-// in the half-split as in the adjacent order. V = 1 serves what is not aligned for that.
+// by launch latency for one. A warp takes `chunk` query heads (or key heads) of one token: the angles, and with them the
+// products of gains, cosines and sines, are computed once for all of them, four heads are in flight at a time and share one
+// reduction (each step halves the values a lane holds, so four sums cost nine steps instead of twenty), and a head lies in
+// the warp's registers between its load and its store. A lane owns V neighbouring pairs per slot; with V = 2 every access is
+// 8 bytes wide (4 for bf16) and a warp's accesses are contiguous, in the half-split as in the adjacent order. V = 1 serves
+// what is not aligned for that.
 //
 // The angle of a far position has lost its fraction in 32 bits (position 10^6 is 0.06 off), so the turns (angle / 2 pi) are
 // a float64 product; their fractional part, at most a half, is exact in float64 and loses 2^-25 of a turn in float32.
@@ -21,8 +23,7 @@
 
 namespace {
 
-constexpr int HEADS = 4;      // heads in flight of a forward warp
-constexpr int BWD_HEADS = 2;  // of a backward warp, which holds two values per element
+constexpr int HEADS = 4;   // heads in flight of a warp
 constexpr int WARPS = 8;
 
 __device__ __forceinline__ void wait_for_inputs() {
@@ -30,10 +31,18 @@ __device__ __forceinline__ void wait_for_inputs() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
+// The sums over the warp of four values; lane l gets that of value l / 8.
+__device__ __forceinline__ float warp_sum4(const float (&s)[4]) {
+    const int lane = threadIdx.x & 31;
+    const bool high = lane & 16, odd = lane & 8;
+    float a = high ? s[2] : s[0], b = high ? s[3] : s[1];
+    a += __shfl_xor_sync(0xffffffffu, high ? s[0] : s[2], 16);
+    b += __shfl_xor_sync(0xffffffffu, high ? s[1] : s[3], 16);
+    float c = odd ? b : a;
+    c += __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    for (int o = 4; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+    return c;
 }
 
 // Where the V pairs of a slot lie in a head: elements [at, at + V) and [to, to + V). Turning pairs of the half-split order
@@ -70,9 +79,9 @@ __device__ __forceinline__ void load_f32(const float *p, float (&v)[V]) {
     }
 }
 
-template <int V>
-__device__ __forceinline__ void load_any(const void *base, int64_t at, bool bf16, float (&v)[V]) {
-    if (!bf16) {
+template <int V, bool BF16>
+__device__ __forceinline__ void load_any(const void *base, int64_t at, float (&v)[V]) {
+    if constexpr (!BF16) {
         load_f32<V>(reinterpret_cast<const float *>(base) + at, v);
     } else if constexpr (V == 2) {
         const uint32_t t = *reinterpret_cast<const uint32_t *>(reinterpret_cast<const uint16_t *>(base) + at);
@@ -83,9 +92,9 @@ __device__ __forceinline__ void load_any(const void *base, int64_t at, bool bf16
     }
 }
 
-template <int V>
-__device__ __forceinline__ void store_any(void *base, int64_t at, bool bf16, const float (&v)[V]) {
-    if (!bf16) {
+template <int V, bool BF16>
+__device__ __forceinline__ void store_any(void *base, int64_t at, const float (&v)[V]) {
+    if constexpr (!BF16) {
         float *p = reinterpret_cast<float *>(base) + at;
         if constexpr (V == 2) *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]);
         else *p = v[0];
@@ -96,22 +105,13 @@ __device__ __forceinline__ void store_any(void *base, int64_t at, bool bf16, con
     }
 }
 
-// Turns the pairs of one slot; the angle's cosine and sine are those of pair v.
+// In the adjacent order two vectors of two hold (p0, q0), (p1, q1): from there to (p0, p1), (q0, q1), and back.
 template <int V>
-__device__ __forceinline__ void turn(float (&f)[V], float (&g)[V], const float (&c)[V], const float (&s)[V], bool split) {
-    if (split || V == 1) {
-#pragma unroll
-        for (int v = 0; v < V; v++) {
-            const float p = f[v], q = g[v];
-            f[v] = p * c[v] - q * s[v];
-            g[v] = q * c[v] + p * s[v];
-        }
-    } else if constexpr (V == 2) {
-        const float p = f[0], q = f[1], r = g[0], t = g[1];
-        f[0] = p * c[0] - q * s[0];
-        f[1] = q * c[0] + p * s[0];
-        g[0] = r * c[1] - t * s[1];
-        g[1] = t * c[1] + r * s[1];
+__device__ __forceinline__ void regroup(float (&f)[V], float (&g)[V], bool adjacent) {
+    if constexpr (V == 2) {
+        const float t = adjacent ? g[0] : f[1];
+        g[0] = adjacent ? f[1] : g[0];
+        f[1] = t;
     }
 }
 
@@ -119,10 +119,9 @@ template <int V, int NP>
 struct Lane {
     Place at[NP];
     float cs[NP][V], sn[NP][V];
-    bool split;
+    float w[NP][V], z[NP][V];   // the gains of the pairs' elements
 
     __device__ __forceinline__ void places(const QmQkArgs &a, int lane) {
-        split = !a.interleaved;
 #pragma unroll
         for (int i = 0; i < NP; i++) at[i] = place<V>(a, (i * 32 + lane) * V);
     }
@@ -141,17 +140,45 @@ struct Lane {
                 }
             }
     }
+    __device__ __forceinline__ void gains(const QmQkArgs &a, const float *gain) {
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+#pragma unroll
+            for (int v = 0; v < V; v++) w[i][v] = z[i][v] = 1.f;
+            if (a.norm && gain && at[i].there) {
+                load_f32<V>(gain + at[i].at, w[i]);
+                load_f32<V>(gain + at[i].to, z[i]);
+                regroup<V>(w[i], z[i], a.interleaved);
+            }
+        }
+    }
 };
 
-template <int V, int NP>
+// A warp's share: heads [first, last) of a token, all of them query heads or all key heads.
+struct Task {
+    int token, first, last;
+    bool is_q;
+    __device__ __forceinline__ Task(const QmQkArgs &a, int64_t task) {
+        token = (int)(task / a.chunks);
+        const int c = (int)(task % a.chunks);
+        is_q = c < a.q_chunks;
+        first = is_q ? c * a.chunk : a.hq + (c - a.q_chunks) * a.chunk;
+        last = min(first + a.chunk, is_q ? a.hq : a.hq + a.hk);
+    }
+    // element 0 of this task's first head in the q or k rows
+    __device__ __forceinline__ int64_t row(const QmQkArgs &a) const {
+        return is_q ? (int64_t)token * a.ldq + (int64_t)first * a.dim : (int64_t)token * a.ldk + (int64_t)(first - a.hq) * a.dim;
+    }
+};
+
+template <int V, int NP, bool BF16>
 __device__ __forceinline__ void forward(const QmQkArgs &a) {
     wait_for_inputs();
     const int lane = threadIdx.x & 31;
-    const int64_t task = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-    if (task >= (int64_t)a.tokens * a.chunks) return;
-    const int token = (int)(task / a.chunks), first = (int)(task % a.chunks) * a.chunk;
-    const int last = min(first + a.chunk, a.hq + a.hk);
-    const float *row = a.x + (int64_t)token * a.ldx;
+    const int64_t number = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+    if (number >= (int64_t)a.tokens * a.chunks) return;
+    const Task t(a, number);
+    const float *row = a.x + (int64_t)t.token * a.ldx + (int64_t)t.first * a.dim;
     Lane<V, NP> l;
     l.places(a, lane);
     float f[HEADS][NP][V], g[HEADS][NP][V];
@@ -162,53 +189,62 @@ __device__ __forceinline__ void forward(const QmQkArgs &a) {
             for (int i = 0; i < NP; i++) {
 #pragma unroll
                 for (int v = 0; v < V; v++) f[u][i][v] = g[u][i][v] = 0.f;
-                if (h0 + u < last && l.at[i].there) {
-                    load_f32<V>(row + (int64_t)(h0 + u) * a.dim + l.at[i].at, f[u][i]);
-                    load_f32<V>(row + (int64_t)(h0 + u) * a.dim + l.at[i].to, g[u][i]);
+                if (h0 + u < t.last && l.at[i].there) {
+                    load_f32<V>(row + (h0 - t.first + u) * a.dim + l.at[i].at, f[u][i]);
+                    load_f32<V>(row + (h0 - t.first + u) * a.dim + l.at[i].to, g[u][i]);
                 }
             }
     };
-    fetch(first);
-    l.angles(a, lane, token);
-    for (int h0 = first; h0 < last; h0 += HEADS) {
-        if (h0 != first) fetch(h0);
+    fetch(t.first);
+    l.gains(a, t.is_q ? a.gain_q : a.gain_k);
+    l.angles(a, lane, t.token);
+    // (p, q) -> r (p w c - q z s, q z c + p w s)
+    float wc[NP][V], zs[NP][V], zc[NP][V], ws[NP][V];
 #pragma unroll
-        for (int u = 0; u < HEADS; u++) {
-            const int h = h0 + u;
-            if (h >= last) break;
-            float r = 1.f;
-            if (a.norm) {
-                float ss = 0.f;
+    for (int i = 0; i < NP; i++)
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            wc[i][v] = l.w[i][v] * l.cs[i][v];
+            ws[i][v] = l.w[i][v] * l.sn[i][v];
+            zc[i][v] = l.z[i][v] * l.cs[i][v];
+            zs[i][v] = l.z[i][v] * l.sn[i][v];
+        }
+    void *out = t.is_q ? a.q : a.k;
+    const int64_t base = t.row(a);
+    for (int h0 = t.first; h0 < t.last; h0 += HEADS) {
+        if (h0 != t.first) fetch(h0);
+        float r = 1.f;   // lane l: the factor of head l / 8
+        if (a.norm) {
+            float ss[HEADS];
+#pragma unroll
+            for (int u = 0; u < HEADS; u++) {
+                ss[u] = 0.f;
 #pragma unroll
                 for (int i = 0; i < NP; i++)
 #pragma unroll
-                    for (int v = 0; v < V; v++) ss += f[u][i][v] * f[u][i][v] + g[u][i][v] * g[u][i][v];
-                r = 1.f / sqrtf(warp_sum(ss) / (float)a.dim + a.eps);
+                    for (int v = 0; v < V; v++) ss[u] += f[u][i][v] * f[u][i][v] + g[u][i][v] * g[u][i][v];
             }
-            const bool is_q = h < a.hq;
-            const float *gain = is_q ? a.gain_q : a.gain_k;
-            void *out = is_q ? a.q : a.k;
-            const int64_t base = is_q ? (int64_t)token * a.ldq + (int64_t)h * a.dim : (int64_t)token * a.ldk + (int64_t)(h - a.hq) * a.dim;
+            r = __frsqrt_rn(warp_sum4(ss) / (float)a.dim + a.eps);
+        }
+#pragma unroll
+        for (int u = 0; u < HEADS; u++) {
+            const float ru = __shfl_sync(0xffffffffu, r, 8 * u);
+            if (h0 + u >= t.last) break;
+            const int64_t at = base + (h0 - t.first + u) * a.dim;
 #pragma unroll
             for (int i = 0; i < NP; i++) {
                 if (!l.at[i].there) continue;
-                if (a.norm) {
-                    float w[V], z[V];
+                regroup<V>(f[u][i], g[u][i], a.interleaved);
 #pragma unroll
-                    for (int v = 0; v < V; v++) w[v] = z[v] = 1.f;
-                    if (gain) {
-                        load_f32<V>(gain + l.at[i].at, w);
-                        load_f32<V>(gain + l.at[i].to, z);
-                    }
-#pragma unroll
-                    for (int v = 0; v < V; v++) {
-                        f[u][i][v] *= r * w[v];
-                        g[u][i][v] *= r * z[v];
-                    }
+                for (int v = 0; v < V; v++) {
+                    const float p = f[u][i][v], q = g[u][i][v];
+                    // (a select where nothing turns: zero times an infinite neighbour is not zero)
+                    f[u][i][v] = ru * (p * wc[i][v] - (l.at[i].turns ? q * zs[i][v] : 0.f));
+                    g[u][i][v] = ru * (q * zc[i][v] + (l.at[i].turns ? p * ws[i][v] : 0.f));
                 }
-                if (l.at[i].turns) turn<V>(f[u][i], g[u][i], l.cs[i], l.sn[i], l.split);
-                store_any<V>(out, base + l.at[i].at, a.bf16 != 0, f[u][i]);
-                store_any<V>(out, base + l.at[i].to, a.bf16 != 0, g[u][i]);
+                regroup<V>(f[u][i], g[u][i], a.interleaved);
+                store_any<V, BF16>(out, at + l.at[i].at, f[u][i]);
+                store_any<V, BF16>(out, at + l.at[i].to, g[u][i]);
             }
         }
     }
@@ -216,10 +252,11 @@ __device__ __forceinline__ void forward(const QmQkArgs &a) {
 
 // A warp walks tokens; what it adds up for the gains stays in its registers, the CTA's warps are added in warp order and
 // qm_qk_gain_sum adds the CTAs in their order: the same bits in every run.
-template <int V, int NP>
+template <int V, int NP, bool BF16>
 __device__ __forceinline__ void backward(const QmQkArgs &a) {
     wait_for_inputs();
     extern __shared__ float sums[];   // [WARPS][2][dim] with the gains' gradients
+    constexpr int H = NP == 1 ? HEADS : 2;   // heads in flight
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Lane<V, NP> l;
     l.places(a, lane);
@@ -231,86 +268,85 @@ __device__ __forceinline__ void backward(const QmQkArgs &a) {
 #pragma unroll
             for (int v = 0; v < V; v++) df[k][i][v] = dg[k][i][v] = 0.f;
     const int64_t tasks = (int64_t)a.tokens * a.chunks;
-    for (int64_t task = (int64_t)blockIdx.x * WARPS + warp; task < tasks; task += (int64_t)gridDim.x * WARPS) {
-        const int token = (int)(task / a.chunks), first = (int)(task % a.chunks) * a.chunk;
-        const int last = min(first + a.chunk, a.hq + a.hk);
-        const float *row = a.x + (int64_t)token * a.ldx;
-        float *drow = a.dx + (int64_t)token * a.lddx;
-        l.angles(a, lane, token);
+    for (int64_t number = (int64_t)blockIdx.x * WARPS + warp; number < tasks; number += (int64_t)gridDim.x * WARPS) {
+        const Task t(a, number);
+        const float *row = a.x + (int64_t)t.token * a.ldx + (int64_t)t.first * a.dim;
+        float *drow = a.dx + (int64_t)t.token * a.lddx + (int64_t)t.first * a.dim;
+        const void *dy = t.is_q ? a.q : a.k;
+        const int64_t base = t.row(a);
+        float f[H][NP][V], g[H][NP][V], p[H][NP][V], q[H][NP][V];
+        auto fetch = [&](int h0) {
 #pragma unroll
-        for (int i = 0; i < NP; i++)
-#pragma unroll
-            for (int v = 0; v < V; v++) l.sn[i][v] = -l.sn[i][v];   // turned back
-        for (int h0 = first; h0 < last; h0 += BWD_HEADS) {
-            float f[BWD_HEADS][NP][V], g[BWD_HEADS][NP][V], p[BWD_HEADS][NP][V], q[BWD_HEADS][NP][V];
-#pragma unroll
-            for (int u = 0; u < BWD_HEADS; u++)
+            for (int u = 0; u < H; u++)
 #pragma unroll
                 for (int i = 0; i < NP; i++) {
-                    const int h = h0 + u;
 #pragma unroll
                     for (int v = 0; v < V; v++) f[u][i][v] = g[u][i][v] = p[u][i][v] = q[u][i][v] = 0.f;
-                    if (h < last && l.at[i].there) {
-                        const bool is_q = h < a.hq;
-                        const void *dy = is_q ? a.q : a.k;
-                        const int64_t base = is_q ? (int64_t)token * a.ldq + (int64_t)h * a.dim : (int64_t)token * a.ldk + (int64_t)(h - a.hq) * a.dim;
+                    if (h0 + u < t.last && l.at[i].there) {
+                        const int at = (h0 - t.first + u) * a.dim;
                         if (a.norm) {
-                            load_f32<V>(row + (int64_t)h * a.dim + l.at[i].at, f[u][i]);
-                            load_f32<V>(row + (int64_t)h * a.dim + l.at[i].to, g[u][i]);
+                            load_f32<V>(row + at + l.at[i].at, f[u][i]);
+                            load_f32<V>(row + at + l.at[i].to, g[u][i]);
                         }
-                        load_any<V>(dy, base + l.at[i].at, a.bf16 != 0, p[u][i]);
-                        load_any<V>(dy, base + l.at[i].to, a.bf16 != 0, q[u][i]);
+                        load_any<V, BF16>(dy, base + at + l.at[i].at, p[u][i]);
+                        load_any<V, BF16>(dy, base + at + l.at[i].to, q[u][i]);
                     }
                 }
+        };
+        fetch(t.first);
+        l.gains(a, t.is_q ? a.gain_q : a.gain_k);
+        l.angles(a, lane, t.token);
+        for (int h0 = t.first; h0 < t.last; h0 += H) {
+            if (h0 != t.first) fetch(h0);
+            float ss[4] = {0.f, 0.f, 0.f, 0.f}, dot[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int u = 0; u < BWD_HEADS; u++) {
-                const int h = h0 + u;
-                if (h >= last) break;
-                const bool is_q = h < a.hq;
-                const float *gain = is_q ? a.gain_q : a.gain_k;
-                float ss = 0.f, dot = 0.f;
-                float w[NP][V], z[NP][V];
+            for (int u = 0; u < H; u++)
 #pragma unroll
                 for (int i = 0; i < NP; i++) {
-                    if (l.at[i].turns) turn<V>(p[u][i], q[u][i], l.cs[i], l.sn[i], l.split);
-#pragma unroll
-                    for (int v = 0; v < V; v++) w[i][v] = z[i][v] = 1.f;
-                    if (a.norm && gain && l.at[i].there) {
-                        load_f32<V>(gain + l.at[i].at, w[i]);
-                        load_f32<V>(gain + l.at[i].to, z[i]);
-                    }
+                    regroup<V>(f[u][i], g[u][i], a.interleaved);
+                    regroup<V>(p[u][i], q[u][i], a.interleaved);
 #pragma unroll
                     for (int v = 0; v < V; v++) {
-                        ss += f[u][i][v] * f[u][i][v] + g[u][i][v] * g[u][i][v];
-                        dot += p[u][i][v] * w[i][v] * f[u][i][v] + q[u][i][v] * z[i][v] * g[u][i][v];
+                        if (l.at[i].turns) {   // turned back
+                            const float b = p[u][i][v], c = q[u][i][v];
+                            p[u][i][v] = b * l.cs[i][v] + c * l.sn[i][v];
+                            q[u][i][v] = c * l.cs[i][v] - b * l.sn[i][v];
+                        }
+                        ss[u] += f[u][i][v] * f[u][i][v] + g[u][i][v] * g[u][i][v];
+                        dot[u] += p[u][i][v] * f[u][i][v] * l.w[i][v] + q[u][i][v] * g[u][i][v] * l.z[i][v];
                     }
                 }
-                float r = 1.f, m = 0.f;
-                if (a.norm) {
-                    ss = warp_sum(ss);
-                    dot = warp_sum(dot);
-                    r = 1.f / sqrtf(ss / (float)a.dim + a.eps);
-                    m = r * dot / (float)a.dim;   // mean of dz * gain * n
-                }
+            // dx = r dz gain - (r^3 mean(dz gain x)) x; lane l: the factors of head l / 8
+            float r = 1.f, m = 0.f;
+            if (a.norm) {
+                r = __frsqrt_rn(warp_sum4(ss) / (float)a.dim + a.eps);
+                m = r * r * r * (warp_sum4(dot) / (float)a.dim);
+            }
+#pragma unroll
+            for (int u = 0; u < H; u++) {
+                const float ru = __shfl_sync(0xffffffffu, r, 8 * u), mu = __shfl_sync(0xffffffffu, m, 8 * u);
+                if (h0 + u >= t.last) break;
+                const int at = (h0 - t.first + u) * a.dim;
 #pragma unroll
                 for (int i = 0; i < NP; i++) {
                     if (!l.at[i].there) continue;
-                    float o[V], t[V];
+                    float o[V], e[V];
 #pragma unroll
                     for (int v = 0; v < V; v++) {
-                        const float nf = f[u][i][v] * r, ng = g[u][i][v] * r;
-                        o[v] = r * (p[u][i][v] * w[i][v] - nf * m);
-                        t[v] = r * (q[u][i][v] * z[i][v] - ng * m);
-                        if (is_q) {
-                            df[0][i][v] += p[u][i][v] * nf;
-                            dg[0][i][v] += q[u][i][v] * ng;
+                        const float x = f[u][i][v], y = g[u][i][v], b = p[u][i][v], c = q[u][i][v];
+                        o[v] = ru * (b * l.w[i][v]) - mu * x;
+                        e[v] = ru * (c * l.z[i][v]) - mu * y;
+                        if (t.is_q) {
+                            df[0][i][v] += b * x * ru;
+                            dg[0][i][v] += c * y * ru;
                         } else {
-                            df[1][i][v] += p[u][i][v] * nf;
-                            dg[1][i][v] += q[u][i][v] * ng;
+                            df[1][i][v] += b * x * ru;
+                            dg[1][i][v] += c * y * ru;
                         }
                     }
-                    store_any<V>(drow, (int64_t)h * a.dim + l.at[i].at, false, o);
-                    store_any<V>(drow, (int64_t)h * a.dim + l.at[i].to, false, t);
+                    regroup<V>(o, e, a.interleaved);
+                    store_any<V, false>(drow, at + l.at[i].at, o);
+                    store_any<V, false>(drow, at + l.at[i].to, e);
                 }
             }
         }
@@ -321,6 +357,7 @@ __device__ __forceinline__ void backward(const QmQkArgs &a) {
 #pragma unroll
         for (int i = 0; i < NP; i++)
             if (l.at[i].there) {
+                regroup<V>(df[k][i], dg[k][i], a.interleaved);
 #pragma unroll
                 for (int v = 0; v < V; v++) {
                     sums[(warp * 2 + k) * a.dim + l.at[i].at + v] = df[k][i][v];
@@ -338,27 +375,41 @@ __device__ __forceinline__ void backward(const QmQkArgs &a) {
 
 }  // namespace
 
-extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_w1(const __grid_constant__ QmQkArgs a) { forward<2, 1>(a); }
-extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_w2(const __grid_constant__ QmQkArgs a) { forward<2, 2>(a); }
-extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_w4(const __grid_constant__ QmQkArgs a) { forward<2, 4>(a); }
-extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_s8(const __grid_constant__ QmQkArgs a) { forward<1, 8>(a); }
-extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w1(const __grid_constant__ QmQkArgs a) { backward<2, 1>(a); }
-extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w2(const __grid_constant__ QmQkArgs a) { backward<2, 2>(a); }
-extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w4(const __grid_constant__ QmQkArgs a) { backward<2, 4>(a); }
-extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_s8(const __grid_constant__ QmQkArgs a) { backward<1, 8>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_w1(const __grid_constant__ QmQkArgs a) { forward<2, 1, false>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_w2(const __grid_constant__ QmQkArgs a) { forward<2, 2, false>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_w4(const __grid_constant__ QmQkArgs a) { forward<2, 4, false>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_s8(const __grid_constant__ QmQkArgs a) { forward<1, 8, false>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_w1_b(const __grid_constant__ QmQkArgs a) { forward<2, 1, true>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_w2_b(const __grid_constant__ QmQkArgs a) { forward<2, 2, true>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_w4_b(const __grid_constant__ QmQkArgs a) { forward<2, 4, true>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_s8_b(const __grid_constant__ QmQkArgs a) { forward<1, 8, true>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w1(const __grid_constant__ QmQkArgs a) { backward<2, 1, false>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w2(const __grid_constant__ QmQkArgs a) { backward<2, 2, false>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w4(const __grid_constant__ QmQkArgs a) { backward<2, 4, false>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_s8(const __grid_constant__ QmQkArgs a) { backward<1, 8, false>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w1_b(const __grid_constant__ QmQkArgs a) { backward<2, 1, true>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w2_b(const __grid_constant__ QmQkArgs a) { backward<2, 2, true>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w4_b(const __grid_constant__ QmQkArgs a) { backward<2, 4, true>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_s8_b(const __grid_constant__ QmQkArgs a) { backward<1, 8, true>(a); }
 
-// One CTA per eight columns of the [2][dim] sums: 32 threads walk the CTAs' rows of a column in float64 (one order, whatever
-// the grid), a warp adds its threads.
-extern "C" __global__ void __launch_bounds__(256) qm_qk_gain_sum(const __grid_constant__ QmGainSumArgs a) {
+// A CTA takes 32 columns of the [2][dim] sums, its 32 warps share the CTAs' rows, everything in float64 and in one order.
+extern "C" __global__ void __launch_bounds__(1024) qm_qk_gain_sum(const __grid_constant__ QmGainSumArgs a) {
     wait_for_inputs();
-    const int col = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (col >= 2 * a.dim) return;
+    __shared__ double part[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
     double s = 0.0;
-    for (int c = lane; c < a.ctas; c += 32) s += (double)a.partial[(int64_t)c * 2 * a.dim + col];
+    if (col < 2 * a.dim) {
+#pragma unroll 4
+        for (int c = warp; c < a.ctas; c += 32) s += (double)a.partial[(int64_t)c * 2 * a.dim + col];
+    }
+    part[warp][lane] = s;
+    __syncthreads();
+    s = part[lane][warp];   // column `warp` of this CTA
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) {
-        float *out = col < a.dim ? a.dq : a.dk;
-        if (out) out[col < a.dim ? col : col - a.dim] = (float)s;
+    const int out_col = blockIdx.x * 32 + warp;
+    if (lane == 0 && out_col < 2 * a.dim) {
+        float *out = out_col < a.dim ? a.dq : a.dk;
+        if (out) out[out_col < a.dim ? out_col : out_col - a.dim] = (float)s;
     }
 }
