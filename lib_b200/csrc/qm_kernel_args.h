@@ -390,22 +390,22 @@ struct QmQkArgs {
     const float *x;          // [tokens][ldx]: q heads, then k heads, dim floats each
     const float *gain_q, *gain_k;  // [dim] or null: ones
     const int32_t *pos;      // [tokens]
-    const double *freq;      // [rot/2] turns per position
+    const uint64_t *freq;    // [rot/2] 2^-64 turns per position
     void *q, *k;             // forward: results; backward: gradients of the results (float32 or bf16)
     float *dx;               // backward: [tokens][lddx]
-    float *partial;          // backward: [CTAs][2][dim] sums of the gains' gradients, or null
+    float *partial;          // backward: [CTAs][dim] sums of the gain's gradient, those for query heads first, or null
     int64_t ldx, ldq, ldk, lddx;
     int32_t tokens, hq, hk, dim, rot;
     int32_t interleaved, norm;
-    int32_t chunk, chunks, q_chunks;   // heads of one warp; how many such groups a token has, and its query heads
-    float eps;
+    int32_t chunk, q_chunks;   // heads of one warp; how many such groups the query heads make
+    float eps, inv_dim;
 };
 
 // The gains' gradients from the CTAs' sums (qm_qk_gain_sum).
 struct QmGainSumArgs {
-    const float *partial;    // [ctas][2][dim]
+    const float *partial;    // [ctas][dim], q_ctas of them for query heads
     float *dq, *dk;          // [dim] or null
-    int32_t ctas, dim;
+    int32_t ctas, q_ctas, dim, pad_;
 };
 
 // Low-rank adapters beside a stored projection (qm_lora.cu). A slot's A lies as [rpad][cols] and as [cols][rpad], its B as

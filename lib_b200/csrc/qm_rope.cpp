@@ -16,8 +16,8 @@ struct qm_rope {
     uint32_t magic;
     qm_ctx *ctx;
     int32_t dim, rot, interleaved;
-    CUdeviceptr freq;       // [rot/2] float64: turns per position
-    CUdeviceptr partial;    // backward: [grad_ctas][2][dim]
+    CUdeviceptr freq;       // [rot/2]: turns per position, in units of 2^-64, whole turns dropped
+    CUdeviceptr partial;    // backward: [grad_ctas][dim]
     int32_t grad_ctas;
 };
 
@@ -29,7 +29,7 @@ extern "C" int32_t qm_rope_create(qm_ctx *c, int32_t head_dim, int32_t rot_dim, 
     if (head_dim < 2 || (head_dim & 1) || rot_dim < 0 || (rot_dim & 1) || rot_dim > head_dim) return QM_ERR_SHAPE;
     if (head_dim > QM_ROPE_MAX_DIM) return QM_ERR_LIMIT;
     if ((flags & ~QM_ROPE_INTERLEAVED) || !(theta > 0.f) || isinf(theta)) return QM_ERR_ARG;
-    std::vector<double> freq;
+    std::vector<uint64_t> freq;
     try {
         freq.resize(rot_dim / 2 + 1);
     } catch (const std::bad_alloc &) {
@@ -38,8 +38,9 @@ extern "C" int32_t qm_rope_create(qm_ctx *c, int32_t head_dim, int32_t rot_dim, 
     for (int i = 0; i < rot_dim / 2; i++) {
         const double f = factors ? (double)factors[i] : 1.0;
         if (!(f > 0.0) || isinf(f)) return QM_ERR_ARG;
-        // (rounded to float64 once: a turn in error is 2^-53 of the position's turns)
-        freq[i] = (double)(powl((long double)theta, -2.0l * i / rot_dim) / (long double)f / (2.0l * acosl(-1.0l)));
+        const long double turns = powl((long double)theta, -2.0l * i / rot_dim) / (long double)f / (2.0l * acosl(-1.0l));
+        if (!isfinite(turns)) return QM_ERR_ARG;
+        freq[i] = (uint64_t)ldexpl(turns - floorl(turns), 64);
     }
     qm_rope *r = new (std::nothrow) qm_rope();
     if (!r) return QM_ERR_NOMEM;
@@ -48,12 +49,12 @@ extern "C" int32_t qm_rope_create(qm_ctx *c, int32_t head_dim, int32_t rot_dim, 
     r->dim = head_dim;
     r->rot = rot_dim;
     r->interleaved = (flags & QM_ROPE_INTERLEAVED) ? 1 : 0;
-    r->grad_ctas = 4 * c->sm_count;
+    r->grad_ctas = 3 * c->sm_count;   // the most that qm_qk_norm_rope_backward launches
     CtxGuard g(c);
     CUresult e = g.rc;
-    if (e == CUDA_SUCCESS) e = c->drv->cuMemAlloc_v2(&r->freq, freq.size() * sizeof(double));
-    if (e == CUDA_SUCCESS) e = c->drv->cuMemAlloc_v2(&r->partial, (size_t)r->grad_ctas * 2 * head_dim * sizeof(float));
-    if (e == CUDA_SUCCESS) e = c->drv->cuMemcpyHtoD_v2(r->freq, freq.data(), freq.size() * sizeof(double));
+    if (e == CUDA_SUCCESS) e = c->drv->cuMemAlloc_v2(&r->freq, freq.size() * sizeof(uint64_t));
+    if (e == CUDA_SUCCESS) e = c->drv->cuMemAlloc_v2(&r->partial, (size_t)r->grad_ctas * head_dim * sizeof(float));
+    if (e == CUDA_SUCCESS) e = c->drv->cuMemcpyHtoD_v2(r->freq, freq.data(), freq.size() * sizeof(uint64_t));
     if (e != CUDA_SUCCESS) {
         if (r->freq) c->drv->cuMemFree_v2(r->freq);
         if (r->partial) c->drv->cuMemFree_v2(r->partial);
@@ -111,7 +112,7 @@ static void fill(QmQkArgs *a, const qm_rope *r, uint64_t x, int64_t ldx, int32_t
     a->gain_q = (const float *)(uintptr_t)gq;
     a->gain_k = (const float *)(uintptr_t)gk;
     a->pos = (const int32_t *)(uintptr_t)pos;
-    a->freq = (const double *)(uintptr_t)r->freq;
+    a->freq = (const uint64_t *)(uintptr_t)r->freq;
     a->q = (void *)(uintptr_t)q;
     a->k = (void *)(uintptr_t)k;
     a->ldx = ldx;
@@ -125,6 +126,7 @@ static void fill(QmQkArgs *a, const qm_rope *r, uint64_t x, int64_t ldx, int32_t
     a->interleaved = r->interleaved;
     a->norm = (flags & QM_QK_NO_NORM) ? 0 : 1;
     a->eps = eps;
+    a->inv_dim = 1.f / (float)r->dim;
 }
 
 // Two neighbouring pairs per lane: whole vectors of two elements everywhere. Otherwise one.
@@ -135,18 +137,17 @@ static bool vectors(const QmQkArgs &a, bool bf16, uint64_t f32_ptrs, int64_t f32
     return a.dim % 4 == 0 && a.rot % 4 == 0 && !(f32_ptrs & 7) && !(qk & part) && !(lds & 1);
 }
 
-// The kernel of a direction: by element type, then by slots of a lane.
-static int kernel(const QmQkArgs &a, int first, bool bf16, bool vec) {
-    return first + (bf16 ? 4 : 0) + (!vec ? 3 : a.dim <= 128 ? 0 : a.dim <= 256 ? 1 : 2);
-}
+// The slots of a lane, and with them the kernel: 0, 1, 2 for vectors of two, 3 for single elements.
+static int form(const QmQkArgs &a, bool vec) { return !vec ? 3 : a.dim <= 128 ? 0 : a.dim <= 256 ? 1 : 2; }
 
-// As many warps as the device holds before a warp gets a second head of its token; then up to 16 heads share the angles
-// (8192 tokens x 40 heads of 128: QK_CHUNK_FIGURES).
-static void deal(const qm_ctx *c, QmQkArgs *a) {
+// As many warps as the device holds before a warp gets a second head of its token; then up to `most` heads share the angles.
+// The groups of heads of a token (grid y, which holds 65535).
+static int64_t deal(const qm_ctx *c, QmQkArgs *a, int64_t most, int64_t groups_max) {
     const int64_t heads = (int64_t)a->hq + a->hk;
-    a->chunk = (int32_t)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, heads), a->tokens * heads / (64ll * c->sm_count)));
+    const int64_t least = (heads + groups_max - 2) / (groups_max - 1);
+    a->chunk = (int32_t)std::max(least, std::min(std::min(most, heads), a->tokens * heads / (64 * (int64_t)c->sm_count)));
     a->q_chunks = (a->hq + a->chunk - 1) / a->chunk;
-    a->chunks = a->q_chunks + (a->hk + a->chunk - 1) / a->chunk;
+    return a->q_chunks + (a->hk + a->chunk - 1) / a->chunk;
 }
 
 extern "C" int32_t qm_qk_norm_rope(qm_ctx *c, qm_rope *r, uint64_t x_dev, int64_t ldx, int32_t tokens, int32_t q_heads,
@@ -172,12 +173,11 @@ extern "C" int32_t qm_qk_norm_rope(qm_ctx *c, qm_rope *r, uint64_t x_dev, int64_
         const int64_t in = ((gap % row) + row) % row;
         if (ldq != ldk || in < q_heads * dim * size || in + k_heads * dim * size > row) return QM_ERR_ARG;
     }
-    deal(c, &a);
-    const int64_t grid = ((int64_t)tokens * a.chunks + 7) / 8;
-    if (grid > 0x7FFFFFFF) return QM_ERR_SHAPE;
+    const int64_t groups = deal(c, &a, 16, 65535);
+    const int kernel = QM_K_QK_NORM_W1 + (bf16 ? 4 : 0) + form(a, vectors(a, bf16, x_dev | q_gain_dev | k_gain_dev, ldx));
     CtxGuard g(c);
     DRV(g.rc);
-    return qm_launch(c, kernel(a, QM_K_QK_NORM_W1, bf16, vectors(a, bf16, x_dev | q_gain_dev | k_gain_dev, ldx)), (unsigned)grid, 1, 256, 0, &a, true);
+    return qm_launch(c, kernel, (unsigned)(((int64_t)tokens + 7) / 8), (unsigned)groups, 256, 0, &a, true);
 }
 
 extern "C" int32_t qm_qk_norm_rope_backward(qm_ctx *c, qm_rope *r, uint64_t x_dev, int64_t ldx, int32_t tokens, int32_t q_heads,
@@ -214,18 +214,21 @@ extern "C" int32_t qm_qk_norm_rope_backward(qm_ctx *c, qm_rope *r, uint64_t x_de
     a.dx = (float *)(uintptr_t)dx_dev;
     a.lddx = lddx;
     a.partial = gains ? (float *)(uintptr_t)r->partial : nullptr;
-    deal(c, &a);
-    const int64_t tasks = (int64_t)tokens * a.chunks;
-    const unsigned grid = (unsigned)std::min<int64_t>((tasks + 7) / 8, r->grad_ctas);
-    rc = qm_launch(c, kernel(a, QM_K_QK_GRAD_W1, bf16, vectors(a, bf16, x_dev | q_gain_dev | k_gain_dev | dx_dev, ldx | lddx)), grid, 1, 256,
-                   gains ? (unsigned)(8 * 2 * dim * 4) : 0, &a, true);
+    // As many CTAs as run at once (registers: three per SM, two, one and one by form), dealt evenly to the groups of heads; a
+    // group's CTAs share its tokens. Groups of at most eight heads, so that few tokens more or less per warp weigh little.
+    const int f = form(a, vectors(a, bf16, x_dev | q_gain_dev | k_gain_dev | dx_dev, ldx | lddx));
+    const int64_t at_once = (f == 0 ? 3 : f == 1 ? 2 : 1) * c->sm_count;
+    const int64_t groups = deal(c, &a, 8, at_once);
+    const int64_t gx = std::min<int64_t>(((int64_t)tokens + 7) / 8, at_once / groups);
+    rc = qm_launch(c, QM_K_QK_GRAD_W1 + (bf16 ? 4 : 0) + f, (unsigned)gx, (unsigned)groups, 256, gains ? (unsigned)(8 * dim * 4) : 0, &a, true);
     if (rc || !gains) return rc;
     QmGainSumArgs s;
     memset(&s, 0, sizeof s);
     s.partial = a.partial;
     s.dq = (float *)(uintptr_t)dq_gain_dev;
     s.dk = (float *)(uintptr_t)dk_gain_dev;
-    s.ctas = (int32_t)grid;
+    s.q_ctas = (int32_t)(a.q_chunks * gx);
+    s.ctas = (int32_t)(groups * gx);
     s.dim = (int32_t)dim;
-    return qm_launch(c, QM_K_QK_GAIN_SUM, (unsigned)((2 * dim + 31) / 32), 1, 1024, 0, &s, true);
+    return qm_launch(c, QM_K_QK_GAIN_SUM, (unsigned)((dim + 31) / 32), 2, 1024, 0, &s, true);
 }

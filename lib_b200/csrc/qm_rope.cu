@@ -15,7 +15,8 @@
 // what is not aligned for that.
 //
 // The angle of a far position has lost its fraction in 32 bits (position 10^6 is 0.06 off), so the turns (angle / 2 pi) are
-// a float64 product; their fractional part, at most a half, is exact in float64 and loses 2^-25 of a turn in float32.
+// a product in 64-bit fixed point, position times the fraction of a turn in units of 2^-64, whose overflow is the whole turns:
+// what is left is exact to 2^-33 of a turn for every position, and three integer instructions.
 #include <cuda_bf16.h>
 #include <stdint.h>
 
@@ -114,6 +115,19 @@ __device__ __forceinline__ void regroup(float (&f)[V], float (&g)[V], bool adjac
         f[1] = t;
     }
 }
+// f(p, q, pair) for every pair of a slot, in either order, without moving anything.
+template <int V, class F>
+__device__ __forceinline__ void pairs(float (&f)[V], float (&g)[V], bool adjacent, F each) {
+    if constexpr (V == 1) {
+        each(f[0], g[0], 0);
+    } else if (adjacent) {
+        each(f[0], f[1], 0);
+        each(g[0], g[1], 1);
+    } else {
+        each(f[0], g[0], 0);
+        each(f[1], g[1], 1);
+    }
+}
 
 template <int V, int NP>
 struct Lane {
@@ -126,7 +140,7 @@ struct Lane {
         for (int i = 0; i < NP; i++) at[i] = place<V>(a, (i * 32 + lane) * V);
     }
     __device__ __forceinline__ void angles(const QmQkArgs &a, int lane, int token) {
-        const double pos = (double)a.pos[token];
+        const uint64_t pos = (uint64_t)(int64_t)a.pos[token];
 #pragma unroll
         for (int i = 0; i < NP; i++)
 #pragma unroll
@@ -135,8 +149,8 @@ struct Lane {
                 cs[i][v] = 1.f;
                 sn[i][v] = 0.f;
                 if (pair < a.rot / 2) {
-                    const double turns = pos * a.freq[pair];
-                    sincospif(2.f * (float)(turns - rint(turns)), &sn[i][v], &cs[i][v]);
+                    const int turns = (int)(uint32_t)((pos * a.freq[pair]) >> 32);   // of 2^-32 turns, between minus and plus a half
+                    sincospif((float)turns * 0x1p-31f, &sn[i][v], &cs[i][v]);
                 }
             }
     }
@@ -154,19 +168,18 @@ struct Lane {
     }
 };
 
-// A warp's share: heads [first, last) of a token, all of them query heads or all key heads.
-struct Task {
-    int token, first, last;
+// A CTA's share: heads [first, last), all of them query heads or all key heads; its warps take tokens.
+struct Share {
+    int first, last;
     bool is_q;
-    __device__ __forceinline__ Task(const QmQkArgs &a, int64_t task) {
-        token = (int)(task / a.chunks);
-        const int c = (int)(task % a.chunks);
+    __device__ __forceinline__ explicit Share(const QmQkArgs &a) {
+        const int c = blockIdx.y;
         is_q = c < a.q_chunks;
         first = is_q ? c * a.chunk : a.hq + (c - a.q_chunks) * a.chunk;
         last = min(first + a.chunk, is_q ? a.hq : a.hq + a.hk);
     }
-    // element 0 of this task's first head in the q or k rows
-    __device__ __forceinline__ int64_t row(const QmQkArgs &a) const {
+    // element 0 of the first head in the q or k row of a token
+    __device__ __forceinline__ int64_t row(const QmQkArgs &a, int token) const {
         return is_q ? (int64_t)token * a.ldq + (int64_t)first * a.dim : (int64_t)token * a.ldk + (int64_t)(first - a.hq) * a.dim;
     }
 };
@@ -175,14 +188,16 @@ template <int V, int NP, bool BF16>
 __device__ __forceinline__ void forward(const QmQkArgs &a) {
     wait_for_inputs();
     const int lane = threadIdx.x & 31;
-    const int64_t number = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-    if (number >= (int64_t)a.tokens * a.chunks) return;
-    const Task t(a, number);
-    const float *row = a.x + (int64_t)t.token * a.ldx + (int64_t)t.first * a.dim;
+    const int token = blockIdx.x * WARPS + (threadIdx.x >> 5);
+    if (token >= a.tokens) return;
+    const Share t(a);
+    const bool adjacent = a.interleaved != 0;
+    const float *row = a.x + (int64_t)token * a.ldx + (int64_t)t.first * a.dim;
     Lane<V, NP> l;
     l.places(a, lane);
     float f[HEADS][NP][V], g[HEADS][NP][V];
     auto fetch = [&](int h0) {
+        const float *p = row + (h0 - t.first) * a.dim;
 #pragma unroll
         for (int u = 0; u < HEADS; u++)
 #pragma unroll
@@ -190,14 +205,14 @@ __device__ __forceinline__ void forward(const QmQkArgs &a) {
 #pragma unroll
                 for (int v = 0; v < V; v++) f[u][i][v] = g[u][i][v] = 0.f;
                 if (h0 + u < t.last && l.at[i].there) {
-                    load_f32<V>(row + (h0 - t.first + u) * a.dim + l.at[i].at, f[u][i]);
-                    load_f32<V>(row + (h0 - t.first + u) * a.dim + l.at[i].to, g[u][i]);
+                    load_f32<V>(p + u * a.dim + l.at[i].at, f[u][i]);
+                    load_f32<V>(p + u * a.dim + l.at[i].to, g[u][i]);
                 }
             }
     };
     fetch(t.first);
     l.gains(a, t.is_q ? a.gain_q : a.gain_k);
-    l.angles(a, lane, t.token);
+    l.angles(a, lane, token);
     // (p, q) -> r (p w c - q z s, q z c + p w s)
     float wc[NP][V], zs[NP][V], zc[NP][V], ws[NP][V];
 #pragma unroll
@@ -210,7 +225,7 @@ __device__ __forceinline__ void forward(const QmQkArgs &a) {
             zs[i][v] = l.z[i][v] * l.sn[i][v];
         }
     void *out = t.is_q ? a.q : a.k;
-    const int64_t base = t.row(a);
+    const int64_t base = t.row(a, token);
     for (int h0 = t.first; h0 < t.last; h0 += HEADS) {
         if (h0 != t.first) fetch(h0);
         float r = 1.f;   // lane l: the factor of head l / 8
@@ -224,7 +239,7 @@ __device__ __forceinline__ void forward(const QmQkArgs &a) {
 #pragma unroll
                     for (int v = 0; v < V; v++) ss[u] += f[u][i][v] * f[u][i][v] + g[u][i][v] * g[u][i][v];
             }
-            r = __frsqrt_rn(warp_sum4(ss) / (float)a.dim + a.eps);
+            r = __frsqrt_rn(warp_sum4(ss) * a.inv_dim + a.eps);
         }
 #pragma unroll
         for (int u = 0; u < HEADS; u++) {
@@ -234,15 +249,18 @@ __device__ __forceinline__ void forward(const QmQkArgs &a) {
 #pragma unroll
             for (int i = 0; i < NP; i++) {
                 if (!l.at[i].there) continue;
-                regroup<V>(f[u][i], g[u][i], a.interleaved);
-#pragma unroll
-                for (int v = 0; v < V; v++) {
-                    const float p = f[u][i][v], q = g[u][i][v];
-                    // (a select where nothing turns: zero times an infinite neighbour is not zero)
-                    f[u][i][v] = ru * (p * wc[i][v] - (l.at[i].turns ? q * zs[i][v] : 0.f));
-                    g[u][i][v] = ru * (q * zc[i][v] + (l.at[i].turns ? p * ws[i][v] : 0.f));
+                if (l.at[i].turns) {
+                    pairs<V>(f[u][i], g[u][i], adjacent, [&](float &p, float &q, int v) {
+                        const float first = p * wc[i][v] - q * zs[i][v];
+                        q = ru * (q * zc[i][v] + p * ws[i][v]);
+                        p = ru * first;
+                    });
+                } else {   // (apart: zero times an infinite neighbour is not zero)
+                    pairs<V>(f[u][i], g[u][i], adjacent, [&](float &p, float &q, int v) {
+                        p *= ru * wc[i][v];
+                        q *= ru * zc[i][v];
+                    });
                 }
-                regroup<V>(f[u][i], g[u][i], a.interleaved);
                 store_any<V, BF16>(out, at + l.at[i].at, f[u][i]);
                 store_any<V, BF16>(out, at + l.at[i].to, g[u][i]);
             }
@@ -255,25 +273,24 @@ __device__ __forceinline__ void forward(const QmQkArgs &a) {
 template <int V, int NP, bool BF16>
 __device__ __forceinline__ void backward(const QmQkArgs &a) {
     wait_for_inputs();
-    extern __shared__ float sums[];   // [WARPS][2][dim] with the gains' gradients
+    extern __shared__ float sums[];   // [WARPS][dim] with the gains' gradients
     constexpr int H = NP == 1 ? HEADS : 2;   // heads in flight
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Share t(a);
+    const bool adjacent = a.interleaved != 0;
     Lane<V, NP> l;
     l.places(a, lane);
-    float df[2][NP][V], dg[2][NP][V];
+    l.gains(a, t.is_q ? a.gain_q : a.gain_k);
+    const void *dy = t.is_q ? a.q : a.k;
+    float df[NP][V], dg[NP][V];
 #pragma unroll
-    for (int k = 0; k < 2; k++)
+    for (int i = 0; i < NP; i++)
 #pragma unroll
-        for (int i = 0; i < NP; i++)
-#pragma unroll
-            for (int v = 0; v < V; v++) df[k][i][v] = dg[k][i][v] = 0.f;
-    const int64_t tasks = (int64_t)a.tokens * a.chunks;
-    for (int64_t number = (int64_t)blockIdx.x * WARPS + warp; number < tasks; number += (int64_t)gridDim.x * WARPS) {
-        const Task t(a, number);
-        const float *row = a.x + (int64_t)t.token * a.ldx + (int64_t)t.first * a.dim;
-        float *drow = a.dx + (int64_t)t.token * a.lddx + (int64_t)t.first * a.dim;
-        const void *dy = t.is_q ? a.q : a.k;
-        const int64_t base = t.row(a);
+        for (int v = 0; v < V; v++) df[i][v] = dg[i][v] = 0.f;
+    for (int token = blockIdx.x * WARPS + warp; token < a.tokens; token += gridDim.x * WARPS) {
+        const float *row = a.x + (int64_t)token * a.ldx + (int64_t)t.first * a.dim;
+        float *drow = a.dx + (int64_t)token * a.lddx + (int64_t)t.first * a.dim;
+        const int64_t base = t.row(a, token);
         float f[H][NP][V], g[H][NP][V], p[H][NP][V], q[H][NP][V];
         auto fetch = [&](int h0) {
 #pragma unroll
@@ -294,8 +311,7 @@ __device__ __forceinline__ void backward(const QmQkArgs &a) {
                 }
         };
         fetch(t.first);
-        l.gains(a, t.is_q ? a.gain_q : a.gain_k);
-        l.angles(a, lane, t.token);
+        l.angles(a, lane, token);
         for (int h0 = t.first; h0 < t.last; h0 += H) {
             if (h0 != t.first) fetch(h0);
             float ss[4] = {0.f, 0.f, 0.f, 0.f}, dot[4] = {0.f, 0.f, 0.f, 0.f};
@@ -303,8 +319,8 @@ __device__ __forceinline__ void backward(const QmQkArgs &a) {
             for (int u = 0; u < H; u++)
 #pragma unroll
                 for (int i = 0; i < NP; i++) {
-                    regroup<V>(f[u][i], g[u][i], a.interleaved);
-                    regroup<V>(p[u][i], q[u][i], a.interleaved);
+                    regroup<V>(f[u][i], g[u][i], adjacent);
+                    regroup<V>(p[u][i], q[u][i], adjacent);
 #pragma unroll
                     for (int v = 0; v < V; v++) {
                         if (l.at[i].turns) {   // turned back
@@ -319,8 +335,8 @@ __device__ __forceinline__ void backward(const QmQkArgs &a) {
             // dx = r dz gain - (r^3 mean(dz gain x)) x; lane l: the factors of head l / 8
             float r = 1.f, m = 0.f;
             if (a.norm) {
-                r = __frsqrt_rn(warp_sum4(ss) / (float)a.dim + a.eps);
-                m = r * r * r * (warp_sum4(dot) / (float)a.dim);
+                r = __frsqrt_rn(warp_sum4(ss) * a.inv_dim + a.eps);
+                m = r * r * r * (warp_sum4(dot) * a.inv_dim);
             }
 #pragma unroll
             for (int u = 0; u < H; u++) {
@@ -330,46 +346,38 @@ __device__ __forceinline__ void backward(const QmQkArgs &a) {
 #pragma unroll
                 for (int i = 0; i < NP; i++) {
                     if (!l.at[i].there) continue;
-                    float o[V], e[V];
 #pragma unroll
                     for (int v = 0; v < V; v++) {
                         const float x = f[u][i][v], y = g[u][i][v], b = p[u][i][v], c = q[u][i][v];
-                        o[v] = ru * (b * l.w[i][v]) - mu * x;
-                        e[v] = ru * (c * l.z[i][v]) - mu * y;
-                        if (t.is_q) {
-                            df[0][i][v] += b * x * ru;
-                            dg[0][i][v] += c * y * ru;
-                        } else {
-                            df[1][i][v] += b * x * ru;
-                            dg[1][i][v] += c * y * ru;
-                        }
+                        df[i][v] += b * x * ru;
+                        dg[i][v] += c * y * ru;
+                        f[u][i][v] = ru * (b * l.w[i][v]) - mu * x;
+                        g[u][i][v] = ru * (c * l.z[i][v]) - mu * y;
                     }
-                    regroup<V>(o, e, a.interleaved);
-                    store_any<V, false>(drow, at + l.at[i].at, o);
-                    store_any<V, false>(drow, at + l.at[i].to, e);
+                    regroup<V>(f[u][i], g[u][i], adjacent);
+                    store_any<V, false>(drow, at + l.at[i].at, f[u][i]);
+                    store_any<V, false>(drow, at + l.at[i].to, g[u][i]);
                 }
             }
         }
     }
     if (!a.partial) return;
 #pragma unroll
-    for (int k = 0; k < 2; k++)
+    for (int i = 0; i < NP; i++)
+        if (l.at[i].there) {
+            regroup<V>(df[i], dg[i], adjacent);
 #pragma unroll
-        for (int i = 0; i < NP; i++)
-            if (l.at[i].there) {
-                regroup<V>(df[k][i], dg[k][i], a.interleaved);
-#pragma unroll
-                for (int v = 0; v < V; v++) {
-                    sums[(warp * 2 + k) * a.dim + l.at[i].at + v] = df[k][i][v];
-                    sums[(warp * 2 + k) * a.dim + l.at[i].to + v] = dg[k][i][v];
-                }
+            for (int v = 0; v < V; v++) {
+                sums[warp * a.dim + l.at[i].at + v] = df[i][v];
+                sums[warp * a.dim + l.at[i].to + v] = dg[i][v];
             }
+        }
     __syncthreads();
-    for (int e = threadIdx.x; e < 2 * a.dim; e += WARPS * 32) {
+    for (int e = threadIdx.x; e < a.dim; e += WARPS * 32) {
         float s = 0.f;
 #pragma unroll
-        for (int w = 0; w < WARPS; w++) s += sums[w * 2 * a.dim + e];
-        a.partial[(int64_t)blockIdx.x * 2 * a.dim + e] = s;
+        for (int w = 0; w < WARPS; w++) s += sums[w * a.dim + e];
+        a.partial[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.dim + e] = s;
     }
 }
 
@@ -383,24 +391,26 @@ extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_w1_b(const _
 extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_w2_b(const __grid_constant__ QmQkArgs a) { forward<2, 2, true>(a); }
 extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_w4_b(const __grid_constant__ QmQkArgs a) { forward<2, 4, true>(a); }
 extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_s8_b(const __grid_constant__ QmQkArgs a) { forward<1, 8, true>(a); }
-extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w1(const __grid_constant__ QmQkArgs a) { backward<2, 1, false>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32, 3) qm_qk_grad_w1(const __grid_constant__ QmQkArgs a) { backward<2, 1, false>(a); }
 extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w2(const __grid_constant__ QmQkArgs a) { backward<2, 2, false>(a); }
 extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w4(const __grid_constant__ QmQkArgs a) { backward<2, 4, false>(a); }
 extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_s8(const __grid_constant__ QmQkArgs a) { backward<1, 8, false>(a); }
-extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w1_b(const __grid_constant__ QmQkArgs a) { backward<2, 1, true>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32, 3) qm_qk_grad_w1_b(const __grid_constant__ QmQkArgs a) { backward<2, 1, true>(a); }
 extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w2_b(const __grid_constant__ QmQkArgs a) { backward<2, 2, true>(a); }
 extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w4_b(const __grid_constant__ QmQkArgs a) { backward<2, 4, true>(a); }
 extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_s8_b(const __grid_constant__ QmQkArgs a) { backward<1, 8, true>(a); }
 
-// A CTA takes 32 columns of the [2][dim] sums, its 32 warps share the CTAs' rows, everything in float64 and in one order.
+// A CTA takes 32 columns of the query (blockIdx.y 0) or key gain, its 32 warps share the CTAs' rows, everything in float64
+// and in one order.
 extern "C" __global__ void __launch_bounds__(1024) qm_qk_gain_sum(const __grid_constant__ QmGainSumArgs a) {
     wait_for_inputs();
     __shared__ double part[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+    const int first = blockIdx.y ? a.q_ctas : 0, last = blockIdx.y ? a.ctas : a.q_ctas;
     double s = 0.0;
-    if (col < 2 * a.dim) {
+    if (col < a.dim) {
 #pragma unroll 4
-        for (int c = warp; c < a.ctas; c += 32) s += (double)a.partial[(int64_t)c * 2 * a.dim + col];
+        for (int c = first + warp; c < last; c += 32) s += (double)a.partial[(int64_t)c * a.dim + col];
     }
     part[warp][lane] = s;
     __syncthreads();
@@ -408,8 +418,6 @@ extern "C" __global__ void __launch_bounds__(1024) qm_qk_gain_sum(const __grid_c
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     const int out_col = blockIdx.x * 32 + warp;
-    if (lane == 0 && out_col < 2 * a.dim) {
-        float *out = out_col < a.dim ? a.dq : a.dk;
-        if (out) out[out_col < a.dim ? out_col : out_col - a.dim] = (float)s;
-    }
+    float *out = blockIdx.y ? a.dk : a.dq;
+    if (lane == 0 && out_col < a.dim && out) out[out_col] = (float)s;
 }
