@@ -43,10 +43,23 @@ __device__ __forceinline__ float peer_f32(uint32_t addr) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
     return v;
 }
-__device__ __forceinline__ float2 peer_f32x2(uint32_t addr) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-    return v;
+// Sum over the first `split` CTAs of the cluster, in their order, of the float4 at this address of each; all are asked for
+// before the first is added.
+__device__ __forceinline__ float4 peers_sum4(uint32_t addr, int split) {
+    float4 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k < split)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v[k].x), "=f"(v[k].y), "=f"(v[k].z), "=f"(v[k].w) : "r"(peer_addr(addr, k)) : "memory");
+    }
+    float4 s = v[0];
+#pragma unroll
+    for (int k = 1; k < 8; k++) {
+        s.x += v[k].x; s.y += v[k].y; s.z += v[k].z; s.w += v[k].w;
+    }
+    return s;
 }
 // 16 bytes of which the first `bytes` are read, the others zeros.
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes) {
@@ -733,28 +746,21 @@ __device__ __forceinline__ void shrink(const QmLoraTcArgs &ta) {
         const float scale = a.scale[t.slot];
         const int rows = (t.count + QM_LORA_BLOCK - 1) / QM_LORA_BLOCK * QM_LORA_BLOCK;   // zeros behind the tokens
         constexpr int LP = QM_LORA_PITCH(RP);
-        // the CTAs take turns over the rows
-        for (int e = tid; e < ((rows - me + a.split - 1) / a.split) * (R / 2); e += SHRINK_THREADS) {
-            const int row = me + (e / (R / 2)) * a.split, r = (e % (R / 2)) * 2;
-            float2 w = make_float2(0.f, 0.f);
-            if (row < t.count) {
-                const uint32_t at = smem_u32(part + row * LD + r);
-                if (a.split > 1) {
-                    for (int k = 0; k < a.split; k++) {
-                        const float2 p = peer_f32x2(peer_addr(at, k));
-                        w.x += p.x;
-                        w.y += p.y;
-                    }
-                } else {
-                    w = *reinterpret_cast<const float2 *>(part + row * LD + r);
-                }
-            }
-            uint32_t p[3], q[3];
-            split3(r < t.rank ? w.x * scale : 0.f, p);
-            split3(r + 1 < t.rank ? w.y * scale : 0.f, q);
+        // the CTAs take turns over the rows, a thread takes four ranks
+        for (int e = tid; e < ((rows - me + a.split - 1) / a.split) * (R / 4); e += SHRINK_THREADS) {
+            const int row = me + (e / (R / 4)) * a.split, r = (e % (R / 4)) * 4;
+            float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row < t.count)
+                w = a.split > 1 ? peers_sum4(smem_u32(part + row * LD + r), a.split) : *reinterpret_cast<const float4 *>(part + row * LD + r);
+            uint32_t p[4][3];
+            split3(r < t.rank ? w.x * scale : 0.f, p[0]);
+            split3(r + 1 < t.rank ? w.y * scale : 0.f, p[1]);
+            split3(r + 2 < t.rank ? w.z * scale : 0.f, p[2]);
+            split3(r + 3 < t.rank ? w.w * scale : 0.f, p[3]);
             uint16_t *out = s.low + ((int64_t)t.row + row) * LP + r;
 #pragma unroll
-            for (int k = 0; k < 3; k++) *reinterpret_cast<uint32_t *>(out + k * R) = p[k] | q[k] << 16;
+            for (int k = 0; k < 3; k++)
+                *reinterpret_cast<uint2 *>(out + k * R) = make_uint2(p[0][k] | p[1][k] << 16, p[2][k] | p[3][k] << 16);
         }
         if (a.split > 1) {
             cluster_arrive();
@@ -1031,22 +1037,28 @@ __device__ __forceinline__ void outer(const QmLoraTcArgs &ta) {
             cluster_arrive();
             cluster_wait();
         }
-        // neighbouring threads take neighbours of the gradient's inner axis: columns of A, ranks of B
+        // The CTAs share the columns, a thread takes four of them; neighbouring threads take neighbours of the gradient's inner
+        // axis, columns of A, ranks of B.
         float *grad = s.grad + slot * s.grad_slot;
-        const int total = a.max_rank * BN, share = (total + a.split - 1) / a.split;
-        for (int e = me * share + tid; e < min(total, (me + 1) * share); e += THREADS) {
-            const int r = s.grad_col == 1 ? e / BN : e % a.max_rank, col = s.grad_col == 1 ? e % BN : e / a.max_rank;
-            if (n0 + col >= s.cols) continue;
-            float w = 0.f;
-            if (r < rank && count > 0) {
-                const uint32_t at = smem_u32(part + r * LD + col);
-                if (a.split > 1) {
-                    for (int k = 0; k < a.split; k++) w += peer_f32(peer_addr(at, k));
-                } else {
-                    w = part[r * LD + col];
-                }
+        const int quads = BN / 4 / a.split;   // of one CTA
+        const bool by_col = s.grad_rank > s.grad_col;
+        const bool vec = s.grad_col == 1 && ((reinterpret_cast<uintptr_t>(grad) | (uintptr_t)(s.grad_rank * 4)) & 15) == 0;
+        for (int e = tid; e < R * quads; e += THREADS) {
+            // (quads is a power of two)
+            const int r = by_col ? e / quads : e % R, col = (me * quads + (by_col ? e & (quads - 1) : e / R)) * 4;
+            if (r >= a.max_rank || n0 + col >= s.cols) continue;
+            float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rank && count > 0)
+                w = a.split > 1 ? peers_sum4(smem_u32(part + r * LD + col), a.split) : *reinterpret_cast<const float4 *>(part + r * LD + col);
+            float *to = grad + r * s.grad_rank + (n0 + col) * s.grad_col;
+            if (vec && n0 + col + 3 < s.cols) {
+                *reinterpret_cast<float4 *>(to) = w;
+            } else {
+                to[0] = w.x;
+                if (n0 + col + 1 < s.cols) to[s.grad_col] = w.y;
+                if (n0 + col + 2 < s.cols) to[2 * s.grad_col] = w.z;
+                if (n0 + col + 3 < s.cols) to[3 * s.grad_col] = w.w;
             }
-            grad[r * s.grad_rank + (n0 + col) * s.grad_col] = w;
         }
         if (a.split > 1) {
             cluster_arrive();
