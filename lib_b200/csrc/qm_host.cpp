@@ -130,7 +130,9 @@ static const KernelName kKernels[QM_K_COUNT] = {
     {QM_MOD_LORA, "qm_lora_outer_r64"}, {QM_MOD_LORA, "qm_lora_outer_r128"}, {QM_MOD_LORA, "qm_lora_expand_r16"},
     {QM_MOD_LORA, "qm_lora_expand_r32"}, {QM_MOD_LORA, "qm_lora_expand_r64"}, {QM_MOD_LORA, "qm_lora_expand_r128"},
     {QM_MOD_LORA, "qm_lora_expand_r16_s"}, {QM_MOD_LORA, "qm_lora_expand_r32_s"}, {QM_MOD_LORA, "qm_lora_expand_r64_s"},
-    {QM_MOD_LORA, "qm_lora_expand_r128_s"},
+    {QM_MOD_LORA, "qm_lora_expand_r128_s"}, {QM_MOD_LORA, "qm_lora_few_r16"}, {QM_MOD_LORA, "qm_lora_few_r32"},
+    {QM_MOD_LORA, "qm_lora_few_r64"}, {QM_MOD_LORA, "qm_lora_few_r128"}, {QM_MOD_LORA, "qm_lora_few_r16_s"},
+    {QM_MOD_LORA, "qm_lora_few_r32_s"}, {QM_MOD_LORA, "qm_lora_few_r64_s"}, {QM_MOD_LORA, "qm_lora_few_r128_s"},
     {QM_MOD_ROPE, "qm_qk_norm_w1"}, {QM_MOD_ROPE, "qm_qk_norm_w2"}, {QM_MOD_ROPE, "qm_qk_norm_w4"}, {QM_MOD_ROPE, "qm_qk_norm_s8"},
     {QM_MOD_ROPE, "qm_qk_norm_w1_b"}, {QM_MOD_ROPE, "qm_qk_norm_w2_b"}, {QM_MOD_ROPE, "qm_qk_norm_w4_b"}, {QM_MOD_ROPE, "qm_qk_norm_s8_b"},
     {QM_MOD_ROPE, "qm_qk_grad_w1"}, {QM_MOD_ROPE, "qm_qk_grad_w2"}, {QM_MOD_ROPE, "qm_qk_grad_w4"}, {QM_MOD_ROPE, "qm_qk_grad_s8"},
@@ -245,7 +247,7 @@ extern "C" int32_t qm_init(int32_t device, qm_ctx **out) {
             r = d->cuFuncSetAttribute(c->fn[k], CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, QM_GEMV_SMEM_MAX);
             if (r != CUDA_SUCCESS) err = (int32_t)r;
         }
-        for (int k = QM_K_LORA_ROWS; k <= QM_K_LORA_EXPAND_R128_S && !err; k++) {
+        for (int k = QM_K_LORA_ROWS; k <= QM_K_LORA_FEW_R128_S && !err; k++) {
             r = d->cuFuncSetAttribute(c->fn[k], CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, QM_GEMV_SMEM_MAX);
             if (r != CUDA_SUCCESS) err = (int32_t)r;
         }

@@ -453,6 +453,22 @@ struct QmLoraRowsArgs {
     int32_t pad_;
 };
 
+// Few bf16 tokens (qm_lora_few_*).
+#define QM_LORA_FEW 128
+struct QmLoraFewArgs {
+    const uint16_t *x;       // [tokens][ldx]
+    const int32_t *ids;      // null: slot 0
+    const float *base;       // null: zeros
+    float *y;
+    const uint16_t *a;       // [slots][rpad][cols]
+    const uint16_t *bt;      // [slots][rows][rpad]
+    const float *scale;
+    const int32_t *rank;
+    int64_t ldx, ldb, ldy;
+    int32_t rows, cols, np, slots, tokens;
+    int32_t nsplit;          // clusters that share the columns of one item
+};
+
 // Tokens in the order of their adapters (qm_lora_lists): group g < slots are the tokens of slot g, group `slots` those
 // without an adapter.
 struct QmLoraListsArgs {

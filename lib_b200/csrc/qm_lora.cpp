@@ -324,8 +324,43 @@ static int32_t batch_check(const qm_lora *l, uint64_t x, int64_t ldx, int32_t to
     return QM_OK;
 }
 
+// Up to QM_LORA_FEW tokens: one launch.
+static int32_t few_launch(qm_ctx *c, const qm_lora *l, uint64_t x, int32_t tokens, int64_t ldx, uint64_t ids_dev, uint64_t base, int64_t ldb,
+                          uint64_t y, int64_t ldy) {
+    QmLoraFewArgs a;
+    memset(&a, 0, sizeof a);
+    a.x = (const uint16_t *)(uintptr_t)x;
+    a.ids = (const int32_t *)(uintptr_t)ids_dev;
+    a.base = (const float *)(uintptr_t)base;
+    a.y = (float *)(uintptr_t)y;
+    a.a = (const uint16_t *)(uintptr_t)l->a;
+    a.bt = (const uint16_t *)(uintptr_t)l->bt;
+    a.scale = (const float *)(uintptr_t)l->scale;
+    a.rank = (const int32_t *)(uintptr_t)l->rank;
+    a.ldx = ldx;
+    a.ldb = ldb;
+    a.ldy = ldy;
+    a.rows = (int32_t)l->rows;
+    a.cols = (int32_t)l->cols;
+    a.np = (int32_t)l->np;
+    a.slots = l->slots;
+    a.tokens = tokens;
+    // Items are between one per 16 tokens and one per token; the device's clusters are dealt to as many as lie between (the
+    // geometric mean), with a piece of 256 columns per CTA at least.
+    const int64_t least = (tokens + 15) / 16, most = ids_dev ? tokens : least;
+    int64_t items = least;
+    while (items * items < least * most) items++;
+    const int64_t pieces = (l->np + QM_LORA_CLUSTER * 256 - 1) / (QM_LORA_CLUSTER * 256);
+    a.nsplit = (int32_t)std::max<int64_t>(1, std::min<int64_t>(pieces, 2 * c->sm_count / (QM_LORA_CLUSTER * items)));
+    const int64_t smem = 8 * 16 * (l->rpad + 4) * 4 + 16 * QM_LORA_EXPAND_ROW(l->rpad / 16) + (QM_LORA_FEW + 24) * 4;
+    const bool vec = !((base | y) & 7) && !((ldb | ldy) & 1);
+    return qm_launch_ex(c, (vec ? QM_K_LORA_FEW_R16 : QM_K_LORA_FEW_R16_S) + rank_kernel(l), (unsigned)(most * a.nsplit * QM_LORA_CLUSTER), 256,
+                        (unsigned)smem, &a, true, false, QM_LORA_CLUSTER);
+}
+
 static int32_t batch_launch(qm_ctx *c, const qm_lora *l, uint64_t x, int32_t tokens, int64_t ldx, uint64_t ids_dev, uint64_t base,
                             int64_t ldb, uint64_t y, int64_t ldy) {
+    if (tokens <= QM_LORA_FEW) return few_launch(c, l, x, tokens, ldx, ids_dev, base, ldb, y, ldy);
     if (ids_dev) {
         int32_t rc = lists_launch(c, l, ids_dev, tokens);
         if (rc) return rc;

@@ -411,6 +411,218 @@ extern "C" __global__ void __launch_bounds__(512) qm_lora_rows(const __grid_cons
     cluster_wait();
 }
 
+// ---- few bf16 tokens -----------------------------------------------------------------------------------------------------
+// Decode batches of up to QM_LORA_FEW tokens in one launch, without lists or a workspace. Up to 16 tokens of one adapter are
+// an item (a token without an adapter is one of its own); every CTA finds the items from the ids, cluster c of eight CTAs
+// takes item c / nsplit, and the clusters behind the last item leave. As in qm_lora_rows a CTA multiplies an eighth of the
+// columns of x with A, the sums meet in distributed shared memory and the CTA goes on with its own columns of B; the products
+// are mma with fragments straight from memory (see expand), the columns of a warp's first piece of B and of base on their way
+// before the sums meet. All that counts is the number of dependent trips to memory.
+namespace {
+
+template <int RP, bool VEC>
+__device__ __forceinline__ void few(const QmLoraFewArgs &a) {
+    wait_for_inputs();
+    extern __shared__ __align__(128) unsigned char smem[];
+    constexpr int R = RP * 16, LD = R + 4, UB = QM_LORA_EXPAND_ROW(RP);
+    constexpr int KB = RP == 1 ? 1 : RP / 2, W = RP == 1 ? 4 : 8;   // as in expand
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+    float *part = reinterpret_cast<float *>(smem);                    // [8 warps][16][LD]; the first one the CTA's sum
+    const uint32_t low = smem_u32(smem) + 8 * 16 * LD * 4;            // [16] rows of three parts
+    int32_t *ids = reinterpret_cast<int32_t *>(smem + 8 * 16 * LD * 4 + 16 * UB);   // [FEW], then [16] the item's tokens, [8]
+    int32_t *rows = ids + QM_LORA_FEW, *found = rows + 16;
+    // the item of this cluster
+    const int item = blockIdx.x / (QM_LORA_CLUSTER * a.nsplit), part_of = blockIdx.x / QM_LORA_CLUSTER % a.nsplit, me = (int)cluster_rank();
+    int mine = -1;
+    if (tid < a.tokens) {
+        mine = a.ids ? a.ids[tid] : 0;
+        if (mine < 0 || mine >= a.slots || a.rank[mine] <= 0) mine = -1;
+    }
+    if (tid < QM_LORA_FEW) ids[tid] = mine;
+    if (tid < 16) rows[tid] = -1;
+    if (tid == 0) found[4] = -1;
+    __syncthreads();
+    int before = 0;   // tokens of the same adapter before this one
+    if (tid < a.tokens)
+        for (int j = 0; j < tid; j++) before += ids[j] == mine;
+    const bool leads = tid < a.tokens && (mine < 0 || before % 16 == 0);
+    const uint32_t vote = __ballot_sync(0xffffffffu, leads);
+    if (lane == 0 && warp < 4) found[warp] = __popc(vote);
+    __syncthreads();
+    if (leads) {
+        int number = __popc(vote & ((1u << lane) - 1));
+        for (int w = 0; w < warp; w++) number += found[w];
+        if (number == item) {
+            found[4] = tid;
+            found[5] = before;
+        }
+    }
+    __syncthreads();
+    const int leader = found[4];
+    if (leader < 0) return;   // the whole cluster
+    const int slot = ids[leader];
+    const int np_cta = (((a.np + a.nsplit * QM_LORA_CLUSTER - 1) / (a.nsplit * QM_LORA_CLUSTER)) + 7) & ~7;
+    const int n0 = min((part_of * QM_LORA_CLUSTER + me) * np_cta, a.rows), nn = min(np_cta, a.rows - n0);
+    if (slot < 0) {
+        if (a.base != a.y)
+            for (int c = tid; c < nn; c += 256) a.y[leader * a.ldy + n0 + c] = a.base ? a.base[leader * a.ldb + n0 + c] : 0.f;
+        return;
+    }
+    if (tid < a.tokens && mine == slot && before >= found[5] && before < found[5] + 16) rows[before - found[5]] = tid;
+    __syncthreads();
+    const int tok[2] = {rows[g], rows[g + 8]};   // the tokens of this lane's fragment rows, -1: none
+    const int rank = a.rank[slot];
+    const float scale = a.scale[slot];
+    // narrow products: steps of 64 columns, dealt to the cluster's warps in turn; lane q has columns 16 q .. 16 q + 15 of a step
+    const int steps = (a.cols + 63) / 64;
+    const int nt = (rank + 7) / 8;
+    float acc[2 * RP][4];
+#pragma unroll
+    for (int n = 0; n < 2 * RP; n++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) acc[n][k] = 0.f;
+    const uint16_t *wa = a.a + (int64_t)slot * R * a.cols;
+    for (int st = warp * QM_LORA_CLUSTER + me; st < steps; st += 8 * QM_LORA_CLUSTER) {
+        const int k0 = st * 64 + 16 * q;
+        const bool in = k0 < a.cols;   // (a multiple of 32: both halves of a lane's columns exist or neither)
+        uint4 x[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                x[h][j] = in && tok[h] >= 0 ? *reinterpret_cast<const uint4 *>(a.x + tok[h] * a.ldx + k0 + 8 * j) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int n0t = 0; n0t < 2 * RP; n0t += 4) {
+            if (n0t >= nt) break;
+            uint4 w[4][2];
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+                if (n0t + n < 2 * RP)
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+                        w[n][j] = in ? *reinterpret_cast<const uint4 *>(wa + (int64_t)((n0t + n) * 8 + g) * a.cols + k0 + 8 * j) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+                if (n0t + n < 2 * RP)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const uint32_t fa[4] = {x[0][j].x, x[1][j].x, x[0][j].y, x[1][j].y}, fc[4] = {x[0][j].z, x[1][j].z, x[0][j].w, x[1][j].w};
+                        mma(acc[n0t + n], fa, w[n][j].x, w[n][j].y);
+                        mma(acc[n0t + n], fc, w[n][j].z, w[n][j].w);
+                    }
+        }
+    }
+    // the first piece of this warp's columns
+    float2 base[4][2];
+    uint32_t fb[KB][4][W / 2];
+    const int kb = RP == 1 ? 1 : (rank + 31) / 32;
+    auto fetch = [&](int c0) {
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int c = c0 + n * 8 + 2 * q;
+                base[n][h] = make_float2(0.f, 0.f);
+                if (a.base && tok[h] >= 0) {
+                    const float *p = a.base + tok[h] * a.ldb + n0 + c;
+                    if (VEC && c + 1 < nn) base[n][h] = *reinterpret_cast<const float2 *>(p);
+                    else {
+                        if (c < nn) base[n][h].x = p[0];
+                        if (c + 1 < nn) base[n][h].y = p[1];
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < KB; k++)
+                if (k < kb) {
+                    const uint16_t *p = a.bt + ((int64_t)slot * a.rows + min(n0 + c0 + n * 8 + g, a.rows - 1)) * R + k * 32 + W * q;
+                    if constexpr (W == 8) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+                        fb[k][n][0] = v.x; fb[k][n][1] = v.y; fb[k][n][2] = v.z; fb[k][n][3] = v.w;
+                    } else {
+                        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+                        fb[k][n][0] = v.x; fb[k][n][1] = v.y;
+                    }
+                }
+        }
+    };
+    if (warp * 32 < nn) fetch(warp * 32);
+#pragma unroll
+    for (int n = 0; n < 2 * RP; n++) {
+        float *p = part + (warp * 16 + g) * LD + n * 8 + 2 * q;
+        *reinterpret_cast<float2 *>(p) = make_float2(acc[n][0], acc[n][1]);
+        *reinterpret_cast<float2 *>(p + 8 * LD) = make_float2(acc[n][2], acc[n][3]);
+    }
+    __syncthreads();
+    for (int e = tid; e < 16 * (R / 4); e += 256) {
+        float *p = part + (e / (R / 4)) * LD + (e % (R / 4)) * 4;
+        float4 v = *reinterpret_cast<float4 *>(p);
+#pragma unroll
+        for (int w = 1; w < 8; w++) {
+            const float4 o = *reinterpret_cast<const float4 *>(p + w * 16 * LD);
+            v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+        }
+        *reinterpret_cast<float4 *>(p) = v;
+    }
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    for (int e = tid; e < 16 * (R / 4); e += 256) {
+        const int row = e / (R / 4), r = (e % (R / 4)) * 4;
+        const float4 v = peers_sum4(smem_u32(part + row * LD + r), QM_LORA_CLUSTER);
+        uint32_t p[4][3];
+        split3(r < rank ? v.x * scale : 0.f, p[0]);
+        split3(r + 1 < rank ? v.y * scale : 0.f, p[1]);
+        split3(r + 2 < rank ? v.z * scale : 0.f, p[2]);
+        split3(r + 3 < rank ? v.w * scale : 0.f, p[3]);
+        unsigned char *out = smem + 8 * 16 * LD * 4 + row * UB + r * 2;
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+            *reinterpret_cast<uint2 *>(out + k * R * 2) = make_uint2(p[0][k] | p[1][k] << 16, p[2][k] | p[3][k] << 16);
+    }
+    __syncthreads();
+    cluster_arrive();   // done with the others' memory; waited for before leaving
+    const uint32_t lm = low + (lane & 15) * UB + (lane >> 4) * 16;
+    for (int c0 = warp * 32; c0 < nn; c0 += 256) {
+        if (c0 != warp * 32) fetch(c0);
+        float d[4][4];
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) d[n][k] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KB; k++)
+            if (k < kb) {
+#pragma unroll
+                for (int p = 2; p >= 0; p--)   // the small parts first
+#pragma unroll
+                    for (int j = 0; j < W / 4; j++) {
+                        uint32_t fa[4];
+                        ldsm4(lm + (p * R + k * 32 + j * 16) * 2, fa);
+#pragma unroll
+                        for (int n = 0; n < 4; n++) mma(d[n], fa, fb[k][n][2 * j], fb[k][n][2 * j + 1]);
+                    }
+            }
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int c = c0 + n * 8 + 2 * q;
+                if (tok[h] < 0) continue;
+                float *p = a.y + tok[h] * a.ldy + n0 + c;
+                const float2 v = make_float2(base[n][h].x + d[n][2 * h], base[n][h].y + d[n][2 * h + 1]);
+                if (VEC && c + 1 < nn) *reinterpret_cast<float2 *>(p) = v;
+                else {
+                    if (c < nn) p[0] = v.x;
+                    if (c + 1 < nn) p[1] = v.y;
+                }
+            }
+    }
+    cluster_wait();
+}
+
+}  // namespace
+
 // ---- the tokens' order by adapter ----------------------------------------------------------------------------------------
 // One CTA. Every warp owns a range of tokens and counts its groups; counts of the warps before and of the groups before give
 // each token its place, so tokens keep their order inside a group, in every run.
@@ -1086,3 +1298,11 @@ extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(1) + 2) * 32
 extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(2) + 2) * 32) qm_lora_outer_r32(const __grid_constant__ QmLoraTcArgs a) { outer<2>(a); }
 extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(4) + 2) * 32) qm_lora_outer_r64(const __grid_constant__ QmLoraTcArgs a) { outer<4>(a); }
 extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(8) + 2) * 32) qm_lora_outer_r128(const __grid_constant__ QmLoraTcArgs a) { outer<8>(a); }
+extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_few_r16(const __grid_constant__ QmLoraFewArgs a) { few<1, true>(a); }
+extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_few_r16_s(const __grid_constant__ QmLoraFewArgs a) { few<1, false>(a); }
+extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_few_r32(const __grid_constant__ QmLoraFewArgs a) { few<2, true>(a); }
+extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_few_r32_s(const __grid_constant__ QmLoraFewArgs a) { few<2, false>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_few_r64(const __grid_constant__ QmLoraFewArgs a) { few<4, true>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_few_r64_s(const __grid_constant__ QmLoraFewArgs a) { few<4, false>(a); }
+extern "C" __global__ void __launch_bounds__(256) qm_lora_few_r128(const __grid_constant__ QmLoraFewArgs a) { few<8, true>(a); }
+extern "C" __global__ void __launch_bounds__(256) qm_lora_few_r128_s(const __grid_constant__ QmLoraFewArgs a) { few<8, false>(a); }
