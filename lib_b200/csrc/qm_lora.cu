@@ -429,22 +429,26 @@ __device__ __forceinline__ void few(const QmLoraFewArgs &a) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
     float *part = reinterpret_cast<float *>(smem);                    // [8 warps][16][LD]; the first one the CTA's sum
     const uint32_t low = smem_u32(smem) + 8 * 16 * LD * 4;            // [16] rows of three parts
-    int32_t *ids = reinterpret_cast<int32_t *>(smem + 8 * 16 * LD * 4 + 16 * UB);   // [FEW], then [16] the item's tokens, [8]
-    int32_t *rows = ids + QM_LORA_FEW, *found = rows + 16;
+    // behind them: [FEW] adapters, [16] the item's tokens, [8] scratch; over the sums, which come later: [4][256] tokens of a
+    // slot in a warp, [256] which slots hold an adapter
+    int32_t *ids = reinterpret_cast<int32_t *>(smem + 8 * 16 * LD * 4 + 16 * UB), *rows = ids + QM_LORA_FEW, *found = rows + 16;
+    uint8_t *count = smem, *known = smem + 1024;
     // the item of this cluster
     const int item = blockIdx.x / (QM_LORA_CLUSTER * a.nsplit), part_of = blockIdx.x / QM_LORA_CLUSTER % a.nsplit, me = (int)cluster_rank();
-    int mine = -1;
-    if (tid < a.tokens) {
-        mine = a.ids ? a.ids[tid] : 0;
-        if (mine < 0 || mine >= a.slots || a.rank[mine] <= 0) mine = -1;
-    }
-    if (tid < QM_LORA_FEW) ids[tid] = mine;
+    int mine = tid < a.tokens ? (a.ids ? a.ids[tid] : 0) : -1;
+    known[tid] = tid < a.slots && a.rank[tid] > 0;
+    reinterpret_cast<uint32_t *>(count)[tid] = 0;
     if (tid < 16) rows[tid] = -1;
     if (tid == 0) found[4] = -1;
     __syncthreads();
-    int before = 0;   // tokens of the same adapter before this one
-    if (tid < a.tokens)
-        for (int j = 0; j < tid; j++) before += ids[j] == mine;
+    if (mine < 0 || mine >= a.slots || !known[mine]) mine = -1;
+    if (tid < QM_LORA_FEW) ids[tid] = mine;
+    const uint32_t same = __match_any_sync(0xffffffffu, mine);
+    if (mine >= 0 && lane == __ffs(same) - 1) count[warp * 256 + mine] = (uint8_t)__popc(same);
+    __syncthreads();
+    int before = __popc(same & ((1u << lane) - 1));   // tokens of the same adapter before this one
+    if (mine >= 0)
+        for (int w = 0; w < warp; w++) before += count[w * 256 + mine];
     const bool leads = tid < a.tokens && (mine < 0 || before % 16 == 0);
     const uint32_t vote = __ballot_sync(0xffffffffu, leads);
     if (lane == 0 && warp < 4) found[warp] = __popc(vote);
