@@ -19,6 +19,8 @@ struct qm_lora {
     CUdeviceptr scale, rank;     // [slots]
     CUdeviceptr low[2];          // [low_rows][pitch] bf16, three parts of rpad ranks: u, v
     int64_t low_rows;
+    int32_t at_once[4];          // clusters of 1, 2, 4, 8 CTAs that run at once with one CTA per SM
+    int32_t few_at_once;         // clusters of qm_lora_few_*
     CUtensorMap w_map[2], low_map[2];
     CUdeviceptr list, offsets, tiles;
 };
@@ -46,6 +48,22 @@ static CUresult tensor_map(qm_ctx *c, CUtensorMap *map, uint64_t p, int64_t cols
     return c->drv->cuTensorMapEncodeTiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (void *)(uintptr_t)p, dims, strides, boxes, one,
                                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+static int rank_kernel(const qm_lora *l) { return l->rpad == 16 ? 0 : l->rpad == 32 ? 1 : l->rpad == 64 ? 2 : 3; }
+// Shared memory of the kernels.
+static int64_t rows_smem(const qm_lora *l) {
+    const int64_t ks = ((l->cols + QM_LORA_CLUSTER - 1) / QM_LORA_CLUSTER + 7) & ~(int64_t)7;
+    const int64_t chunk = (int64_t)l->rpad * QM_LORA_CHUNK * 2;
+    return 16ll * l->rpad * 4 + 8 * 4 + chunk + std::max<int64_t>(8 * ks * 4, 32 * QM_LORA_CHUNK * 4 + chunk);
+}
+static int64_t few_smem(const qm_lora *l) {
+    return 8 * 16 * (l->rpad + 4) * 4 + 16 * QM_LORA_EXPAND_ROW(l->rpad / 16) + (QM_LORA_FEW + 24) * 4;
+}
+static int64_t shrink_smem(const qm_lora *l) { return 1024 + QM_LORA_SHRINK_STAGES(l->rpad / 16) * (16384 + l->rpad * 128ll) + 128; }
+static int64_t outer_smem(const qm_lora *l) {
+    const int rp = l->rpad / 16;
+    return 1024 + QM_LORA_OUTER_STAGES(rp) * 8192ll * (QM_LORA_PITCH(rp) / 64 + QM_LORA_OUTER_COLS(rp) / 64) + 128;
 }
 
 extern "C" int32_t qm_lora_create(qm_ctx *c, int64_t rows, int64_t cols, int32_t adapters, int32_t max_rank, int32_t max_tokens,
@@ -93,6 +111,9 @@ extern "C" int32_t qm_lora_create(qm_ctx *c, int64_t rows, int64_t cols, int32_t
         lora_release(c, l);
         return (int32_t)r;
     }
+    for (int i = 0; i < 4; i++)
+        l->at_once[i] = qm_max_clusters(c, QM_K_LORA_OUTER_R16 + rank_kernel(l), 1 << i, (QM_LORA_OUTER_READERS(l->rpad / 16) + 2) * 32, (unsigned)outer_smem(l));
+    l->few_at_once = qm_max_clusters(c, QM_K_LORA_FEW_R16 + rank_kernel(l), QM_LORA_CLUSTER, 256, (unsigned)few_smem(l));
     *out = l;
     return QM_OK;
 }
@@ -187,13 +208,11 @@ static int32_t rows_launch(qm_ctx *c, const qm_lora *l, uint64_t x_dev, uint64_t
     a.m = m;
     a.xop = (int32_t)(flags & 0xFu);
     a.eps = 1e-6f;
-    // clusters per row: no more than run at once, and none with less than a chunk of columns per CTA
+    // clusters per row: no more than run at once (one CTA per SM), and none with less than a chunk of columns per CTA. (Eight
+    // rows of 6144 columns: 9.2 us with one, 13.6 with two, of which one has to wait; five of 10007: 9.8, 8.3 and with three 7.3.)
     const int64_t most = (l->np + QM_LORA_CLUSTER * QM_LORA_CHUNK - 1) / (QM_LORA_CLUSTER * QM_LORA_CHUNK);
-    a.nsplit = (int32_t)std::max<int64_t>(1, std::min<int64_t>(most, c->sm_count / (QM_LORA_CLUSTER * m)));
-    const int64_t ks = ((l->cols + QM_LORA_CLUSTER - 1) / QM_LORA_CLUSTER + 7) & ~(int64_t)7;
-    const int64_t chunk = (int64_t)l->rpad * QM_LORA_CHUNK * 2;
-    const int64_t smem = 16ll * l->rpad * 4 + 8 * 4 + chunk + std::max<int64_t>(8 * ks * 4, 32 * QM_LORA_CHUNK * 4 + chunk);
-    if (smem > QM_GEMV_SMEM_MAX) return QM_ERR_LIMIT;
+    a.nsplit = (int32_t)std::max<int64_t>(1, std::min<int64_t>(most, l->at_once[3] / m));
+    const int64_t smem = rows_smem(l);
     return qm_launch_ex(c, QM_K_LORA_ROWS, (unsigned)(m * a.nsplit * QM_LORA_CLUSTER), 512, (unsigned)smem, &a, true, false, QM_LORA_CLUSTER);
 }
 
@@ -224,8 +243,6 @@ extern "C" int32_t qm_matvec_lora(qm_ctx *c, qm_weight h, qm_lora *l, uint64_t x
 }
 
 // ---- bf16 batches ----------------------------------------------------------------------------------
-static int rank_kernel(const qm_lora *l) { return l->rpad == 16 ? 0 : l->rpad == 32 ? 1 : l->rpad == 64 ? 2 : 3; }
-
 static int32_t lists_launch(qm_ctx *c, const qm_lora *l, uint64_t ids_dev, int32_t tokens) {
     QmLoraListsArgs a;
     memset(&a, 0, sizeof a);
@@ -272,13 +289,15 @@ static int32_t batch_args(qm_ctx *c, QmLoraTcArgs *ta, const qm_lora *l, uint64_
     return QM_OK;
 }
 
-// CTAs that share one piece of work of `steps` steps, `at_once` CTAs running at a time: 1, 2, 4 or 8, whichever takes the
-// fewest steps in all, a CTA's start and end counted as eight.
-static int32_t share(int64_t units, int64_t steps, int64_t at_once) {
+// CTAs that share one piece of work of `steps` steps, `per_sm` CTAs on an SM: 1, 2, 4 or 8, whichever takes the fewest steps
+// in all, a CTA's start and end counted as ten. (Clusters of eight leave 28 of the 148 SMs idle.)
+static int32_t share(const qm_lora *l, int64_t units, int64_t steps, int per_sm) {
     int32_t best = 1;
     int64_t least = INT64_MAX;
-    for (int32_t s = 1; s <= 8; s *= 2) {
-        const int64_t cost = (units * s + at_once - 1) / at_once * ((steps + s - 1) / s + 8);
+    for (int i = 0; i < 4; i++) {
+        const int32_t s = 1 << i;
+        const int64_t clusters = (int64_t)per_sm * std::max(1, l->at_once[i]);
+        const int64_t cost = (units + clusters - 1) / clusters * ((steps + s - 1) / s + 10);
         if (cost < least) {
             least = cost;
             best = s;
@@ -292,11 +311,9 @@ static int32_t shrink_launch(qm_ctx *c, const qm_lora *l, QmLoraTcArgs *ta, int 
     const int64_t cols = sides == 2 ? std::max(l->cols, l->rows) : l->cols;
     a->first_side = sides == 2 && l->rows > l->cols;   // the longer one first, the shorter one fills its last wave
     // (the tiles that are there for certain; those that short lists add come on top)
-    a->split = share(sides * (int64_t)((a->tokens + QM_LORA_TILE - 1) / QM_LORA_TILE), (cols + 63) / 64, 2ll * c->sm_count);
-    const int rp = l->rpad / 16;
-    const int64_t smem = 1024 + QM_LORA_SHRINK_STAGES(rp) * (16384 + l->rpad * 128ll) + 128;
-    return qm_launch_ex(c, QM_K_LORA_SHRINK_R16 + rank_kernel(l), (unsigned)(sides * a->tiles_max * a->split), 192, (unsigned)smem, ta, true,
-                        false, a->split);
+    a->split = share(l, sides * (int64_t)((a->tokens + QM_LORA_TILE - 1) / QM_LORA_TILE), (cols + 63) / 64, 2);
+    return qm_launch_ex(c, QM_K_LORA_SHRINK_R16 + rank_kernel(l), (unsigned)(sides * a->tiles_max * a->split), 192, (unsigned)shrink_smem(l), ta,
+                        true, false, a->split);
 }
 
 static int32_t expand_launch(qm_ctx *c, const qm_lora *l, QmLoraBatchArgs *a, int out_side, uint64_t base, int64_t ldb, uint64_t y,
@@ -345,14 +362,13 @@ static int32_t few_launch(qm_ctx *c, const qm_lora *l, uint64_t x, int32_t token
     a.np = (int32_t)l->np;
     a.slots = l->slots;
     a.tokens = tokens;
-    // Items are between one per 16 tokens and one per token; the device's clusters are dealt to as many as lie between (the
-    // geometric mean), with a piece of 256 columns per CTA at least.
-    const int64_t least = (tokens + 15) / 16, most = ids_dev ? tokens : least;
-    int64_t items = least;
-    while (items * items < least * most) items++;
+    // There may be as many items as tokens, and clusters that find none cost as much to launch: the columns of an item are
+    // shared by more clusters only while all of them run at once, with 256 columns per CTA at least. (64 tokens on 32 adapters,
+    // 6144 columns: one cluster per item 9.3 us, two 14.1, three 15.8.)
+    const int64_t most = ids_dev ? tokens : (tokens + 15) / 16;
     const int64_t pieces = (l->np + QM_LORA_CLUSTER * 256 - 1) / (QM_LORA_CLUSTER * 256);
-    a.nsplit = (int32_t)std::max<int64_t>(1, std::min<int64_t>(pieces, 2 * c->sm_count / (QM_LORA_CLUSTER * items)));
-    const int64_t smem = 8 * 16 * (l->rpad + 4) * 4 + 16 * QM_LORA_EXPAND_ROW(l->rpad / 16) + (QM_LORA_FEW + 24) * 4;
+    a.nsplit = (int32_t)std::max<int64_t>(1, std::min<int64_t>(pieces, l->few_at_once / most));
+    const int64_t smem = few_smem(l);
     const bool vec = !((base | y) & 7) && !((ldb | ldy) & 1);
     return qm_launch_ex(c, (vec ? QM_K_LORA_FEW_R16 : QM_K_LORA_FEW_R16_S) + rank_kernel(l), (unsigned)(most * a.nsplit * QM_LORA_CLUSTER), 256,
                         (unsigned)smem, &a, true, false, QM_LORA_CLUSTER);
@@ -447,10 +463,8 @@ extern "C" int32_t qm_lora_backward(qm_ctx *c, qm_lora *l, uint64_t x_bf16_dev, 
     const int64_t ba = (l->cols + bn - 1) / bn, bb = (l->rows + bn - 1) / bn;
     const int64_t slots = ids_dev ? std::min(l->slots, tokens) : 1;
     a.outer_units = (int32_t)(std::max(ba, bb) * l->slots);
-    a.split = share(((da_dev ? ba : 0) + (db_dev ? bb : 0)) * slots, (tokens / slots + 63) / 64, c->sm_count);
-    const int64_t smem = 1024 + QM_LORA_OUTER_STAGES(rp) * 8192ll * (QM_LORA_PITCH(rp) / 64 + bn / 64) + 128;
+    a.split = share(l, ((da_dev ? ba : 0) + (db_dev ? bb : 0)) * slots, (tokens / slots + 63) / 64, 1);
     if (2ll * a.outer_units * a.split > 0x7FFFFFFF) return QM_ERR_LIMIT;
     return qm_launch_ex(c, QM_K_LORA_OUTER_R16 + rank_kernel(l), (unsigned)(2 * a.outer_units * a.split), (QM_LORA_OUTER_READERS(rp) + 2) * 32,
-                        (unsigned)smem, &ta, true, false,
-                        a.split);
+                        (unsigned)outer_smem(l), &ta, true, false, a.split);
 }

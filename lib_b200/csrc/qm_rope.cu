@@ -81,19 +81,6 @@ __device__ __forceinline__ void load_f32(const float *p, float (&v)[V]) {
 }
 
 template <int V, bool BF16>
-__device__ __forceinline__ void load_any(const void *base, int64_t at, float (&v)[V]) {
-    if constexpr (!BF16) {
-        load_f32<V>(reinterpret_cast<const float *>(base) + at, v);
-    } else if constexpr (V == 2) {
-        const uint32_t t = *reinterpret_cast<const uint32_t *>(reinterpret_cast<const uint16_t *>(base) + at);
-        v[0] = __uint_as_float(t << 16);
-        v[1] = __uint_as_float(t & 0xFFFF0000u);
-    } else {
-        v[0] = __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(base)[at] << 16);
-    }
-}
-
-template <int V, bool BF16>
 __device__ __forceinline__ void store_any(void *base, int64_t at, const float (&v)[V]) {
     if constexpr (!BF16) {
         float *p = reinterpret_cast<float *>(base) + at;
@@ -268,13 +255,42 @@ __device__ __forceinline__ void forward(const QmQkArgs &a) {
     }
 }
 
-// A warp walks tokens; what it adds up for the gains stays in its registers, the CTA's warps are added in warp order and
-// qm_qk_gain_sum adds the CTAs in their order: the same bits in every run.
+// Two heads as they come from memory; gradients keep their type until they are used.
+template <int V, int NP, bool BF16>
+struct Pair {
+    float f[2][NP][V], g[2][NP][V];
+    uint32_t p[2][NP][V], q[2][NP][V];   // float32 bits, or in element 0 the bf16 of the whole vector
+
+    __device__ __forceinline__ static void raw(const void *base, int64_t at, uint32_t (&v)[V]) {
+        if constexpr (!BF16) {
+            float t[V];
+            load_f32<V>(reinterpret_cast<const float *>(base) + at, t);
+#pragma unroll
+            for (int i = 0; i < V; i++) v[i] = __float_as_uint(t[i]);
+        } else if constexpr (V == 2) {
+            v[0] = *reinterpret_cast<const uint32_t *>(reinterpret_cast<const uint16_t *>(base) + at);
+        } else {
+            v[0] = reinterpret_cast<const uint16_t *>(base)[at];
+        }
+    }
+    __device__ __forceinline__ static void values(const uint32_t (&v)[V], float (&t)[V]) {
+        if constexpr (!BF16) {
+#pragma unroll
+            for (int i = 0; i < V; i++) t[i] = __uint_as_float(v[i]);
+        } else {
+            t[0] = __uint_as_float(v[0] << 16);
+            if constexpr (V == 2) t[1] = __uint_as_float(v[0] & 0xFFFF0000u);
+        }
+    }
+};
+
+// A warp walks tokens, two heads at a time, the next two on their way while two are worked on; what it adds up for the gains
+// stays in its registers, the CTA's warps are added in warp order and qm_qk_gain_sum adds the CTAs in their order: the same
+// bits in every run.
 template <int V, int NP, bool BF16>
 __device__ __forceinline__ void backward(const QmQkArgs &a) {
     wait_for_inputs();
     extern __shared__ float sums[];   // [WARPS][dim] with the gains' gradients
-    constexpr int H = NP == 1 ? HEADS : 2;   // heads in flight
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const Share t(a);
     const bool adjacent = a.interleaved != 0;
@@ -287,78 +303,108 @@ __device__ __forceinline__ void backward(const QmQkArgs &a) {
     for (int i = 0; i < NP; i++)
 #pragma unroll
         for (int v = 0; v < V; v++) df[i][v] = dg[i][v] = 0.f;
-    for (int token = blockIdx.x * WARPS + warp; token < a.tokens; token += gridDim.x * WARPS) {
-        const float *row = a.x + (int64_t)token * a.ldx + (int64_t)t.first * a.dim;
-        float *drow = a.dx + (int64_t)token * a.lddx + (int64_t)t.first * a.dim;
-        const int64_t base = t.row(a, token);
-        float f[H][NP][V], g[H][NP][V], p[H][NP][V], q[H][NP][V];
-        auto fetch = [&](int h0) {
+    const int stride = gridDim.x * WARPS;
+    auto fetch = [&](Pair<V, NP, BF16> &b, int token, int h0) {
+        const float *row = a.x + (int64_t)token * a.ldx + (int64_t)h0 * a.dim;
+        const int64_t base = t.row(a, token) + (h0 - t.first) * a.dim;
 #pragma unroll
-            for (int u = 0; u < H; u++)
+        for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int i = 0; i < NP; i++) {
+            for (int i = 0; i < NP; i++) {
 #pragma unroll
-                    for (int v = 0; v < V; v++) f[u][i][v] = g[u][i][v] = p[u][i][v] = q[u][i][v] = 0.f;
-                    if (h0 + u < t.last && l.at[i].there) {
-                        const int at = (h0 - t.first + u) * a.dim;
-                        if (a.norm) {
-                            load_f32<V>(row + at + l.at[i].at, f[u][i]);
-                            load_f32<V>(row + at + l.at[i].to, g[u][i]);
-                        }
-                        load_any<V, BF16>(dy, base + at + l.at[i].at, p[u][i]);
-                        load_any<V, BF16>(dy, base + at + l.at[i].to, q[u][i]);
-                    }
+                for (int v = 0; v < V; v++) {
+                    b.f[u][i][v] = b.g[u][i][v] = 0.f;
+                    b.p[u][i][v] = b.q[u][i][v] = 0u;
                 }
-        };
-        fetch(t.first);
-        l.angles(a, lane, token);
-        for (int h0 = t.first; h0 < t.last; h0 += H) {
-            if (h0 != t.first) fetch(h0);
-            float ss[4] = {0.f, 0.f, 0.f, 0.f}, dot[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int u = 0; u < H; u++)
-#pragma unroll
-                for (int i = 0; i < NP; i++) {
-                    regroup<V>(f[u][i], g[u][i], adjacent);
-                    regroup<V>(p[u][i], q[u][i], adjacent);
-#pragma unroll
-                    for (int v = 0; v < V; v++) {
-                        if (l.at[i].turns) {   // turned back
-                            const float b = p[u][i][v], c = q[u][i][v];
-                            p[u][i][v] = b * l.cs[i][v] + c * l.sn[i][v];
-                            q[u][i][v] = c * l.cs[i][v] - b * l.sn[i][v];
-                        }
-                        ss[u] += f[u][i][v] * f[u][i][v] + g[u][i][v] * g[u][i][v];
-                        dot[u] += p[u][i][v] * f[u][i][v] * l.w[i][v] + q[u][i][v] * g[u][i][v] * l.z[i][v];
+                if (h0 + u < t.last && l.at[i].there) {
+                    if (a.norm) {
+                        load_f32<V>(row + u * a.dim + l.at[i].at, b.f[u][i]);
+                        load_f32<V>(row + u * a.dim + l.at[i].to, b.g[u][i]);
                     }
-                }
-            // dx = r dz gain - (r^3 mean(dz gain x)) x; lane l: the factors of head l / 8
-            float r = 1.f, m = 0.f;
-            if (a.norm) {
-                r = __frsqrt_rn(warp_sum4(ss) * a.inv_dim + a.eps);
-                m = r * r * r * (warp_sum4(dot) * a.inv_dim);
-            }
-#pragma unroll
-            for (int u = 0; u < H; u++) {
-                const float ru = __shfl_sync(0xffffffffu, r, 8 * u), mu = __shfl_sync(0xffffffffu, m, 8 * u);
-                if (h0 + u >= t.last) break;
-                const int at = (h0 - t.first + u) * a.dim;
-#pragma unroll
-                for (int i = 0; i < NP; i++) {
-                    if (!l.at[i].there) continue;
-#pragma unroll
-                    for (int v = 0; v < V; v++) {
-                        const float x = f[u][i][v], y = g[u][i][v], b = p[u][i][v], c = q[u][i][v];
-                        df[i][v] += b * x * ru;
-                        dg[i][v] += c * y * ru;
-                        f[u][i][v] = ru * (b * l.w[i][v]) - mu * x;
-                        g[u][i][v] = ru * (c * l.z[i][v]) - mu * y;
-                    }
-                    regroup<V>(f[u][i], g[u][i], adjacent);
-                    store_any<V, false>(drow, at + l.at[i].at, f[u][i]);
-                    store_any<V, false>(drow, at + l.at[i].to, g[u][i]);
+                    b.raw(dy, base + u * a.dim + l.at[i].at, b.p[u][i]);
+                    b.raw(dy, base + u * a.dim + l.at[i].to, b.q[u][i]);
                 }
             }
+    };
+    auto work = [&](Pair<V, NP, BF16> &b, int token, int h0) {
+        float *drow = a.dx + (int64_t)token * a.lddx + (int64_t)h0 * a.dim;
+        if (h0 == t.first) l.angles(a, lane, token);
+        float p[2][NP][V], q[2][NP][V], sum[4] = {0.f, 0.f, 0.f, 0.f};   // the squares of both heads, then their products
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                b.values(b.p[u][i], p[u][i]);
+                b.values(b.q[u][i], q[u][i]);
+                regroup<V>(b.f[u][i], b.g[u][i], adjacent);
+                regroup<V>(p[u][i], q[u][i], adjacent);
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    if (l.at[i].turns) {   // turned back
+                        const float y = p[u][i][v], z = q[u][i][v];
+                        p[u][i][v] = y * l.cs[i][v] + z * l.sn[i][v];
+                        q[u][i][v] = z * l.cs[i][v] - y * l.sn[i][v];
+                    }
+                    sum[u] += b.f[u][i][v] * b.f[u][i][v] + b.g[u][i][v] * b.g[u][i][v];
+                    sum[2 + u] += p[u][i][v] * b.f[u][i][v] * l.w[i][v] + q[u][i][v] * b.g[u][i][v] * l.z[i][v];
+                }
+            }
+        // dx = r dz gain - (r^3 mean(dz gain x)) x
+        float s = 0.f, r = 1.f;
+        if (a.norm) {
+            s = warp_sum4(sum) * a.inv_dim;
+            r = __frsqrt_rn(s + a.eps);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const float ru = __shfl_sync(0xffffffffu, r, 8 * u), mu = a.norm ? ru * ru * ru * __shfl_sync(0xffffffffu, s, 16 + 8 * u) : 0.f;
+            if (h0 + u >= t.last) break;
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                if (!l.at[i].there) continue;
+                float o[V], e[V];
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    const float x = b.f[u][i][v], y = b.g[u][i][v], c = p[u][i][v], d = q[u][i][v];
+                    df[i][v] += c * x * ru;
+                    dg[i][v] += d * y * ru;
+                    o[v] = ru * (c * l.w[i][v]) - mu * x;
+                    e[v] = ru * (d * l.z[i][v]) - mu * y;
+                }
+                regroup<V>(o, e, adjacent);
+                store_any<V, false>(drow, u * a.dim + l.at[i].at, o);
+                store_any<V, false>(drow, u * a.dim + l.at[i].to, e);
+            }
+        }
+    };
+    auto after = [&](int &token, int &h0) {
+        h0 += 2;
+        if (h0 >= t.last) {
+            h0 = t.first;
+            token += stride;
+        }
+    };
+    int token = blockIdx.x * WARPS + warp, h0 = t.first;
+    if constexpr (NP <= 2) {
+        Pair<V, NP, BF16> b, c;
+        if (token < a.tokens) fetch(b, token, h0);
+        while (token < a.tokens) {
+            int token2 = token, h2 = h0;
+            after(token2, h2);
+            if (token2 < a.tokens) fetch(c, token2, h2);
+            work(b, token, h0);
+            if (token2 >= a.tokens) break;
+            token = token2;
+            h0 = h2;
+            after(token, h0);
+            if (token < a.tokens) fetch(b, token, h0);
+            work(c, token2, h2);
+        }
+    } else {   // (two such pairs do not fit in the registers)
+        for (; token < a.tokens; after(token, h0)) {
+            Pair<V, NP, BF16> b;
+            fetch(b, token, h0);
+            work(b, token, h0);
         }
     }
     if (!a.partial) return;
@@ -392,11 +438,11 @@ extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_w2_b(const _
 extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_w4_b(const __grid_constant__ QmQkArgs a) { forward<2, 4, true>(a); }
 extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_norm_s8_b(const __grid_constant__ QmQkArgs a) { forward<1, 8, true>(a); }
 extern "C" __global__ void __launch_bounds__(WARPS * 32, 3) qm_qk_grad_w1(const __grid_constant__ QmQkArgs a) { backward<2, 1, false>(a); }
-extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w2(const __grid_constant__ QmQkArgs a) { backward<2, 2, false>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32, 2) qm_qk_grad_w2(const __grid_constant__ QmQkArgs a) { backward<2, 2, false>(a); }
 extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w4(const __grid_constant__ QmQkArgs a) { backward<2, 4, false>(a); }
 extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_s8(const __grid_constant__ QmQkArgs a) { backward<1, 8, false>(a); }
 extern "C" __global__ void __launch_bounds__(WARPS * 32, 3) qm_qk_grad_w1_b(const __grid_constant__ QmQkArgs a) { backward<2, 1, true>(a); }
-extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w2_b(const __grid_constant__ QmQkArgs a) { backward<2, 2, true>(a); }
+extern "C" __global__ void __launch_bounds__(WARPS * 32, 2) qm_qk_grad_w2_b(const __grid_constant__ QmQkArgs a) { backward<2, 2, true>(a); }
 extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_w4_b(const __grid_constant__ QmQkArgs a) { backward<2, 4, true>(a); }
 extern "C" __global__ void __launch_bounds__(WARPS * 32) qm_qk_grad_s8_b(const __grid_constant__ QmQkArgs a) { backward<1, 8, true>(a); }
 
