@@ -208,7 +208,9 @@ QM_API int32_t qm_matmul_bf16(qm_ctx *ctx, qm_weight w, uint64_t a_dev, int32_t 
  * qm_lora_matvec: 1..8 float32 rows, x, x2 and flags as for qm_matvec (the same input transforms f); for single tokens.
  * qm_lora_matmul_bf16: any number of tokens up to max_tokens, x bf16 [tokens][ldx] (16-byte aligned, ldx a multiple
  *   of 8), f the identity.
- * qm_lora_backward: gradients of qm_lora_matmul_bf16. dy bf16 [tokens][lddy] (16-byte aligned, lddy a multiple of 8):
+ * qm_lora_backward: gradients of qm_lora_matmul_bf16. dy bf16 [tokens][lddy]; where it is not 16-byte aligned with lddy a
+ *   multiple of 8 it is copied first, into memory of the handle that the first such call allocates (it is refused under
+ *   capture with CUDA_ERROR_STREAM_CAPTURE_UNSUPPORTED):
  *   dx[t] = base[t] + scale_a A_a^T (B_a^T dy[t])   float32 [tokens][lddx] (base: the frozen weights' share, as above)
  *   da[a] = scale_a sum_t (B_a^T dy[t]) x[t]^T      float32 [adapters][max_rank][cols]
  *   db[a] = scale_a sum_t dy[t] (A_a x[t])^T        float32 [adapters][rows][max_rank]

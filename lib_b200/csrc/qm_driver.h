@@ -44,6 +44,7 @@
     X(cuGraphLaunch, CUresult (*)(CUgraphExec, CUstream))                                         \
     X(cuGraphExecDestroy, CUresult (*)(CUgraphExec))                                              \
     X(cuGraphDestroy, CUresult (*)(CUgraph))                                                      \
+    X(cuStreamWaitEvent, CUresult (*)(CUstream, CUevent, unsigned int))                           \
     X(cuEventCreate, CUresult (*)(CUevent *, unsigned int))                                       \
     X(cuEventRecord, CUresult (*)(CUevent, CUstream))                                             \
     X(cuEventSynchronize, CUresult (*)(CUevent))                                                  \

@@ -124,7 +124,7 @@ static const KernelName kKernels[QM_K_COUNT] = {
     {QM_MOD_Q4K, "qm_fused_q4k_dd_c2d2_x4"}, {QM_MOD_Q4K, "qm_fused_q4k_dd_c2d3_x4"}, {QM_MOD_Q4K, "qm_fused_q4k_dd_c2d4_x4"},
     {QM_MOD_Q4K, "qm_fused_q4k_dd_n2d2_x4"}, {QM_MOD_Q4K, "qm_fused_q4k_dd_n2d3_x4"},
     {QM_MOD_Q4K, "qm_fused_q4k_dd_n2d2"}, {QM_MOD_Q4K, "qm_fused_q4k_dd_n2d3"},
-    {QM_MOD_LORA, "qm_lora_set"},      {QM_MOD_LORA, "qm_lora_rows"},     {QM_MOD_LORA, "qm_lora_lists"},
+    {QM_MOD_LORA, "qm_lora_set"},      {QM_MOD_LORA, "qm_lora_align"},      {QM_MOD_LORA, "qm_lora_rows"},     {QM_MOD_LORA, "qm_lora_lists"},
     {QM_MOD_LORA, "qm_lora_shrink_r16"}, {QM_MOD_LORA, "qm_lora_shrink_r32"}, {QM_MOD_LORA, "qm_lora_shrink_r64"},
     {QM_MOD_LORA, "qm_lora_shrink_r128"}, {QM_MOD_LORA, "qm_lora_outer_r16"}, {QM_MOD_LORA, "qm_lora_outer_r32"},
     {QM_MOD_LORA, "qm_lora_outer_r64"}, {QM_MOD_LORA, "qm_lora_outer_r128"}, {QM_MOD_LORA, "qm_lora_expand_r16"},

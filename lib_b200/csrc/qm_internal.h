@@ -34,7 +34,7 @@ enum {
     QM_K_LEAN_SUM, QM_K_Q40_LEAN_X2_D4, QM_K_Q40_LEAN_X2_D2, QM_K_Q80_LEAN_X2_D2,
     QM_K_DD_X4_C2D2, QM_K_DD_X4_C2D3, QM_K_DD_X4_C2D4, QM_K_DD_X4_N2D2, QM_K_DD_X4_N2D3,
     QM_K_FUSED_Q4K_DD_N2D2, QM_K_FUSED_Q4K_DD_N2D3,
-    QM_K_LORA_SET, QM_K_LORA_ROWS, QM_K_LORA_LISTS, QM_K_LORA_SHRINK_R16, QM_K_LORA_SHRINK_R32, QM_K_LORA_SHRINK_R64,
+    QM_K_LORA_SET, QM_K_LORA_ALIGN, QM_K_LORA_ROWS, QM_K_LORA_LISTS, QM_K_LORA_SHRINK_R16, QM_K_LORA_SHRINK_R32, QM_K_LORA_SHRINK_R64,
     QM_K_LORA_SHRINK_R128, QM_K_LORA_OUTER_R16, QM_K_LORA_OUTER_R32, QM_K_LORA_OUTER_R64, QM_K_LORA_OUTER_R128,
     QM_K_LORA_EXPAND_R16, QM_K_LORA_EXPAND_R32, QM_K_LORA_EXPAND_R64, QM_K_LORA_EXPAND_R128,
     QM_K_LORA_EXPAND_R16_S, QM_K_LORA_EXPAND_R32_S, QM_K_LORA_EXPAND_R64_S, QM_K_LORA_EXPAND_R128_S,

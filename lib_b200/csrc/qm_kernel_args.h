@@ -481,6 +481,14 @@ struct QmLoraListsArgs {
     int32_t tokens, slots, tiles_max, pad_;
 };
 
+// rows x cols bf16 from rows `ld` elements apart to rows `pitch` elements apart, zeros behind the columns (qm_lora_align).
+struct QmLoraAlignArgs {
+    const uint16_t *src;
+    uint16_t *dst;
+    int64_t ld, pitch;
+    int32_t rows, cols;
+};
+
 // One product with a narrow matrix: a side of the adapters. Forward: x with A; backward also dy with B.
 struct QmLoraSide {
     const uint16_t *wt;      // [slots][cols][rpad] bf16

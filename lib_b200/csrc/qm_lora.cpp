@@ -21,8 +21,11 @@ struct qm_lora {
     int64_t low_rows;
     int32_t at_once[4];          // clusters of 1, 2, 4, 8 CTAs that run at once with one CTA per SM
     int32_t few_at_once;         // clusters of qm_lora_few_*
+    CUstream side;               // the backward pass: dx beside the gradients of A and B
+    CUevent fork, join;
     CUtensorMap w_map[2], low_map[2];
     CUdeviceptr list, offsets, tiles;
+    CUdeviceptr aligned;         // [max_tokens][np] bf16, from the first backward pass on whose dy no tensor map takes
 };
 
 static int32_t lora_check(qm_ctx *c, const qm_lora *l) { return l && l->magic == QM_LORA_MAGIC && l->ctx == c ? QM_OK : QM_ERR_ARG; }
@@ -34,9 +37,12 @@ static int64_t lora_tiles(const qm_lora *l, int64_t tokens, bool listed) {
 }
 
 static void lora_release(qm_ctx *c, qm_lora *l) {
-    CUdeviceptr all[] = {l->a, l->b, l->at, l->bt, l->scale, l->rank, l->low[0], l->low[1], l->list, l->offsets, l->tiles};
+    CUdeviceptr all[] = {l->a, l->b, l->at, l->bt, l->scale, l->rank, l->low[0], l->low[1], l->list, l->offsets, l->tiles, l->aligned};
     for (CUdeviceptr p : all)
         if (p) c->drv->cuMemFree_v2(p);
+    if (l->fork) c->drv->cuEventDestroy_v2(l->fork);
+    if (l->join) c->drv->cuEventDestroy_v2(l->join);
+    if (l->side) c->drv->cuStreamDestroy_v2(l->side);
     l->magic = 0;
     delete l;
 }
@@ -101,6 +107,9 @@ extern "C" int32_t qm_lora_create(qm_ctx *c, int64_t rows, int64_t cols, int32_t
     for (auto &n : need)
         if (r == CUDA_SUCCESS) r = c->drv->cuMemAlloc_v2(n.p, (size_t)n.bytes);
     if (r == CUDA_SUCCESS) r = c->drv->cuMemsetD8Async(l->rank, 0, (size_t)adapters * 4, c->stream);
+    if (r == CUDA_SUCCESS) r = c->drv->cuStreamCreate(&l->side, CU_STREAM_NON_BLOCKING);
+    if (r == CUDA_SUCCESS) r = c->drv->cuEventCreate(&l->fork, CU_EVENT_DISABLE_TIMING);
+    if (r == CUDA_SUCCESS) r = c->drv->cuEventCreate(&l->join, CU_EVENT_DISABLE_TIMING);
     const int64_t wide[2] = {cols, rows}, w_pitch[2] = {cols, l->np};
     const CUdeviceptr w[2] = {l->a, l->b};
     for (int i = 0; i < 2; i++) {
@@ -413,6 +422,29 @@ extern "C" int32_t qm_matmul_bf16_lora(qm_ctx *c, qm_weight h, qm_lora *l, uint6
     return batch_launch(c, l, a_dev, m, lda, ids_dev, c_dev, ldc, c_dev, ldc);
 }
 
+// dy where a tensor map takes it: itself, or a copy in the handle (of its full size at once, so that no later call moves it).
+static int32_t align_dy(qm_ctx *c, qm_lora *l, uint64_t *dy, int64_t *lddy, int32_t tokens) {
+    if (!(*dy & 15) && !(*lddy & 7)) return QM_OK;
+    if (!l->aligned) {
+        CUstreamCaptureStatus capturing = CU_STREAM_CAPTURE_STATUS_NONE;
+        DRV(c->drv->cuStreamIsCapturing(c->stream, &capturing));
+        if (capturing != CU_STREAM_CAPTURE_STATUS_NONE) return CUDA_ERROR_STREAM_CAPTURE_UNSUPPORTED;
+        DRV(c->drv->cuMemAlloc_v2(&l->aligned, (size_t)l->max_tokens * l->np * 2));
+    }
+    QmLoraAlignArgs a;
+    memset(&a, 0, sizeof a);
+    a.src = (const uint16_t *)(uintptr_t)*dy;
+    a.dst = (uint16_t *)(uintptr_t)l->aligned;
+    a.ld = *lddy;
+    a.pitch = l->np;
+    a.rows = tokens;
+    a.cols = (int32_t)l->rows;
+    *dy = l->aligned;
+    *lddy = l->np;
+    const int64_t work = ((int64_t)tokens * l->np / 8 + 255) / 256;
+    return qm_launch(c, QM_K_LORA_ALIGN, (unsigned)std::min<int64_t>(work, 8ll * c->sm_count), 1, 256, 0, &a, true);
+}
+
 extern "C" int32_t qm_lora_backward(qm_ctx *c, qm_lora *l, uint64_t x_bf16_dev, int64_t ldx, uint64_t dy_bf16_dev, int64_t lddy,
                                     int32_t tokens, uint64_t ids_dev, uint64_t base_dev, int64_t ldb, uint64_t dx_dev, int64_t lddx,
                                     uint64_t da_dev, uint64_t db_dev) {
@@ -423,7 +455,7 @@ extern "C" int32_t qm_lora_backward(qm_ctx *c, qm_lora *l, uint64_t x_bf16_dev, 
     if (tokens < 0 || ldx < l->cols || lddy < l->rows || ldx > (1 << 30) || lddy > (1 << 30)) return QM_ERR_SHAPE;
     if (tokens > l->max_tokens) return QM_ERR_LIMIT;
     if (tokens && (!x_bf16_dev || !dy_bf16_dev)) return QM_ERR_ARG;
-    if (((x_bf16_dev | dy_bf16_dev) & 15) || (ldx & 7) || (lddy & 7) || ((ids_dev | da_dev | db_dev) & 3)) return QM_ERR_ARG;
+    if ((x_bf16_dev & 15) || (ldx & 7) || (dy_bf16_dev & 1) || ((ids_dev | da_dev | db_dev) & 3)) return QM_ERR_ARG;
     const int64_t na = (int64_t)l->slots * l->max_rank * l->cols, nb = (int64_t)l->slots * l->max_rank * l->rows;
     if (dx_dev) {
         rc = batch_check(l, x_bf16_dev, ldx, tokens, ids_dev, base_dev, ldb, dx_dev, lddx, l->cols, l->cols);
@@ -441,13 +473,25 @@ extern "C" int32_t qm_lora_backward(qm_ctx *c, qm_lora *l, uint64_t x_bf16_dev, 
         rc = lists_launch(c, l, ids_dev, tokens);
         if (rc) return rc;
     }
+    rc = align_dy(c, l, &dy_bf16_dev, &lddy, tokens);
+    if (rc) return rc;
     QmLoraTcArgs ta;
     rc = batch_args(c, &ta, l, x_bf16_dev, ldx, dy_bf16_dev, lddy, ids_dev, tokens);
     if (!rc) rc = shrink_launch(c, l, &ta, 2);
     if (rc) return rc;
     QmLoraBatchArgs &a = ta.b;
+    const bool both = dx_dev && (da_dev || db_dev);
     if (dx_dev) {
+        // dx and the gradients of A and B need nothing of each other: dx goes beside them, on a stream of the handle
+        CUstream main = c->stream;
+        if (both) {
+            DRV(c->drv->cuEventRecord(l->fork, main));
+            DRV(c->drv->cuStreamWaitEvent(l->side, l->fork, 0));
+            c->stream = l->side;
+        }
         rc = expand_launch(c, l, &a, 0, base_dev, ldb, dx_dev, lddx);
+        c->stream = main;
+        if (both) DRV(c->drv->cuEventRecord(l->join, l->side));
         if (rc) return rc;
     }
     if (!da_dev && !db_dev) return QM_OK;
@@ -465,6 +509,8 @@ extern "C" int32_t qm_lora_backward(qm_ctx *c, qm_lora *l, uint64_t x_bf16_dev, 
     a.outer_units = (int32_t)(std::max(ba, bb) * l->slots);
     a.split = share(l, ((da_dev ? ba : 0) + (db_dev ? bb : 0)) * slots, (tokens / slots + 63) / 64, 1);
     if (2ll * a.outer_units * a.split > 0x7FFFFFFF) return QM_ERR_LIMIT;
-    return qm_launch_ex(c, QM_K_LORA_OUTER_R16 + rank_kernel(l), (unsigned)(2 * a.outer_units * a.split), (QM_LORA_OUTER_READERS(rp) + 2) * 32,
+    rc = qm_launch_ex(c, QM_K_LORA_OUTER_R16 + rank_kernel(l), (unsigned)(2 * a.outer_units * a.split), (QM_LORA_OUTER_READERS(rp) + 2) * 32,
                         (unsigned)outer_smem(l), &ta, true, false, a.split);
+    if (both) DRV(c->drv->cuStreamWaitEvent(c->stream, l->join, 0));
+    return rc;
 }

@@ -735,6 +735,24 @@ extern "C" __global__ void __launch_bounds__(1024) qm_lora_lists(const __grid_co
     }
 }
 
+// A copy of bf16 rows whose addresses or pitch no tensor map takes, 16-byte aligned: a thread writes eight columns at a time.
+extern "C" __global__ void __launch_bounds__(256) qm_lora_align(const __grid_constant__ QmLoraAlignArgs a) {
+    wait_for_inputs();
+    const int64_t pieces = a.pitch / 8, total = pieces * a.rows;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
+        const int64_t row = e / pieces;
+        const int c = (int)(e - row * pieces) * 8;
+        const uint16_t *p = a.src + row * a.ld + c;
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t lo = c + 2 * i < a.cols ? p[2 * i] : 0u, hi = c + 2 * i + 1 < a.cols ? p[2 * i + 1] : 0u;
+            w[i] = lo | hi << 16;
+        }
+        *reinterpret_cast<uint4 *>(a.dst + row * a.pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
 // ---- tcgen05 plumbing ----------------------------------------------------------------------------------------------------
 namespace {
 

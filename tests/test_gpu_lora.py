@@ -327,6 +327,33 @@ def test_backward_parts_and_repeats(ctx, adapters):
     assert (dx == 5.0).all() and (da == 0).all() and (db == 0).all()
 
 
+@pytest.mark.parametrize("shift,lddy", [(0, 129), (1, 136), (3, 131), (8, 133)])
+def test_backward_of_unaligned_gradients(ctx, adapters, shift, lddy):
+    """dy rows at any address and pitch give the bits of aligned ones; the first such call is refused under capture."""
+    rows, cols, tokens = 129, 96, 150
+    ad = adapters(rows, cols, 2, 16, tokens, {0: 16, 1: 3})
+    x, ids = torch.randn(tokens, cols, device="cuda").to(BF16), make_ids("mixed", tokens, {0: 16, 1: 3}, 2)
+    flat = torch.full((tokens * lddy + 16,), float("nan"), dtype=BF16, device="cuda")
+    dy = flat[shift:shift + tokens * lddy].view(tokens, lddy)[:, :rows]
+    dy.copy_(torch.randn(tokens, rows, device="cuda"))
+    even = torch.full((tokens, 136), float("nan"), dtype=BF16, device="cuda")
+    even[:, :rows].copy_(dy)
+
+    def call(dev, ld):
+        out = [torch.empty(tokens, cols, device="cuda"), torch.empty(2, 16, cols, device="cuda"), torch.empty(2, rows, 16, device="cuda")]
+        torch.cuda.synchronize()
+        ad.h.backward(x.data_ptr(), cols, dev, ld, tokens, ids.data_ptr(), 0, 0, out[0].data_ptr(), cols, out[1].data_ptr(), out[2].data_ptr())
+        ctx.sync()
+        return out
+
+    with pytest.raises(lib_b200.QmError) as e:
+        capture.launches(ctx, lambda: ad.h.backward(x.data_ptr(), cols, flat.data_ptr() + 2 * shift, lddy, tokens, ids.data_ptr(), 0, 0,
+                                                    even.data_ptr(), cols, 0, 0))
+    assert e.value.code == 900      # CUDA_ERROR_STREAM_CAPTURE_UNSUPPORTED
+    for a, b in zip(call(flat.data_ptr() + 2 * shift, lddy), call(even.data_ptr(), 136)):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("type,kept", [(_capi.TYPE_F32, torch.float32), (_capi.TYPE_F16, torch.float16), (_capi.TYPE_BF16, BF16)])
 def test_slots_are_replaced_and_emptied(ctx, adapters, type, kept):
     rows, cols = 130, 64
@@ -521,8 +548,8 @@ def test_refusals(ctx, adapters):
         assert code(lambda: h.matmul_bf16(**{**ok, **change})) == want, change
     h.matmul_bf16(X, 0, 64, I, 0, 0, Y, 64)      # no tokens: nothing to do
     ok = dict(x_dev=X, ldx=64, dy_dev=D, lddy=64, tokens=4, ids_dev=I, base_dev=B, ldb=64, dx_dev=Y, lddx=64, da_dev=B + 8192, db_dev=B + 16384)
-    for change, want in [(dict(dx_dev=0, da_dev=0, db_dev=0), ARG), (dict(tokens=17), LIMIT), (dict(tokens=-1), SHAPE), (dict(lddy=56), SHAPE), (dict(lddy=68), ARG),
-                         (dict(dy_dev=D + 2), ARG), (dict(dy_dev=0), ARG), (dict(x_dev=0), ARG), (dict(lddx=63), SHAPE), (dict(dx_dev=D), ARG), (dict(dx_dev=X), ARG),
+    for change, want in [(dict(dx_dev=0, da_dev=0, db_dev=0), ARG), (dict(tokens=17), LIMIT), (dict(tokens=-1), SHAPE), (dict(lddy=56), SHAPE),
+                         (dict(dy_dev=D + 1), ARG), (dict(dy_dev=0), ARG), (dict(x_dev=0), ARG), (dict(lddx=63), SHAPE), (dict(dx_dev=D), ARG), (dict(dx_dev=X), ARG),
                          (dict(da_dev=B + 2), ARG), (dict(base_dev=Y + 4), ARG)]:
         assert code(lambda: h.backward(**{**ok, **change})) == want, change
     w = ctx.store_create(_capi.Q8_0, 96, 64)
