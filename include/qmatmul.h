@@ -198,8 +198,9 @@ QM_API int32_t qm_matmul_bf16(qm_ctx *ctx, qm_weight w, uint64_t a_dev, int32_t 
  *   y[t] = base[t] + scale_a * B_a (A_a f(x[t])),   a = ids[t] (int32, on the device; ids_dev = 0: slot 0 for all).
  * A token whose id is outside [0, adapters) or names an empty slot keeps base[t]. base_dev = 0 stands for zeros; it may be
  * y_dev itself with ldb = ldy, any other overlap of y with an input is refused. All sums are float32; adapters are held in
- * bf16. max_tokens (<= 2^20) bounds the tokens of one bf16 call and sizes the handle's workspace: calls with bf16
- * activations and their graphs that share a handle must be ordered, on one stream or with events.
+ * bf16. max_tokens (<= 2^20) bounds the tokens of one bf16 call and sizes the handle's workspace: qm_lora_matmul_bf16 of
+ * more than 128 tokens and qm_lora_backward use it, and such calls (and graphs of them) that share a handle must be ordered,
+ * on one stream or with events; the calls without it may overlap one another.
  * Capture into a graph is allowed; everything is asynchronous on the context's stream. Device pointers.
  *
  * qm_lora_set: fills a slot from device memory, A [rank][cols] and B [rows][rank] row by row, `type` a GGUF tensor type
@@ -215,7 +216,7 @@ QM_API int32_t qm_matmul_bf16(qm_ctx *ctx, qm_weight w, uint64_t a_dev, int32_t 
  *   da[a] = scale_a sum_t (B_a^T dy[t]) x[t]^T      float32 [adapters][max_rank][cols]
  *   db[a] = scale_a sum_t dy[t] (A_a x[t])^T        float32 [adapters][rows][max_rank]
  *   over the tokens of each adapter, added in a fixed order (the same bits in every run); ranks past a slot's own and
- *   adapters without a token get zeros. dx_dev, da_dev or db_dev may be 0: not wanted.
+ *   adapters without a token get zeros. dx_dev, da_dev or db_dev may be 0: not wanted; da and db may overlap nothing.
  * qm_matvec_lora, qm_matmul_bf16_lora: qm_matvec / qm_matmul_bf16 with the stored matrix w, then the adapters onto its
  *   result; w must have the handle's rows and cols. */
 #define QM_TYPE_F32 0

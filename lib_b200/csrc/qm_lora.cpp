@@ -337,6 +337,25 @@ static int32_t expand_launch(qm_ctx *c, const qm_lora *l, QmLoraBatchArgs *a, in
                      (unsigned)((a->side[out_side].cols + 255) / 256), 256, (unsigned)(65536 + 64 * QM_LORA_EXPAND_ROW(l->rpad / 16)), a, true);
 }
 
+static int32_t outer_launch(qm_ctx *c, const qm_lora *l, QmLoraTcArgs *ta, bool listed, uint64_t da, uint64_t db) {
+    QmLoraBatchArgs *a = &ta->b;
+    a->side[0].grad = (float *)(uintptr_t)da;
+    a->side[0].grad_slot = (int64_t)l->max_rank * l->cols;
+    a->side[0].grad_rank = l->cols;
+    a->side[0].grad_col = 1;
+    a->side[1].grad = (float *)(uintptr_t)db;
+    a->side[1].grad_slot = (int64_t)l->max_rank * l->rows;
+    a->side[1].grad_rank = 1;
+    a->side[1].grad_col = l->max_rank;
+    const int rp = l->rpad / 16, bn = QM_LORA_OUTER_COLS(rp);
+    const int64_t ba = (l->cols + bn - 1) / bn, bb = (l->rows + bn - 1) / bn;
+    const int64_t slots = listed ? std::min(l->slots, a->tokens) : 1;
+    a->outer_units = (int32_t)(std::max(ba, bb) * l->slots);
+    a->split = share(l, ((da ? ba : 0) + (db ? bb : 0)) * slots, (a->tokens / slots + 63) / 64, 1);
+    return qm_launch_ex(c, QM_K_LORA_OUTER_R16 + rank_kernel(l), (unsigned)(2 * a->outer_units * a->split), (QM_LORA_OUTER_READERS(rp) + 2) * 32,
+                        (unsigned)outer_smem(l), ta, true, false, a->split);
+}
+
 static int32_t batch_check(const qm_lora *l, uint64_t x, int64_t ldx, int32_t tokens, uint64_t ids_dev, uint64_t base, int64_t ldb,
                            uint64_t y, int64_t ldy, int64_t in_cols, int64_t out_cols) {
     if (tokens < 0 || ldx < in_cols || ldy < out_cols || (base && ldb < out_cols)) return QM_ERR_SHAPE;
@@ -462,6 +481,15 @@ extern "C" int32_t qm_lora_backward(qm_ctx *c, qm_lora *l, uint64_t x_bf16_dev, 
         if (rc) return rc;
         if (tokens && rows_meet(dy_bf16_dev, lddy * 2, l->rows * 2, dx_dev, lddx * 4, l->cols * 4, tokens)) return QM_ERR_ARG;
     }
+    // a gradient of A or B on nothing else
+    const struct {
+        uint64_t p;
+        int64_t bytes;
+    } span[] = {{da_dev, na * 4}, {db_dev, nb * 4}, {dx_dev, ((tokens - 1) * lddx + l->cols) * 4}, {base_dev, ((tokens - 1) * ldb + l->cols) * 4},
+                {x_bf16_dev, ((tokens - 1) * ldx + l->cols) * 2}, {dy_bf16_dev, ((tokens - 1) * lddy + l->rows) * 2}, {ids_dev, tokens * 4ll}};
+    for (int i = 0; i < 2; i++)
+        for (int k = i + 1; k < 7 && tokens; k++)
+            if (span[i].p && span[k].p && span[i].p < span[k].p + (uint64_t)span[k].bytes && span[k].p < span[i].p + (uint64_t)span[i].bytes) return QM_ERR_ARG;
     CtxGuard g(c);
     DRV(g.rc);
     if (tokens == 0) {
@@ -480,37 +508,21 @@ extern "C" int32_t qm_lora_backward(qm_ctx *c, qm_lora *l, uint64_t x_bf16_dev, 
     if (!rc) rc = shrink_launch(c, l, &ta, 2);
     if (rc) return rc;
     QmLoraBatchArgs &a = ta.b;
-    const bool both = dx_dev && (da_dev || db_dev);
-    if (dx_dev) {
-        // dx and the gradients of A and B need nothing of each other: dx goes beside them, on a stream of the handle
-        CUstream main = c->stream;
-        if (both) {
-            DRV(c->drv->cuEventRecord(l->fork, main));
-            DRV(c->drv->cuStreamWaitEvent(l->side, l->fork, 0));
-            c->stream = l->side;
-        }
-        rc = expand_launch(c, l, &a, 0, base_dev, ldb, dx_dev, lddx);
-        c->stream = main;
-        if (both) DRV(c->drv->cuEventRecord(l->join, l->side));
-        if (rc) return rc;
+    // dx and the gradients of A and B need nothing of each other: with both wanted dx goes beside the others, on a stream of
+    // the handle (777 tokens, 6144 x 4096, rank 8: 53 -> 44 us)
+    const bool grads = da_dev || db_dev, both = dx_dev && grads;
+    CUstream main = c->stream;
+    if (both) {
+        DRV(c->drv->cuEventRecord(l->fork, main));
+        DRV(c->drv->cuStreamWaitEvent(l->side, l->fork, 0));
+        c->stream = l->side;
     }
-    if (!da_dev && !db_dev) return QM_OK;
-    a.side[0].grad = (float *)(uintptr_t)da_dev;
-    a.side[0].grad_slot = (int64_t)l->max_rank * l->cols;
-    a.side[0].grad_rank = l->cols;
-    a.side[0].grad_col = 1;
-    a.side[1].grad = (float *)(uintptr_t)db_dev;
-    a.side[1].grad_slot = (int64_t)l->max_rank * l->rows;
-    a.side[1].grad_rank = 1;
-    a.side[1].grad_col = l->max_rank;
-    const int rp = l->rpad / 16, bn = QM_LORA_OUTER_COLS(rp);
-    const int64_t ba = (l->cols + bn - 1) / bn, bb = (l->rows + bn - 1) / bn;
-    const int64_t slots = ids_dev ? std::min(l->slots, tokens) : 1;
-    a.outer_units = (int32_t)(std::max(ba, bb) * l->slots);
-    a.split = share(l, ((da_dev ? ba : 0) + (db_dev ? bb : 0)) * slots, (tokens / slots + 63) / 64, 1);
-    if (2ll * a.outer_units * a.split > 0x7FFFFFFF) return QM_ERR_LIMIT;
-    rc = qm_launch_ex(c, QM_K_LORA_OUTER_R16 + rank_kernel(l), (unsigned)(2 * a.outer_units * a.split), (QM_LORA_OUTER_READERS(rp) + 2) * 32,
-                        (unsigned)outer_smem(l), &ta, true, false, a.split);
-    if (both) DRV(c->drv->cuStreamWaitEvent(c->stream, l->join, 0));
+    if (dx_dev) rc = expand_launch(c, l, &a, 0, base_dev, ldb, dx_dev, lddx);
+    c->stream = main;
+    if (grads && !rc) rc = outer_launch(c, l, &ta, ids_dev != 0, da_dev, db_dev);
+    if (both) {   // whatever became of the launches
+        DRV(c->drv->cuEventRecord(l->join, l->side));
+        DRV(c->drv->cuStreamWaitEvent(main, l->join, 0));
+    }
     return rc;
 }

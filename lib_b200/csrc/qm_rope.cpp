@@ -86,6 +86,11 @@ static Span span_of(uint64_t base, int64_t rows, int64_t pitch, int64_t width) {
     return {base, base + (uint64_t)((rows - 1) * pitch + width)};
 }
 static bool overlap(const Span &a, const Span &b) { return a.lo < b.hi && b.lo < a.hi; }
+// A result on the positions or a gain.
+static bool on_small(const Span &out, uint64_t pos, int64_t tokens, uint64_t gq, uint64_t gk, int64_t dim) {
+    return (pos && overlap(out, span_of(pos, tokens, 4, 4))) || (gq && overlap(out, span_of(gq, 1, 0, dim * 4))) ||
+           (gk && overlap(out, span_of(gk, 1, 0, dim * 4)));
+}
 
 // What both directions ask of their arguments. `out`: dx of the backward pass (0 forward); q and k are results or their
 // gradients. Results may lie on the raw heads they come from, place for place; any other overlap of a result is refused.
@@ -165,6 +170,8 @@ extern "C" int32_t qm_qk_norm_rope(qm_ctx *c, qm_rope *r, uint64_t x_dev, int64_
     const Span k = k_heads ? span_of(k_out, tokens, ldk * size, k_heads * dim * size) : Span{0, 0};
     const bool q_on = !bf16 && q_out == x_dev && ldq == ldx;
     const bool k_on = !bf16 && k_out == x_dev + (uint64_t)q_heads * dim * 4 && ldk == ldx;
+    if ((q_heads && on_small(q, pos_dev, tokens, q_gain_dev, k_gain_dev, dim)) || (k_heads && on_small(k, pos_dev, tokens, q_gain_dev, k_gain_dev, dim)))
+        return QM_ERR_ARG;
     if (q_heads && overlap(q, x) && !q_on) return QM_ERR_ARG;
     if (k_heads && overlap(k, x) && !k_on) return QM_ERR_ARG;
     // side by side in one buffer of rows (q_on and k_on among them) the two do not meet
@@ -211,6 +218,8 @@ extern "C" int32_t qm_qk_norm_rope_backward(qm_ctx *c, qm_rope *r, uint64_t x_de
     if (k_heads && overlap(dx, span_of(dk_dev, tokens, lddk * size, k_heads * dim * size)) &&
         !(size == 4 && dk_dev == dx_dev + (uint64_t)q_heads * dim * 4 && lddk == lddx))
         return QM_ERR_ARG;
+    if (on_small(dx, pos_dev, tokens, q_gain_dev, k_gain_dev, dim) || on_small(dx, 0, 1, dq_gain_dev, dk_gain_dev, dim)) return QM_ERR_ARG;
+    if (dq_gain_dev && dk_gain_dev && overlap(span_of(dq_gain_dev, 1, 0, dim * 4), span_of(dk_gain_dev, 1, 0, dim * 4))) return QM_ERR_ARG;
     a.dx = (float *)(uintptr_t)dx_dev;
     a.lddx = lddx;
     a.partial = gains ? (float *)(uintptr_t)r->partial : nullptr;

@@ -146,6 +146,15 @@ BATCHES = [
     (770, 2080, 200, {0: 128, 3: 65}, "apart", "mixed"),
     (256, 1024, 4099, {0: 8, 1: 16}, "none", "runs"),
     (300, 128, 256, {i: 4 for i in range(256)}, "apart", "each"),
+    (130, 32, 129, {0: 2}, "apart", "all"),                     # fewer columns than a cluster has CTAs
+    (1, 64, 200, {1: 33, 0: 1}, "in place", "mixed"),
+    (64, 64, 200001, {0: 4, 3: 2}, "apart", "runs"),            # many tiles of one adapter
+    # up to 128 tokens: one launch
+    (4096, 4096, 100, {0: 128, 1: 65, 2: 33}, "apart", "mixed"),
+    (1031, 2080, 128, {0: 64, 1: 40, 7: 9}, "in place", "runs"),
+    (6144, 14336, 100, {0: 32}, "none", "all"),
+    (28672, 96, 17, {0: 16, 1: 3}, "apart", "mixed"),
+    (512, 1024, 128, {i: 1 + i % 16 for i in range(128)}, "apart", "each"),
 ]
 
 
@@ -223,6 +232,7 @@ GRADS = [
     (4096, 2048, 1025, {0: 16}, "all"),
     (520, 1024, 515, {0: 128, 1: 90, 2: 3}, "runs"),
     (264, 64, 64, {i: 4 for i in range(64)}, "each"),
+    (72, 96, 70001, {0: 9, 1: 16}, "runs"),
 ]
 
 
@@ -550,7 +560,7 @@ def test_refusals(ctx, adapters):
     ok = dict(x_dev=X, ldx=64, dy_dev=D, lddy=64, tokens=4, ids_dev=I, base_dev=B, ldb=64, dx_dev=Y, lddx=64, da_dev=B + 8192, db_dev=B + 16384)
     for change, want in [(dict(dx_dev=0, da_dev=0, db_dev=0), ARG), (dict(tokens=17), LIMIT), (dict(tokens=-1), SHAPE), (dict(lddy=56), SHAPE),
                          (dict(dy_dev=D + 1), ARG), (dict(dy_dev=0), ARG), (dict(x_dev=0), ARG), (dict(lddx=63), SHAPE), (dict(dx_dev=D), ARG), (dict(dx_dev=X), ARG),
-                         (dict(da_dev=B + 2), ARG), (dict(base_dev=Y + 4), ARG)]:
+                         (dict(da_dev=B + 2), ARG), (dict(base_dev=Y + 4), ARG), (dict(da_dev=X), ARG), (dict(db_dev=B + 8192), ARG), (dict(db_dev=Y + 8), ARG)]:
         assert code(lambda: h.backward(**{**ok, **change})) == want, change
     w = ctx.store_create(_capi.Q8_0, 96, 64)
     assert code(ctx.matvec_lora, w, h, X, 1, 64, 0, Y, 96) == SHAPE     # a matrix of another shape

@@ -50,6 +50,8 @@ CASES = [
     (65, 4, 4, 128, 0, False, True, True, True, 1, 0),        # norm alone
     (2500, 9, 2, 128, 128, False, True, True, True, 0, 0),    # several heads per warp, an odd number of them
     (300, 3, 1, 510, 254, True, False, True, True, 0, 0),
+    (3, 1500, 2, 64, 64, False, False, True, True, 0, 0),     # more heads than CTAs
+    (5000, 2, 1, 192, 96, True, True, True, True, 0, 4),
 ]
 
 
@@ -289,14 +291,15 @@ def test_refusals(ctx):
     bad = [(dict(tokens=-1), SHAPE), (dict(q_heads=-1), SHAPE), (dict(q_heads=0, k_heads=0), SHAPE), (dict(ldx=23), SHAPE), (dict(ldq=15), SHAPE), (dict(ldk=7), SHAPE),
            (dict(ldx=1 << 40), SHAPE), (dict(eps=-1.0), SHAPE), (dict(eps=float("nan")), SHAPE), (dict(x_dev=0), ARG), (dict(pos_dev=0), ARG), (dict(q_dev=0), ARG),
            (dict(k_dev=0), ARG), (dict(x_dev=X + 2), ARG), (dict(q_dev=Q + 2), ARG), (dict(flags=4), ARG), (dict(q_gain_dev=P + 1), ARG), (dict(pos_dev=P + 2), ARG)]
-    for change, want in bad + [(dict(q_dev=X + 4), ARG), (dict(q_dev=X, ldq=36), ARG), (dict(k_dev=Q), ARG), (dict(k_dev=Q + 32), ARG), (dict(q_dev=X, ldq=32, flags=2), ARG)]:
+    for change, want in bad + [(dict(q_dev=X + 4), ARG), (dict(q_dev=X, ldq=36), ARG), (dict(k_dev=Q), ARG), (dict(k_dev=Q + 32), ARG), (dict(q_dev=P), ARG), (dict(k_gain_dev=K), ARG), (dict(q_dev=X, ldq=32, flags=2), ARG)]:
         assert code(rope.qk_norm, **{**ok, **change}) == want, change
     both = {**ok, "ldq": 24, "ldk": 24, "k_dev": Q + 64}
     rope.qk_norm(**both)          # q and k side by side in rows of their own
     ok = {**{k: v for k, v in ok.items() if k[:2] not in ("q_", "k_", "ld")}, "ldx": 32, "q_heads": 2, "k_heads": 1, "q_gain_dev": 0, "k_gain_dev": 0, "dq_dev": Q, "lddq": 16,
           "dk_dev": K, "lddk": 8, "dx_dev": D, "lddx": 24}
     for change, want in [(dict(dx_dev=0), ARG), (dict(lddx=23), SHAPE), (dict(dx_dev=D + 1), ARG), (dict(dq_dev=0), ARG), (dict(lddq=15), SHAPE), (dict(dx_dev=X + 32), ARG),
-                         (dict(dx_dev=Q), ARG), (dict(dx_dev=K), ARG), (dict(flags=1, dq_gain_dev=D), ARG), (dict(dk_gain_dev=D + 2), ARG), (dict(tokens=-1), SHAPE)]:
+                         (dict(dx_dev=Q), ARG), (dict(dx_dev=K), ARG), (dict(flags=1, dq_gain_dev=D), ARG), (dict(dk_gain_dev=D + 2), ARG), (dict(tokens=-1), SHAPE), (dict(dk_gain_dev=D), ARG),
+                         (dict(dq_gain_dev=P + 64, dk_gain_dev=P + 68), ARG)]:
         assert code(rope.qk_norm_backward, **{**ok, **change}) == want, change
     assert lib_b200.lib.qm_rope_destroy(ctx._h, None) == ARG
     ctx.sync()
