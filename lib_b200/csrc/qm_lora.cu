@@ -1049,6 +1049,25 @@ __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
         }
     }
     copy_commit();
+    constexpr int KB = RP == 1 ? 1 : RP / 2;      // groups of 32 ranks (one of 16)
+    constexpr int W = RP == 1 ? 4 : 8;            // ranks of a lane
+    const int kb = RP == 1 ? (rank > 0) : (rank + 31) / 32;
+    // (asked for before base, behind which they would come last)
+    uint32_t fb[KB][4][W / 2];
+#pragma unroll
+    for (int k = 0; k < KB; k++)
+#pragma unroll
+        for (int n = 0; n < 4; n++)   // (a column behind the last one: any other, the result is not stored)
+            if (k < kb) {
+                const uint16_t *p = s.wt + ((int64_t)t.slot * s.cols + min(c0 + n * 8 + g, s.cols - 1)) * R + k * 32 + W * q;
+                if constexpr (W == 8) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+                    fb[k][n][0] = v.x; fb[k][n][1] = v.y; fb[k][n][2] = v.z; fb[k][n][3] = v.w;
+                } else {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+                    fb[k][n][0] = v.x; fb[k][n][1] = v.y;
+                }
+            }
     const bool mine = c0 < s.cols;
 #pragma unroll
     for (int m = 0; m < 4; m++) {
@@ -1072,24 +1091,6 @@ __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
         }
         copy_commit();
     }
-    constexpr int KB = RP == 1 ? 1 : RP / 2;      // groups of 32 ranks (one of 16)
-    constexpr int W = RP == 1 ? 4 : 8;            // ranks of a lane
-    const int kb = RP == 1 ? (rank > 0) : (rank + 31) / 32;
-    uint32_t fb[KB][4][W / 2];
-#pragma unroll
-    for (int k = 0; k < KB; k++)
-#pragma unroll
-        for (int n = 0; n < 4; n++)   // (a column behind the last one: any other, the result is not stored)
-            if (k < kb) {
-                const uint16_t *p = s.wt + ((int64_t)t.slot * s.cols + min(c0 + n * 8 + g, s.cols - 1)) * R + k * 32 + W * q;
-                if constexpr (W == 8) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(p);
-                    fb[k][n][0] = v.x; fb[k][n][1] = v.y; fb[k][n][2] = v.z; fb[k][n][3] = v.w;
-                } else {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-                    fb[k][n][0] = v.x; fb[k][n][1] = v.y;
-                }
-            }
     copy_wait<4>();
     __syncthreads();
     if (!mine) return;
