@@ -16,7 +16,13 @@
 //
 // The angle of a far position has lost its fraction in 32 bits (position 10^6 is 0.06 off), so the turns (angle / 2 pi) are
 // a product in 64-bit fixed point, position times the fraction of a turn in units of 2^-64, whose overflow is the whole turns:
-// what is left is exact to 2^-33 of a turn for every position, and three integer instructions.
+// what is left, in a few integer instructions, is off by at most 2^-31 of a turn at every position, before it is rounded to
+// float32 as any fraction would be. (The same in float64 kept the FP64 pipe busy: 52 -> 45 us at the size below, with a grid
+// that needs no division to find its heads.)
+//
+// One B200, 40 heads of 128, half-split: 8192 tokens to bf16 44.7 us (5.6 TB/s, 0.86 of the measured copy rate; the first form
+// with one reduction per head and gains read for every head 64 us, bound by instruction issue); 4096 tokens backward 49.6 us
+// (4.2 TB/s, 0.65; 47 us of it the pass itself, the rest qm_qk_gain_sum); one token 4.4 us, the cost of a launch.
 #include <cuda_bf16.h>
 #include <stdint.h>
 
