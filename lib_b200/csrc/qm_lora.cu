@@ -3,13 +3,24 @@
 //   y[t] = base[t] + s B (A f(x[t])) with the A, B and s of token t's adapter; tokens without one keep their base row.
 //   Backward: u = s A x, v = s B^T dy, dx = base + A^T v, dA = sum_t v x^T, dB = sum_t dy u^T over an adapter's tokens.
 //
-// Everything is a product with a matrix of at most 128 rows, so what bounds it is the wide side: x, base and y, dy, dx.
-// Three kinds of products cover both directions, each over tiles of 64 tokens of one adapter:
+// Everything is a product with a matrix of at most 128 rows, so what bounds it is the wide side: x, base and y, dy, dx. Three
+// kinds of products cover both directions:
 //   shrink  low[t][r]  = sum_c x[t][c] w[r][c]   (x with A; dy with the transposed B)
 //   expand  y[t][c]    = base[t][c] + sum_r low[t][r] w[r][c]
 //   outer   grad[r][c] = sum_t low[t][r] x[t][c]
 // The 16-bit operands are multiplied as they are. low is a float32 sum; where it is an operand it is taken as the sum of
-// three bf16 (8 bits each: all 24 bits of the value), one mma for each, so no rounding to 16 bits enters a result.
+// three bf16 (8 bits each: all 24 bits of the value), one product for each, so no rounding to 16 bits enters a result.
+//
+// Forms: qm_lora_rows for 1..8 float32 rows and qm_lora_few_* for up to 128 bf16 tokens do shrink and expand in one launch;
+// beyond, and in the backward pass, qm_lora_lists orders the tokens by adapter and shrink, expand and outer are launches of
+// their own. Measured on one B200, calls back to back, floor = what has to move at the measured copy rate of 6.54 TB/s:
+//   1 row, 4096 x 4096, rank 16                       5.3 us   floor 0.05 (launch, five dependent trips to memory)
+//   8 rows, 8 adapters, 6144 x 4096, rank 64          9.2 us   floor 1.4  (the same, 112 KB of A and B per CTA)
+//   64 tokens, 32 adapters, 6144 x 4096, rank 16      9.3 us   floor 1.9
+//   391 tokens, 28672 x 4096, rank 32                  36 us   floor 15   (expand: base in, y out)
+//   2048 tokens, 4096 x 14336, rank 64                 48 us   floor 22
+//   backward, 777 tokens, 6144 x 4096, rank 8          44 us   floor 6.5  (seven short launches)
+//   backward, 4096 tokens, 28672 x 4096, rank 32      155 us   floor 63   (dy is read twice: 235 MB more)
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -905,7 +916,9 @@ __device__ __forceinline__ bool neighbours(const int (&rows)[4], int there) {
 // A cluster of `split` CTAs takes one tile of 128 tokens of one adapter, the CTAs taking turns over its columns, 64 per
 // stage: the adapter's ranks and the tokens by TMA, 32 tokens that are neighbours as one box, others by their numbers. One
 // thread issues the products (M = the tokens, N = the ranks) into tensor memory. What a CTA reads from memory is all that
-// bounds it. The CTAs' sums meet in distributed shared memory and are added in a fixed order.
+// bounds it. The CTAs' sums meet in distributed shared memory and are added in a fixed order. 4096 tokens, x of 4096 and dy of
+// 28672 columns, rank 32: 52 us, 5.2 TB/s (legacy mma with cp.async: 67 us, and 71 instead of 22 at 2048 tokens x 14336, rank
+// 64, where its fragments kept the issue slots and the shared memory busy).
 constexpr int SHRINK_THREADS = 192;   // four warps that read the accumulators, one that loads, one that multiplies
 
 template <int RP>
@@ -1008,8 +1021,10 @@ __device__ __forceinline__ void shrink(const QmLoraTcArgs &ta) {
 // A CTA takes half a tile's tokens x 256 columns, each of its eight warps 32 columns. All of base is asked for at the start
 // (cp.async into the warp's own shared memory, no registers held), the tokens' narrow products once for the CTA; the
 // adapter's fragments of the columns stay in registers while the warp goes through the tokens, 16 at a time. The products
-// are added to base in shared memory and leave in rows of 128 bytes. Legacy mma on purpose: 16 to 128 ranks x 3 parts are too
-// little work to bound anything, and its fragments need neither tensor memory nor a second pass over the results.
+// are added to base in shared memory and leave in rows of 128 bytes. Legacy mma on purpose: the same step by tcgen05 (operands
+// by TMA, results through tensor memory and shared memory, 128 columns per CTA) took 22.5 us instead of 20.5 at 2048 tokens x
+// 4096, rank 64, and 34 instead of 22 at 391 x 28672, rank 32, because every CTA then waits for tensor memory and two barriers
+// more; leaving the products out altogether saves 1 us. Copying base to y by the same steps takes 13.6 and 18 us.
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -1157,7 +1172,8 @@ __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
 // tokens, 64 per stage. Both operands lie token by token, which is along M and N: M = the three parts of the ranks side by
 // side, as they lie in the workspace, so one product takes all of them, N = the columns. 32 tokens that are neighbours come
 // as boxes, others by their numbers; behind the slot's last token come zeros. The parts, and the CTAs' sums, are added in a
-// fixed order.
+// fixed order. 4096 tokens of 4096 and 28672 columns, rank 32: 61 us (legacy mma 129), about 10 of them start and end of a CTA;
+// 128 column blocks leave 20 SMs to dx, which runs beside it.
 template <int RP>
 __device__ __forceinline__ void outer(const QmLoraTcArgs &ta) {
     const QmLoraBatchArgs &a = ta.b;
