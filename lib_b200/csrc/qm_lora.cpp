@@ -515,11 +515,12 @@ extern "C" int32_t qm_lora_backward(qm_ctx *c, qm_lora *l, uint64_t x_bf16_dev, 
     if (both) {
         DRV(c->drv->cuEventRecord(l->fork, main));
         DRV(c->drv->cuStreamWaitEvent(l->side, l->fork, 0));
-        c->stream = l->side;
     }
-    if (dx_dev) rc = expand_launch(c, l, &a, 0, base_dev, ldb, dx_dev, lddx);
+    // (first, so that its CTAs, one to an SM, find their place)
+    if (grads) rc = outer_launch(c, l, &ta, ids_dev != 0, da_dev, db_dev);
+    if (both) c->stream = l->side;
+    if (dx_dev && !rc) rc = expand_launch(c, l, &ta.b, 0, base_dev, ldb, dx_dev, lddx);
     c->stream = main;
-    if (grads && !rc) rc = outer_launch(c, l, &ta, ids_dev != 0, da_dev, db_dev);
     if (both) {   // whatever became of the launches
         DRV(c->drv->cuEventRecord(l->join, l->side));
         DRV(c->drv->cuStreamWaitEvent(main, l->join, 0));
