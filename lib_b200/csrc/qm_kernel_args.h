@@ -449,8 +449,8 @@ struct QmLoraRowsArgs {
     int32_t rows, cols, np, rpad, slots, m;
     int32_t xop;
     float eps;
-    int32_t nsplit;          // clusters that share the columns of one group of rows
-    int32_t pad_;
+    int32_t parts[8];        // by items - 1: clusters that share an item's columns
+    int32_t width[8];        // and the columns of one of their CTAs
 };
 
 // Few bf16 tokens (qm_lora_few_*).
@@ -466,7 +466,8 @@ struct QmLoraFewArgs {
     const int32_t *rank;
     int64_t ldx, ldb, ldy;
     int32_t rows, cols, np, slots, tokens;
-    int32_t nsplit;          // clusters that share the columns of one item
+    int32_t pieces;          // the most clusters that share an item's columns
+    int32_t at_once, pad_;   // clusters that run at once
 };
 
 // Tokens in the order of their adapters (qm_lora_lists): group g < slots are the tokens of slot g, group `slots` those

@@ -64,7 +64,7 @@ static int64_t rows_smem(const qm_lora *l) {
     return 16ll * l->rpad * 4 + 8 * 4 + chunk + std::max<int64_t>(8 * ks * 4, 32 * QM_LORA_CHUNK * 4 + chunk);
 }
 static int64_t few_smem(const qm_lora *l) {
-    return 8 * 16 * (l->rpad + 4) * 4 + 16 * QM_LORA_EXPAND_ROW(l->rpad / 16) + (QM_LORA_FEW + 24) * 4;
+    return 8 * 16 * (l->rpad + 4) * 4 + 16 * QM_LORA_EXPAND_ROW(l->rpad / 16) + (3 * QM_LORA_FEW + 24) * 4;
 }
 static int64_t shrink_smem(const qm_lora *l) { return 1024 + QM_LORA_SHRINK_STAGES(l->rpad / 16) * (16384 + l->rpad * 128ll) + 128; }
 static int64_t outer_smem(const qm_lora *l) {
@@ -217,12 +217,17 @@ static int32_t rows_launch(qm_ctx *c, const qm_lora *l, uint64_t x_dev, uint64_t
     a.m = m;
     a.xop = (int32_t)(flags & 0xFu);
     a.eps = 1e-6f;
-    // clusters per row: no more than run at once (one CTA per SM), and none with less than a chunk of columns per CTA. (Eight
-    // rows of 6144 columns: 9.2 us with one, 13.6 with two, of which one has to wait; five of 10007: 9.8, 8.3 and with three 7.3.)
-    const int64_t most = (l->np + QM_LORA_CLUSTER * QM_LORA_CHUNK - 1) / (QM_LORA_CLUSTER * QM_LORA_CHUNK);
-    a.nsplit = (int32_t)std::max<int64_t>(1, std::min<int64_t>(most, l->at_once[3] / m));
-    const int64_t smem = rows_smem(l);
-    return qm_launch_ex(c, QM_K_LORA_ROWS, (unsigned)(m * a.nsplit * QM_LORA_CLUSTER), 512, (unsigned)smem, &a, true, false, QM_LORA_CLUSTER);
+    // As many clusters as run at once (one CTA per SM), and none with less than a chunk of columns per CTA. (Eight rows on
+    // eight adapters, 6144 columns: 9.2 us; with sixteen clusters, of which one has to wait, 13.6.)
+    const int64_t pieces = (l->np + QM_LORA_CLUSTER * QM_LORA_CHUNK - 1) / (QM_LORA_CLUSTER * QM_LORA_CHUNK);
+    int64_t clusters = m;
+    for (int i = 1; i <= 8; i++) {
+        const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(pieces, l->at_once[3] / i));
+        a.parts[i - 1] = (int32_t)parts;
+        a.width[i - 1] = (int32_t)(((l->np + parts * QM_LORA_CLUSTER - 1) / (parts * QM_LORA_CLUSTER) + 7) & ~(int64_t)7);
+        if (i <= m) clusters = std::max(clusters, i * parts);
+    }
+    return qm_launch_ex(c, QM_K_LORA_ROWS, (unsigned)(clusters * QM_LORA_CLUSTER), 512, (unsigned)rows_smem(l), &a, true, false, QM_LORA_CLUSTER);
 }
 
 extern "C" int32_t qm_lora_matvec(qm_ctx *c, qm_lora *l, uint64_t x_dev, uint64_t x2_dev, int32_t m, int64_t ldx, uint64_t ids_dev,
@@ -390,16 +395,13 @@ static int32_t few_launch(qm_ctx *c, const qm_lora *l, uint64_t x, int32_t token
     a.np = (int32_t)l->np;
     a.slots = l->slots;
     a.tokens = tokens;
-    // There may be as many items as tokens, and clusters that find none cost as much to launch: the columns of an item are
-    // shared by more clusters only while all of them run at once, with 256 columns per CTA at least. (64 tokens on 32 adapters,
-    // 6144 columns: one cluster per item 9.3 us, two 14.1, three 15.8.)
-    const int64_t most = ids_dev ? tokens : (tokens + 15) / 16;
-    const int64_t pieces = (l->np + QM_LORA_CLUSTER * 256 - 1) / (QM_LORA_CLUSTER * 256);
-    a.nsplit = (int32_t)std::max<int64_t>(1, std::min<int64_t>(pieces, l->few_at_once / most));
-    const int64_t smem = few_smem(l);
+    a.pieces = (int32_t)((l->np + QM_LORA_CLUSTER * 256 - 1) / (QM_LORA_CLUSTER * 256));
+    const int64_t most = ids_dev ? tokens : (tokens + 15) / 16;   // items
+    a.at_once = l->few_at_once;
+    const int64_t clusters = std::max(most, std::min<int64_t>(l->few_at_once, most * a.pieces));
     const bool vec = !((base | y) & 7) && !((ldb | ldy) & 1);
-    return qm_launch_ex(c, (vec ? QM_K_LORA_FEW_R16 : QM_K_LORA_FEW_R16_S) + rank_kernel(l), (unsigned)(most * a.nsplit * QM_LORA_CLUSTER), 256,
-                        (unsigned)smem, &a, true, false, QM_LORA_CLUSTER);
+    return qm_launch_ex(c, (vec ? QM_K_LORA_FEW_R16 : QM_K_LORA_FEW_R16_S) + rank_kernel(l), (unsigned)(clusters * QM_LORA_CLUSTER), 256,
+                        (unsigned)few_smem(l), &a, true, false, QM_LORA_CLUSTER);
 }
 
 static int32_t batch_launch(qm_ctx *c, const qm_lora *l, uint64_t x, int32_t tokens, int64_t ldx, uint64_t ids_dev, uint64_t base,

@@ -183,11 +183,11 @@ extern "C" __global__ void __launch_bounds__(256) qm_lora_set(const __grid_const
 }
 
 // ---- 1..8 float32 rows ---------------------------------------------------------------------------------------------------
-// One launch: a cluster of eight CTAs takes the rows of one adapter (the cluster of the first such row; the others leave at
-// once). Each CTA multiplies an eighth of x with its columns of A, the partial sums meet in distributed shared memory, and
-// each CTA then adds its own columns of B. `nsplit` clusters share the columns and repeat the first half. At these sizes only
-// trips to memory count: the first columns of B and of base are on their way before A is read, and a warp asks for up to four
-// ranks of A at a time.
+// One launch: the rows with one id are an item, and as many clusters of eight
+// CTAs as run at once are dealt to the items, which every CTA finds from the ids; the clusters of an item share its columns.
+// Each CTA multiplies an eighth of x with its columns of A, the partial sums meet in distributed shared memory, and each CTA
+// then adds its own columns of B. At these sizes only trips to memory count: the first columns of B and of base are on their
+// way before A is read, and a warp asks for up to four ranks of A at a time.
 namespace {
 
 struct RowsShared {
@@ -280,21 +280,39 @@ extern "C" __global__ void __launch_bounds__(512) qm_lora_rows(const __grid_cons
     wait_for_inputs();
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int cluster = blockIdx.x / QM_LORA_CLUSTER, me = (int)cluster_rank();
-    const int row = cluster / a.nsplit, part = cluster % a.nsplit;
-    const int np_cta = (((a.np + a.nsplit * QM_LORA_CLUSTER - 1) / (a.nsplit * QM_LORA_CLUSTER)) + 7) & ~7;
+    const int me = (int)cluster_rank();
+    // every lane of every warp: its row's adapter, the rows that share it, and whether the row is the first of them (worked
+    // out while the adapter's rank is on its way)
+    const int id = lane < a.m ? (a.ids ? a.ids[lane] : 0) : -1;
+    const int lane_rank = id >= 0 && id < a.slots ? a.rank[id] : 0;
+    uint32_t equal = 0;
+    if (lane < a.m) equal = __match_any_sync((1u << a.m) - 1, id);
+    const uint32_t first = __ballot_sync(0xffffffffu, lane < a.m && __ffs(equal) - 1 == lane);
+    const int items = __popc(first), parts = a.parts[items - 1];
+    int item = 0, part = blockIdx.x / QM_LORA_CLUSTER;
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+        if (part >= parts) {
+            part -= parts;
+            item++;
+        }
+    if (item >= items) return;   // the whole cluster
+    uint32_t behind = first;
+#pragma unroll
+    for (int k = 0; k < 7; k++)
+        if (k < item) behind &= behind - 1;
+    const int row = __ffs(behind) - 1;
+    const int slot = __shfl_sync(0xffffffffu, id, row), r = __shfl_sync(0xffffffffu, lane_rank, row);
+    const uint32_t same = __shfl_sync(0xffffffffu, equal, row);   // the rows of this adapter
+    const int np_cta = a.width[items - 1];
     const int n0 = min((part * QM_LORA_CLUSTER + me) * np_cta, a.rows), nn = min(np_cta, a.rows - n0);
-    const int id = a.ids && lane < a.m ? a.ids[lane] : 0;
-    const int slot = __shfl_sync(0xffffffffu, id, row);
-    const uint32_t same = __ballot_sync(0xffffffffu, lane < a.m && id == slot);   // the rows of this adapter
-    const bool named = slot >= 0 && slot < a.slots;
-    const int r = named ? a.rank[slot] : 0;
     if (r == 0) {   // no adapter
         if (a.base != a.y)
-            for (int c = tid; c < nn; c += 512) a.y[row * a.ldy + n0 + c] = a.base ? a.base[row * a.ldb + n0 + c] : 0.f;
+            for (int i = 0; i < a.m; i++)
+                if (same >> i & 1)
+                    for (int c = tid; c < nn; c += 512) a.y[i * a.ldy + n0 + c] = a.base ? a.base[i * a.ldb + n0 + c] : 0.f;
         return;
     }
-    if (__ffs(same) - 1 < row) return;   // an earlier row's cluster has this one
     const int nr = __popc(same);
     auto row_of = [&](int i) {   // the i-th row of this adapter
         uint32_t left = same;
@@ -424,11 +442,14 @@ extern "C" __global__ void __launch_bounds__(512) qm_lora_rows(const __grid_cons
 
 // ---- few bf16 tokens -----------------------------------------------------------------------------------------------------
 // Decode batches of up to QM_LORA_FEW tokens in one launch, without lists or a workspace. Up to 16 tokens of one adapter are
-// an item (a token without an adapter is one of its own); every CTA finds the items from the ids, cluster c of eight CTAs
-// takes item c / nsplit, and the clusters behind the last item leave. As in qm_lora_rows a CTA multiplies an eighth of the
+// an item (a token without an adapter is one of its own). Every CTA finds the items from the ids; each gets a cluster of eight
+// CTAs, or as many as share the ones that run at once evenly, and the clusters behind the last item leave (which is not free:
+// 64 tokens on 32 adapters take 9 us with 64 clusters and 14 with 128). As in qm_lora_rows a CTA multiplies an eighth of the
 // columns of x with A, the sums meet in distributed shared memory and the CTA goes on with its own columns of B; the products
 // are mma with fragments straight from memory (see expand), the columns of a warp's first piece of B and of base on their way
-// before the sums meet. All that counts is the number of dependent trips to memory.
+// before the sums meet. All that counts is the number of dependent trips to memory. Against the three launches of larger
+// batches: 32 tokens of one adapter of rank 16, 6144 x 4096, 6.8 us instead of 14.3; 128 on 32, 9.6 instead of 18.2; 128 on
+// one, 28672 x 4096, 16.3 instead of 20.8; 128 on two of rank 128 there, the one place where the order turns, 43 instead of 35.
 namespace {
 
 template <int RP, bool VEC>
@@ -440,17 +461,17 @@ __device__ __forceinline__ void few(const QmLoraFewArgs &a) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
     float *part = reinterpret_cast<float *>(smem);                    // [8 warps][16][LD]; the first one the CTA's sum
     const uint32_t low = smem_u32(smem) + 8 * 16 * LD * 4;            // [16] rows of three parts
-    // behind them: [FEW] adapters, [16] the item's tokens, [8] scratch; over the sums, which come later: [4][256] tokens of a
-    // slot in a warp, [256] which slots hold an adapter
-    int32_t *ids = reinterpret_cast<int32_t *>(smem + 8 * 16 * LD * 4 + 16 * UB), *rows = ids + QM_LORA_FEW, *found = rows + 16;
+    // behind them: [FEW] adapters, [FEW] tokens of the same adapter before, [FEW] the items' first tokens, [16] the item's
+    // tokens, [8] scratch; over the sums, which come later: [4][256] tokens of a slot in a warp, [256] which slots hold an
+    // adapter
+    int32_t *ids = reinterpret_cast<int32_t *>(smem + 8 * 16 * LD * 4 + 16 * UB), *earlier = ids + QM_LORA_FEW, *leaders = earlier + QM_LORA_FEW;
+    int32_t *rows = leaders + QM_LORA_FEW, *found = rows + 16;
     uint8_t *count = smem, *known = smem + 1024;
-    // the item of this cluster
-    const int item = blockIdx.x / (QM_LORA_CLUSTER * a.nsplit), part_of = blockIdx.x / QM_LORA_CLUSTER % a.nsplit, me = (int)cluster_rank();
+    const int me = (int)cluster_rank();
     int mine = tid < a.tokens ? (a.ids ? a.ids[tid] : 0) : -1;
     known[tid] = tid < a.slots && a.rank[tid] > 0;
     reinterpret_cast<uint32_t *>(count)[tid] = 0;
     if (tid < 16) rows[tid] = -1;
-    if (tid == 0) found[4] = -1;
     __syncthreads();
     if (mine < 0 || mine >= a.slots || !known[mine]) mine = -1;
     if (tid < QM_LORA_FEW) ids[tid] = mine;
@@ -463,27 +484,27 @@ __device__ __forceinline__ void few(const QmLoraFewArgs &a) {
     const bool leads = tid < a.tokens && (mine < 0 || before % 16 == 0);
     const uint32_t vote = __ballot_sync(0xffffffffu, leads);
     if (lane == 0 && warp < 4) found[warp] = __popc(vote);
+    if (tid < QM_LORA_FEW) earlier[tid] = before;
     __syncthreads();
     if (leads) {
         int number = __popc(vote & ((1u << lane) - 1));
         for (int w = 0; w < warp; w++) number += found[w];
-        if (number == item) {
-            found[4] = tid;
-            found[5] = before;
-        }
+        leaders[number] = tid;
     }
     __syncthreads();
-    const int leader = found[4];
-    if (leader < 0) return;   // the whole cluster
+    const int items = found[0] + found[1] + found[2] + found[3], parts = max(1, min(a.pieces, a.at_once / items));
+    const int np_cta = (((a.np + parts * QM_LORA_CLUSTER - 1) / (parts * QM_LORA_CLUSTER)) + 7) & ~7;
+    const int unit = blockIdx.x / QM_LORA_CLUSTER;
+    if (unit >= items * parts) return;   // the whole cluster
+    const int leader = leaders[unit / parts];
     const int slot = ids[leader];
-    const int np_cta = (((a.np + a.nsplit * QM_LORA_CLUSTER - 1) / (a.nsplit * QM_LORA_CLUSTER)) + 7) & ~7;
-    const int n0 = min((part_of * QM_LORA_CLUSTER + me) * np_cta, a.rows), nn = min(np_cta, a.rows - n0);
+    const int n0 = min((unit % parts * QM_LORA_CLUSTER + me) * np_cta, a.rows), nn = min(np_cta, a.rows - n0);
     if (slot < 0) {
         if (a.base != a.y)
             for (int c = tid; c < nn; c += 256) a.y[leader * a.ldy + n0 + c] = a.base ? a.base[leader * a.ldb + n0 + c] : 0.f;
         return;
     }
-    if (tid < a.tokens && mine == slot && before >= found[5] && before < found[5] + 16) rows[before - found[5]] = tid;
+    if (tid < a.tokens && mine == slot && before >= earlier[leader] && before < earlier[leader] + 16) rows[before - earlier[leader]] = tid;
     __syncthreads();
     const int tok[2] = {rows[g], rows[g + 8]};   // the tokens of this lane's fragment rows, -1: none
     const int rank = a.rank[slot];
@@ -599,7 +620,6 @@ __device__ __forceinline__ void few(const QmLoraFewArgs &a) {
     cluster_arrive();   // done with the others' memory; waited for before leaving
     const uint32_t lm = low + (lane & 15) * UB + (lane >> 4) * 16;
     for (int c0 = warp * 32; c0 < nn; c0 += 256) {
-        if (c0 != warp * 32) fetch(c0);
         float d[4][4];
 #pragma unroll
         for (int n = 0; n < 4; n++)
@@ -622,14 +642,21 @@ __device__ __forceinline__ void few(const QmLoraFewArgs &a) {
         for (int n = 0; n < 4; n++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
+                d[n][2 * h] += base[n][h].x;
+                d[n][2 * h + 1] += base[n][h].y;
+            }
+        if (c0 + 256 < nn) fetch(c0 + 256);
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
                 const int c = c0 + n * 8 + 2 * q;
                 if (tok[h] < 0) continue;
                 float *p = a.y + tok[h] * a.ldy + n0 + c;
-                const float2 v = make_float2(base[n][h].x + d[n][2 * h], base[n][h].y + d[n][2 * h + 1]);
-                if (VEC && c + 1 < nn) *reinterpret_cast<float2 *>(p) = v;
+                if (VEC && c + 1 < nn) *reinterpret_cast<float2 *>(p) = make_float2(d[n][2 * h], d[n][2 * h + 1]);
                 else {
-                    if (c < nn) p[0] = v.x;
-                    if (c + 1 < nn) p[1] = v.y;
+                    if (c < nn) p[0] = d[n][2 * h];
+                    if (c + 1 < nn) p[1] = d[n][2 * h + 1];
                 }
             }
     }
@@ -1339,8 +1366,8 @@ extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(4) + 2) * 32
 extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(8) + 2) * 32) qm_lora_outer_r128(const __grid_constant__ QmLoraTcArgs a) { outer<8>(a); }
 extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_few_r16(const __grid_constant__ QmLoraFewArgs a) { few<1, true>(a); }
 extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_few_r16_s(const __grid_constant__ QmLoraFewArgs a) { few<1, false>(a); }
-extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_few_r32(const __grid_constant__ QmLoraFewArgs a) { few<2, true>(a); }
-extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_few_r32_s(const __grid_constant__ QmLoraFewArgs a) { few<2, false>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_few_r32(const __grid_constant__ QmLoraFewArgs a) { few<2, true>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_few_r32_s(const __grid_constant__ QmLoraFewArgs a) { few<2, false>(a); }
 extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_few_r64(const __grid_constant__ QmLoraFewArgs a) { few<4, true>(a); }
 extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_few_r64_s(const __grid_constant__ QmLoraFewArgs a) { few<4, false>(a); }
 extern "C" __global__ void __launch_bounds__(256) qm_lora_few_r128(const __grid_constant__ QmLoraFewArgs a) { few<8, true>(a); }
