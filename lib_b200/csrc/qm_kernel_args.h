@@ -422,6 +422,8 @@ struct QmGainSumArgs {
 #define QM_LORA_SHRINK_STAGES(rp) ((rp) <= 2 ? 5 : (rp) == 4 ? 4 : 3)
 #define QM_LORA_OUTER_STAGES(rp) ((rp) == 8 ? 3 : (rp) == 4 ? 5 : 4)
 #define QM_LORA_EXPAND_ROW(rp) (96 * (rp) + 16)   // bytes of a token's narrow products in expand's shared memory
+// warps of expand: with 8 KB of base each and the narrow products three CTAs fit on an SM, beyond 32 ranks two
+#define QM_LORA_EXPAND_WARPS(rp) ((rp) == 2 ? 7 : 8)
 #define QM_LORA_OUTER_COLS(rp) ((rp) <= 2 ? 256 : 128)
 #define QM_LORA_OUTER_READERS(rp) ((rp) == 8 ? 12 : 8)
 

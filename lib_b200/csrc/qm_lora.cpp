@@ -338,8 +338,10 @@ static int32_t expand_launch(qm_ctx *c, const qm_lora *l, QmLoraBatchArgs *a, in
     a->y = (float *)(uintptr_t)y;
     a->ldy = ldy;
     const bool vec = !((base | y) & 15) && !((ldb | ldy) & 3) && a->side[out_side].cols % 4 == 0;
+    const int rp = l->rpad / 16, threads = QM_LORA_EXPAND_WARPS(rp) * 32;
     return qm_launch(c, (vec ? QM_K_LORA_EXPAND_R16 : QM_K_LORA_EXPAND_R16_S) + rank_kernel(l), (unsigned)(2 * a->tiles_max),
-                     (unsigned)((a->side[out_side].cols + 255) / 256), 256, (unsigned)(65536 + 64 * QM_LORA_EXPAND_ROW(l->rpad / 16)), a, true);
+                     (unsigned)((a->side[out_side].cols + threads - 1) / threads), (unsigned)threads,
+                     (unsigned)(threads * 256 + 64 * QM_LORA_EXPAND_ROW(rp)), a, true);
 }
 
 static int32_t outer_launch(qm_ctx *c, const qm_lora *l, QmLoraTcArgs *ta, bool listed, uint64_t da, uint64_t db) {

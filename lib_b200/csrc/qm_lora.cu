@@ -1045,13 +1045,16 @@ __device__ __forceinline__ void shrink(const QmLoraTcArgs &ta) {
 }
 
 // ---- expand --------------------------------------------------------------------------------------------------------------
-// A CTA takes half a tile's tokens x 256 columns, each of its eight warps 32 columns. All of base is asked for at the start
-// (cp.async into the warp's own shared memory, no registers held), the tokens' narrow products once for the CTA; the
-// adapter's fragments of the columns stay in registers while the warp goes through the tokens, 16 at a time. The products
-// are added to base in shared memory and leave in rows of 128 bytes. Legacy mma on purpose: the same step by tcgen05 (operands
-// by TMA, results through tensor memory and shared memory, 128 columns per CTA) took 22.5 us instead of 20.5 at 2048 tokens x
-// 4096, rank 64, and 34 instead of 22 at 391 x 28672, rank 32, because every CTA then waits for tensor memory and two barriers
-// more; leaving the products out altogether saves 1 us. Copying base to y by the same steps takes 13.6 and 18 us.
+// A CTA takes half a tile's tokens x 32 columns for each of its seven or eight warps: as many as leave room for a third CTA on
+// the SM, beyond 32 ranks for a second one, which has its base on its way while this one multiplies (4096 tokens x 4096, rank
+// 32: three CTAs of seven warps 26.5 us, two of eight 28.6; at rank 64 three would have six, 21.8 us for 2048 tokens against
+// 20.5 with two of eight). All of base is asked for at the start (cp.async into the warp's own shared memory, no registers
+// held), the tokens' narrow products once for the CTA; the adapter's fragments of the columns stay in registers while the warp
+// goes through the tokens, 16 at a time. The products are added to base in shared memory and leave in rows of 128 bytes.
+// Legacy mma on purpose: the same step by tcgen05 (operands by TMA, results through tensor memory and shared memory, 128
+// columns per CTA) took 22.5 us instead of 20.5 at 2048 tokens x 4096, rank 64, and 34 instead of 22 at 391 x 28672, rank 32,
+// because every CTA then waits for tensor memory and two barriers more; leaving the products out altogether saves 1 us.
+// Copying base to y by the same steps takes 13.6 and 18 us.
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -1062,8 +1065,8 @@ __device__ __forceinline__ int staged(int r, int c) { return r * 32 + (((c >> 2)
 template <int RP, bool VEC>
 __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
     wait_for_inputs();
-    extern __shared__ __align__(128) unsigned char smem[];   // [8 warps][4][16][32] floats, then [64] rows of narrow products
-    constexpr int R = RP * 16, LP = QM_LORA_PITCH(RP), UB = QM_LORA_EXPAND_ROW(RP);
+    extern __shared__ __align__(128) unsigned char smem[];   // [warps][4][16][32] floats, then [64] rows of narrow products
+    constexpr int THREADS = QM_LORA_EXPAND_WARPS(RP) * 32, R = RP * 16, LP = QM_LORA_PITCH(RP), UB = QM_LORA_EXPAND_ROW(RP);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     Tile t = get_tile(a, blockIdx.x >> 1);
     if (blockIdx.x & 1) {
@@ -1074,18 +1077,18 @@ __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
     t.count = min(t.count, 64);
     if (t.count <= 0) return;
     const QmLoraSide &s = a.side[a.out_side];
-    const int c0 = blockIdx.y * 256 + warp * 32;
+    const int c0 = blockIdx.y * THREADS + warp * 32;   // (a column per thread)
     const int rank = t.slot < 0 ? 0 : t.rank;
     if (rank == 0 && a.base == a.y) return;
     const int mt = (t.count + 15) >> 4;
     const int g = lane >> 2, q = lane & 3;
     float *own = reinterpret_cast<float *>(smem) + warp * 4 * 512;
-    const uint32_t low = smem_u32(smem) + 65536;
+    const uint32_t low = smem_u32(smem) + THREADS * 256;
     // the tokens' numbers: lane holds rows l and 32 + l
     const int tok0 = token_at(a, t.first + min(lane, t.count - 1)), tok1 = token_at(a, t.first + min(lane + 32, t.count - 1));
     if (rank > 0) {
         const uint16_t *src = a.side[1 - a.out_side].low + (int64_t)t.row * LP;
-        for (int e = tid; e < mt * 16 * (6 * RP); e += 256) {   // rows of 3 R ranks: 6 RP pieces of 16 bytes
+        for (int e = tid; e < mt * 16 * (6 * RP); e += THREADS) {   // rows of 3 R ranks: 6 RP pieces of 16 bytes
             const int row = e / (6 * RP), piece = e % (6 * RP);
             copy16(low + row * UB + piece * 16, src + row * LP + piece * 8, 16);
         }
@@ -1352,14 +1355,14 @@ extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r16(
 extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r32(const __grid_constant__ QmLoraTcArgs a) { shrink<2>(a); }
 extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r64(const __grid_constant__ QmLoraTcArgs a) { shrink<4>(a); }
 extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r128(const __grid_constant__ QmLoraTcArgs a) { shrink<8>(a); }
-extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r16(const __grid_constant__ QmLoraBatchArgs a) { expand<1, true>(a); }
-extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r16_s(const __grid_constant__ QmLoraBatchArgs a) { expand<1, false>(a); }
-extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r32(const __grid_constant__ QmLoraBatchArgs a) { expand<2, true>(a); }
-extern "C" __global__ void __launch_bounds__(256, 3) qm_lora_expand_r32_s(const __grid_constant__ QmLoraBatchArgs a) { expand<2, false>(a); }
-extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_expand_r64(const __grid_constant__ QmLoraBatchArgs a) { expand<4, true>(a); }
-extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_expand_r64_s(const __grid_constant__ QmLoraBatchArgs a) { expand<4, false>(a); }
-extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_expand_r128(const __grid_constant__ QmLoraBatchArgs a) { expand<8, true>(a); }
-extern "C" __global__ void __launch_bounds__(256, 2) qm_lora_expand_r128_s(const __grid_constant__ QmLoraBatchArgs a) { expand<8, false>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(1) * 32, 3) qm_lora_expand_r16(const __grid_constant__ QmLoraBatchArgs a) { expand<1, true>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(1) * 32, 3) qm_lora_expand_r16_s(const __grid_constant__ QmLoraBatchArgs a) { expand<1, false>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(2) * 32, 3) qm_lora_expand_r32(const __grid_constant__ QmLoraBatchArgs a) { expand<2, true>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(2) * 32, 3) qm_lora_expand_r32_s(const __grid_constant__ QmLoraBatchArgs a) { expand<2, false>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(4) * 32, 3) qm_lora_expand_r64(const __grid_constant__ QmLoraBatchArgs a) { expand<4, true>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(4) * 32, 3) qm_lora_expand_r64_s(const __grid_constant__ QmLoraBatchArgs a) { expand<4, false>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(8) * 32, 2) qm_lora_expand_r128(const __grid_constant__ QmLoraBatchArgs a) { expand<8, true>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(8) * 32, 2) qm_lora_expand_r128_s(const __grid_constant__ QmLoraBatchArgs a) { expand<8, false>(a); }
 extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(1) + 2) * 32) qm_lora_outer_r16(const __grid_constant__ QmLoraTcArgs a) { outer<1>(a); }
 extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(2) + 2) * 32) qm_lora_outer_r32(const __grid_constant__ QmLoraTcArgs a) { outer<2>(a); }
 extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(4) + 2) * 32) qm_lora_outer_r64(const __grid_constant__ QmLoraTcArgs a) { outer<4>(a); }
