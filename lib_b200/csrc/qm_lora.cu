@@ -14,13 +14,13 @@
 // Forms: qm_lora_rows for 1..8 float32 rows and qm_lora_few_* for up to 128 bf16 tokens do shrink and expand in one launch;
 // beyond, and in the backward pass, qm_lora_lists orders the tokens by adapter and shrink, expand and outer are launches of
 // their own. Measured on one B200, calls back to back, floor = what has to move at the measured copy rate of 6.54 TB/s:
-//   1 row, 4096 x 4096, rank 16                       5.3 us   floor 0.05 (launch, five dependent trips to memory)
-//   8 rows, 8 adapters, 6144 x 4096, rank 64          9.2 us   floor 1.4  (the same, 112 KB of A and B per CTA)
+//   1 row, 4096 x 4096, rank 16                       5.5 us   floor 0.05 (launch, five dependent trips to memory)
+//   8 rows, 8 adapters, 6144 x 4096, rank 64          9.0 us   floor 1.4  (the same, 144 KB of A and B per CTA)
 //   64 tokens, 32 adapters, 6144 x 4096, rank 16      9.3 us   floor 1.9
-//   391 tokens, 28672 x 4096, rank 32                  36 us   floor 15   (expand: base in, y out)
+//   391 tokens, 28672 x 4096, rank 32                  35 us   floor 15   (expand: base in, y out)
 //   2048 tokens, 4096 x 14336, rank 64                 48 us   floor 22
 //   backward, 777 tokens, 6144 x 4096, rank 8          44 us   floor 6.5  (seven short launches)
-//   backward, 4096 tokens, 28672 x 4096, rank 32      155 us   floor 63   (dy is read twice: 235 MB more)
+//   backward, 4096 tokens, 28672 x 4096, rank 32      151 us   floor 63   (dy is read twice: 235 MB more)
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
