@@ -130,7 +130,10 @@ static const KernelName kKernels[QM_K_COUNT] = {
     {QM_MOD_LORA, "qm_lora_outer_r64"}, {QM_MOD_LORA, "qm_lora_outer_r128"}, {QM_MOD_LORA, "qm_lora_expand_r16"},
     {QM_MOD_LORA, "qm_lora_expand_r32"}, {QM_MOD_LORA, "qm_lora_expand_r64"}, {QM_MOD_LORA, "qm_lora_expand_r128"},
     {QM_MOD_LORA, "qm_lora_expand_r16_s"}, {QM_MOD_LORA, "qm_lora_expand_r32_s"}, {QM_MOD_LORA, "qm_lora_expand_r64_s"},
-    {QM_MOD_LORA, "qm_lora_expand_r128_s"}, {QM_MOD_LORA, "qm_lora_few_r16"}, {QM_MOD_LORA, "qm_lora_few_r32"},
+    {QM_MOD_LORA, "qm_lora_expand_r128_s"}, {QM_MOD_LORA, "qm_lora_shrink_r16_m"}, {QM_MOD_LORA, "qm_lora_shrink_r32_m"},
+    {QM_MOD_LORA, "qm_lora_shrink_r64_m"}, {QM_MOD_LORA, "qm_lora_shrink_r128_m"}, {QM_MOD_LORA, "qm_lora_expand_r16_m"},
+    {QM_MOD_LORA, "qm_lora_expand_r32_m"}, {QM_MOD_LORA, "qm_lora_expand_r64_m"}, {QM_MOD_LORA, "qm_lora_expand_r128_m"},
+    {QM_MOD_LORA, "qm_lora_few_r16"}, {QM_MOD_LORA, "qm_lora_few_r32"},
     {QM_MOD_LORA, "qm_lora_few_r64"}, {QM_MOD_LORA, "qm_lora_few_r128"}, {QM_MOD_LORA, "qm_lora_few_r16_s"},
     {QM_MOD_LORA, "qm_lora_few_r32_s"}, {QM_MOD_LORA, "qm_lora_few_r64_s"}, {QM_MOD_LORA, "qm_lora_few_r128_s"},
     {QM_MOD_ROPE, "qm_qk_norm_w1"}, {QM_MOD_ROPE, "qm_qk_norm_w2"}, {QM_MOD_ROPE, "qm_qk_norm_w4"}, {QM_MOD_ROPE, "qm_qk_norm_s8"},

@@ -38,6 +38,8 @@ enum {
     QM_K_LORA_SHRINK_R128, QM_K_LORA_OUTER_R16, QM_K_LORA_OUTER_R32, QM_K_LORA_OUTER_R64, QM_K_LORA_OUTER_R128,
     QM_K_LORA_EXPAND_R16, QM_K_LORA_EXPAND_R32, QM_K_LORA_EXPAND_R64, QM_K_LORA_EXPAND_R128,
     QM_K_LORA_EXPAND_R16_S, QM_K_LORA_EXPAND_R32_S, QM_K_LORA_EXPAND_R64_S, QM_K_LORA_EXPAND_R128_S,
+    QM_K_LORA_SHRINK_R16_M, QM_K_LORA_SHRINK_R32_M, QM_K_LORA_SHRINK_R64_M, QM_K_LORA_SHRINK_R128_M,
+    QM_K_LORA_EXPAND_R16_M, QM_K_LORA_EXPAND_R32_M, QM_K_LORA_EXPAND_R64_M, QM_K_LORA_EXPAND_R128_M,
     QM_K_LORA_FEW_R16, QM_K_LORA_FEW_R32, QM_K_LORA_FEW_R64, QM_K_LORA_FEW_R128,
     QM_K_LORA_FEW_R16_S, QM_K_LORA_FEW_R32_S, QM_K_LORA_FEW_R64_S, QM_K_LORA_FEW_R128_S,
     QM_K_QK_NORM_W1, QM_K_QK_NORM_W2, QM_K_QK_NORM_W4, QM_K_QK_NORM_S8,

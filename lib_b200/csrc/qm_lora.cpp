@@ -320,14 +320,31 @@ static int32_t share(const qm_lora *l, int64_t units, int64_t steps, int per_sm)
     return best;
 }
 
+// Clusters of `split` CTAs that run at once, `per_sm` CTAs on an SM.
+static int64_t at_once(const qm_lora *l, int32_t split, int per_sm) {
+    return (int64_t)per_sm * std::max(1, l->at_once[split == 1 ? 0 : split == 2 ? 1 : split == 4 ? 2 : 3]);
+}
+// How many tiles there are only the device knows, so the grids are made for every adapter having tokens. A CTA without a tile
+// costs about 1 ns of the whole (4 ns where it asks for tensor memory): thousands of them are a loss with hundreds of slots of
+// which few are in use, and then _m kernels with a grid that fills the GPU a few times take one tile after another. 256 slots,
+// four in use: 391 tokens, 28672 x 4096, rank 32: 39 us instead of 96; 2048 tokens, 4096 x 4096, rank 16: 31 instead of 43. With
+// all 256 in use they take 247 instead of 261 and 104 instead of 102. For every grid they would cost 5 % (2048 tokens, four
+// slots: 28.5 instead of 26.6), and for both sides of a backward pass, whose next kernel starts while the last tiles are worked
+// on, 5 % too (2048 tokens, four of 256 slots: 357 us instead of 341).
+constexpr int64_t IDLE_SHRINK = 1024, IDLE_EXPAND = 8192;
+
 static int32_t shrink_launch(qm_ctx *c, const qm_lora *l, QmLoraTcArgs *ta, int sides) {
     QmLoraBatchArgs *a = &ta->b;
     const int64_t cols = sides == 2 ? std::max(l->cols, l->rows) : l->cols;
+    const int64_t whole = sides * (((int64_t)a->tokens + QM_LORA_TILE - 1) / QM_LORA_TILE);
     a->first_side = sides == 2 && l->rows > l->cols;   // the longer one first, the shorter one fills its last wave
     // (the tiles that are there for certain; those that short lists add come on top)
-    a->split = share(l, sides * (int64_t)((a->tokens + QM_LORA_TILE - 1) / QM_LORA_TILE), (cols + 63) / 64, 2);
-    return qm_launch_ex(c, QM_K_LORA_SHRINK_R16 + rank_kernel(l), (unsigned)(sides * a->tiles_max * a->split), 192, (unsigned)shrink_smem(l), ta,
-                        true, false, a->split);
+    a->split = share(l, whole, (cols + 63) / 64, 2);
+    int64_t clusters = sides * (int64_t)a->tiles_max;
+    const bool many = sides == 1 && (clusters - whole) * a->split > IDLE_SHRINK;
+    if (many) clusters = std::min(clusters, std::max(whole, 2 * at_once(l, a->split, 2)));
+    return qm_launch_ex(c, (many ? QM_K_LORA_SHRINK_R16_M : QM_K_LORA_SHRINK_R16) + rank_kernel(l), (unsigned)(clusters * a->split), 192,
+                        (unsigned)shrink_smem(l), ta, true, false, a->split);
 }
 
 static int32_t expand_launch(qm_ctx *c, const qm_lora *l, QmLoraBatchArgs *a, int out_side, uint64_t base, int64_t ldb, uint64_t y,
@@ -338,9 +355,14 @@ static int32_t expand_launch(qm_ctx *c, const qm_lora *l, QmLoraBatchArgs *a, in
     a->y = (float *)(uintptr_t)y;
     a->ldy = ldy;
     const bool vec = !((base | y) & 15) && !((ldb | ldy) & 3) && a->side[out_side].cols % 4 == 0;
-    const int rp = l->rpad / 16, threads = QM_LORA_EXPAND_WARPS(rp) * 32;
-    return qm_launch(c, (vec ? QM_K_LORA_EXPAND_R16 : QM_K_LORA_EXPAND_R16_S) + rank_kernel(l), (unsigned)(2 * a->tiles_max),
-                     (unsigned)((a->side[out_side].cols + threads - 1) / threads), (unsigned)threads,
+    const int rp = l->rpad / 16, threads = QM_LORA_EXPAND_WARPS(rp) * 32, across = (a->side[out_side].cols + threads - 1) / threads;
+    const int64_t whole = ((int64_t)a->tokens + 63) / 64;
+    int64_t halves = 2 * (int64_t)a->tiles_max;
+    const bool many = vec && (halves - whole) * across > IDLE_EXPAND;
+    // (an odd number: the halves of a CTA are first and second ones in turn, second ones are often empty)
+    if (many) halves = std::min(halves, std::max<int64_t>(whole, 8ll * c->sm_count / across) | 1);
+    return qm_launch(c, (many ? QM_K_LORA_EXPAND_R16_M : vec ? QM_K_LORA_EXPAND_R16 : QM_K_LORA_EXPAND_R16_S) + rank_kernel(l), (unsigned)halves,
+                     (unsigned)across, (unsigned)threads,
                      (unsigned)(threads * 256 + 64 * QM_LORA_EXPAND_ROW(rp)), a, true);
 }
 

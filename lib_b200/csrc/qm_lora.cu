@@ -885,14 +885,26 @@ __device__ __forceinline__ void pipe_close(const Pipe &p, uint32_t cols) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// Where a CTA that takes one piece of work after another is: stages and periods before this piece, and whether every wait has
+// ended so far (after one that has not, its warp does no more).
+struct Progress {
+    int stages, periods;
+    bool ok;
+};
+__device__ __forceinline__ void advance(Progress &g, int cn) {
+    g.stages += cn;
+    g.periods += (cn + PERIOD - 1) / PERIOD;
+}
+// Before the stages that ordinary loads and stores have used are filled by TMA again.
+__device__ __forceinline__ void stages_used() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // The multiplying thread: stage by stage, `issue(stage address, accumulator, first of a period)`.
 template <int STAGES, int NACC, class F>
-__device__ __forceinline__ void pipe_multiply(const Pipe &p, uint32_t base, uint32_t stage_bytes, int cn, unsigned int *status, F issue) {
-    for (int c = 0; c < cn; c++) {
-        const int st = c % STAGES, period = c / PERIOD, acc = period % NACC;
-        bool ok = true;
-        if (c % PERIOD == 0 && period >= NACC) ok = qm::mbar_wait_bounded(p.acc_empty + 8 * acc, (uint32_t)(period / NACC - 1) & 1u);
-        if (!ok || !qm::mbar_wait_bounded(p.full + 8 * st, (uint32_t)(c / STAGES) & 1u)) {
+__device__ __forceinline__ void pipe_multiply(const Pipe &p, Progress &g, uint32_t base, uint32_t stage_bytes, int cn, unsigned int *status, F issue) {
+    for (int c = 0; c < cn && g.ok; c++) {
+        const int n = g.stages + c, st = n % STAGES, period = g.periods + c / PERIOD, acc = period % NACC;
+        if (c % PERIOD == 0 && period >= NACC) g.ok = qm::mbar_wait_bounded(p.acc_empty + 8 * acc, (uint32_t)(period / NACC - 1) & 1u);
+        g.ok = g.ok && qm::mbar_wait_bounded(p.full + 8 * st, (uint32_t)(n / STAGES) & 1u);
+        if (!g.ok) {
             atomicOr(status, QM_STATUS_TIMEOUT);
             return;
         }
@@ -904,13 +916,15 @@ __device__ __forceinline__ void pipe_multiply(const Pipe &p, uint32_t base, uint
 }
 // A reading warp: adds each period's accumulator columns `first`.. to v.
 template <int N, int NACC>
-__device__ __forceinline__ void pipe_read(const Pipe &p, uint32_t acc_cols, uint32_t first, int cn, unsigned int *status, float (&v)[N]) {
+__device__ __forceinline__ void pipe_read(const Pipe &p, Progress &g, uint32_t acc_cols, uint32_t first, int cn, unsigned int *status, float (&v)[N]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int i = 0; i < N; i++) v[i] = 0.f;
-    for (int period = 0; period * PERIOD < cn; period++) {
-        const int acc = period % NACC;
-        if (!qm::mbar_wait_bounded(p.acc_full + 8 * acc, (uint32_t)(period / NACC) & 1u)) {
+    for (int i = 0; i * PERIOD < cn && g.ok; i++) {
+        const int period = g.periods + i, acc = period % NACC;
+        // (one answer for the warp, whose lanes are together for what follows)
+        g.ok = __all_sync(0xffffffffu, qm::mbar_wait_bounded(p.acc_full + 8 * acc, (uint32_t)(period / NACC) & 1u));
+        if (!g.ok) {
             if (lane == 0) atomicOr(status, QM_STATUS_TIMEOUT);
             return;
         }
@@ -946,9 +960,10 @@ __device__ __forceinline__ bool neighbours(const int (&rows)[4], int there) {
 // bounds it. The CTAs' sums meet in distributed shared memory and are added in a fixed order. 4096 tokens, x of 4096 and dy of
 // 28672 columns, rank 32: 52 us, 5.2 TB/s (legacy mma with cp.async: 67 us, and 71 instead of 22 at 2048 tokens x 14336, rank
 // 64, where its fragments kept the issue slots and the shared memory busy).
+// MANY: one side, fewer clusters than there may be tiles, each takes one after another.
 constexpr int SHRINK_THREADS = 192;   // four warps that read the accumulators, one that loads, one that multiplies
 
-template <int RP>
+template <int RP, bool MANY>
 __device__ __forceinline__ void shrink(const QmLoraTcArgs &ta) {
     const QmLoraBatchArgs &a = ta.b;
     extern __shared__ unsigned char smem_raw[];
@@ -958,11 +973,13 @@ __device__ __forceinline__ void shrink(const QmLoraTcArgs &ta) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const Pipe pipe = pipe_open<STAGES>(smem + STAGES * STAGE, TCOLS, 4);
     const int me = a.split > 1 ? (int)cluster_rank() : 0;
-    const int unit = blockIdx.x / a.split;
-    const int side = unit < a.tiles_max ? a.first_side : 1 - a.first_side;
-    const QmLoraSide &s = a.side[side];
-    const Tile t = get_tile(a, unit < a.tiles_max ? unit : unit - a.tiles_max);
-    if (t.count > 0 && t.slot >= 0) {   // the same for the whole cluster
+    Progress at_now = {0, 0, true};
+    int unit = blockIdx.x / a.split;
+    do {
+        const int side = unit < a.tiles_max ? a.first_side : 1 - a.first_side;
+        const QmLoraSide &s = a.side[side];
+        const Tile t = get_tile(a, unit < a.tiles_max ? unit : unit - a.tiles_max);
+        if (t.count <= 0 || t.slot < 0) continue;   // the same for the whole cluster
         const int chunks = (s.cols + 63) / 64, cn = max(0, (chunks - me + a.split - 1) / a.split);
         const uint32_t base = smem_u32(smem);
         float *part = reinterpret_cast<float *>(smem);   // [128][R + 4], over the stages once they are done
@@ -977,9 +994,10 @@ __device__ __forceinline__ void shrink(const QmLoraTcArgs &ta) {
             const bool box = neighbours(rows, there);
             const bool one = box ? (lane & 7) == 0 && there > 0 : there > 0;
             const uint32_t bytes = __reduce_add_sync(0xffffffffu, one ? (box ? 4096u : 512u) : 0u) + R * 128;
-            for (int c = 0; c < cn; c++) {
-                const int st = c % STAGES;
-                if (c >= STAGES && !qm::mbar_wait_bounded(pipe.empty + 8 * st, (uint32_t)(c / STAGES - 1) & 1u)) {
+            for (int c = 0; c < cn && at_now.ok; c++) {
+                const int n = at_now.stages + c, st = n % STAGES;
+                at_now.ok = n < STAGES || qm::mbar_wait_bounded(pipe.empty + 8 * st, (uint32_t)(n / STAGES - 1) & 1u);
+                if (!at_now.ok) {
                     if (lane == 0) atomicOr(a.status, QM_STATUS_TIMEOUT);
                     break;
                 }
@@ -997,14 +1015,14 @@ __device__ __forceinline__ void shrink(const QmLoraTcArgs &ta) {
             }
         } else if (warp == 5) {
             if (lane == 0)
-                pipe_multiply<STAGES, 2>(pipe, base, STAGE, cn, a.status, [&](uint32_t at, int acc, bool first) {
+                pipe_multiply<STAGES, 2>(pipe, at_now, base, STAGE, cn, a.status, [&](uint32_t at, int acc, bool first) {
                     const uint64_t x = tile_desc(at, 16), w = tile_desc(at + XB, 16);
 #pragma unroll
                     for (int k = 0; k < 4; k++)   // 16 columns = 32 bytes = 2 descriptor units
                         tc_mma(pipe.tmem + acc * R, x + 2 * k, w + 2 * k, tc_idesc(R, false), !first || k > 0);
                 });
         } else {
-            pipe_read<R, 2>(pipe, R, 0, cn, a.status, v);
+            pipe_read<R, 2>(pipe, at_now, R, 0, cn, a.status, v);
         }
         __syncthreads();   // nothing uses the stages any more
         if (warp < 4) {
@@ -1036,11 +1054,15 @@ __device__ __forceinline__ void shrink(const QmLoraTcArgs &ta) {
             for (int k = 0; k < 3; k++)
                 *reinterpret_cast<uint2 *>(out + k * R) = make_uint2(p[0][k] | p[1][k] << 16, p[2][k] | p[3][k] << 16);
         }
+        if (MANY) stages_used();
         if (a.split > 1) {
             cluster_arrive();
             cluster_wait();
+        } else if (MANY) {
+            __syncthreads();
         }
-    }
+        advance(at_now, cn);
+    } while (MANY && (unit += gridDim.x / a.split) < a.tiles_max);
     pipe_close(pipe, TCOLS);
 }
 
@@ -1055,6 +1077,7 @@ __device__ __forceinline__ void shrink(const QmLoraTcArgs &ta) {
 // columns per CTA) took 22.5 us instead of 20.5 at 2048 tokens x 4096, rank 64, and 34 instead of 22 at 391 x 28672, rank 32,
 // because every CTA then waits for tensor memory and two barriers more; leaving the products out altogether saves 1 us.
 // Copying base to y by the same steps takes 13.6 and 18 us.
+// MANY: fewer CTAs than there may be halves of tiles, each takes one after another.
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -1062,139 +1085,146 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void *src, int bytes) 
 // the fragments' accesses (four rows x 32 bytes at a time) nor whole rows meet a bank twice.
 __device__ __forceinline__ int staged(int r, int c) { return r * 32 + (((c >> 2) ^ (2 * (r & 3))) << 2) + (c & 3); }
 
-template <int RP, bool VEC>
+template <int RP, bool VEC, bool MANY>
 __device__ __forceinline__ void expand(const QmLoraBatchArgs &a) {
     wait_for_inputs();
     extern __shared__ __align__(128) unsigned char smem[];   // [warps][4][16][32] floats, then [64] rows of narrow products
     constexpr int THREADS = QM_LORA_EXPAND_WARPS(RP) * 32, R = RP * 16, LP = QM_LORA_PITCH(RP), UB = QM_LORA_EXPAND_ROW(RP);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    Tile t = get_tile(a, blockIdx.x >> 1);
-    if (blockIdx.x & 1) {
-        t.first += 64;
-        t.row += 64;
-        t.count -= 64;
-    }
-    t.count = min(t.count, 64);
-    if (t.count <= 0) return;
     const QmLoraSide &s = a.side[a.out_side];
     const int c0 = blockIdx.y * THREADS + warp * 32;   // (a column per thread)
-    const int rank = t.slot < 0 ? 0 : t.rank;
-    if (rank == 0 && a.base == a.y) return;
-    const int mt = (t.count + 15) >> 4;
-    const int g = lane >> 2, q = lane & 3;
-    float *own = reinterpret_cast<float *>(smem) + warp * 4 * 512;
-    const uint32_t low = smem_u32(smem) + THREADS * 256;
-    // the tokens' numbers: lane holds rows l and 32 + l
-    const int tok0 = token_at(a, t.first + min(lane, t.count - 1)), tok1 = token_at(a, t.first + min(lane + 32, t.count - 1));
-    if (rank > 0) {
-        const uint16_t *src = a.side[1 - a.out_side].low + (int64_t)t.row * LP;
-        for (int e = tid; e < mt * 16 * (6 * RP); e += THREADS) {   // rows of 3 R ranks: 6 RP pieces of 16 bytes
-            const int row = e / (6 * RP), piece = e % (6 * RP);
-            copy16(low + row * UB + piece * 16, src + row * LP + piece * 8, 16);
+    int half = blockIdx.x;
+    bool used = false;   // shared memory
+    do {
+        Tile t = get_tile(a, half >> 1);
+        if (MANY && t.count <= 0) return;
+        if (half & 1) {
+            t.first += 64;
+            t.row += 64;
+            t.count -= 64;
         }
-    }
-    copy_commit();
-    constexpr int KB = RP == 1 ? 1 : RP / 2;      // groups of 32 ranks (one of 16)
-    constexpr int W = RP == 1 ? 4 : 8;            // ranks of a lane
-    const int kb = RP == 1 ? (rank > 0) : (rank + 31) / 32;
-    // (asked for before base, behind which they would come last)
-    uint32_t fb[KB][4][W / 2];
+        t.count = min(t.count, 64);
+        if (t.count <= 0) continue;
+        const int rank = t.slot < 0 ? 0 : t.rank;
+        if (rank == 0 && a.base == a.y) continue;
+        if (MANY && used) __syncthreads();
+        used = true;
+        const int mt = (t.count + 15) >> 4;
+        const int g = lane >> 2, q = lane & 3;
+        float *own = reinterpret_cast<float *>(smem) + warp * 4 * 512;
+        const uint32_t low = smem_u32(smem) + THREADS * 256;
+        // the tokens' numbers: lane holds rows l and 32 + l
+        const int tok0 = token_at(a, t.first + min(lane, t.count - 1)), tok1 = token_at(a, t.first + min(lane + 32, t.count - 1));
+        if (rank > 0) {
+            const uint16_t *src = a.side[1 - a.out_side].low + (int64_t)t.row * LP;
+            for (int e = tid; e < mt * 16 * (6 * RP); e += THREADS) {   // rows of 3 R ranks: 6 RP pieces of 16 bytes
+                const int row = e / (6 * RP), piece = e % (6 * RP);
+                copy16(low + row * UB + piece * 16, src + row * LP + piece * 8, 16);
+            }
+        }
+        copy_commit();
+        constexpr int KB = RP == 1 ? 1 : RP / 2;      // groups of 32 ranks (one of 16)
+        constexpr int W = RP == 1 ? 4 : 8;            // ranks of a lane
+        const int kb = RP == 1 ? (rank > 0) : (rank + 31) / 32;
+        // (asked for before base, behind which they would come last)
+        uint32_t fb[KB][4][W / 2];
 #pragma unroll
-    for (int k = 0; k < KB; k++)
+        for (int k = 0; k < KB; k++)
 #pragma unroll
-        for (int n = 0; n < 4; n++)   // (a column behind the last one: any other, the result is not stored)
-            if (k < kb) {
-                const uint16_t *p = s.wt + ((int64_t)t.slot * s.cols + min(c0 + n * 8 + g, s.cols - 1)) * R + k * 32 + W * q;
-                if constexpr (W == 8) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(p);
-                    fb[k][n][0] = v.x; fb[k][n][1] = v.y; fb[k][n][2] = v.z; fb[k][n][3] = v.w;
+            for (int n = 0; n < 4; n++)   // (a column behind the last one: any other, the result is not stored)
+                if (k < kb) {
+                    const uint16_t *p = s.wt + ((int64_t)t.slot * s.cols + min(c0 + n * 8 + g, s.cols - 1)) * R + k * 32 + W * q;
+                    if constexpr (W == 8) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+                        fb[k][n][0] = v.x; fb[k][n][1] = v.y; fb[k][n][2] = v.z; fb[k][n][3] = v.w;
+                    } else {
+                        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+                        fb[k][n][0] = v.x; fb[k][n][1] = v.y;
+                    }
+                }
+        const bool mine = c0 < s.cols;
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            if (m < mt && mine) {
+                if constexpr (VEC) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int r = (lane >> 3) + 4 * i, c = 4 * (lane & 7);
+                        const int64_t row = __shfl_sync(0xffffffffu, m < 2 ? tok0 : tok1, (m & 1) * 16 + r);
+                        const bool in = a.base && m * 16 + r < t.count && c0 + c < s.cols;
+                        copy16(smem_u32(own + m * 512 + staged(r, c)), in ? (const void *)(a.base + row * a.ldb + c0 + c) : (const void *)s.wt, in ? 16 : 0);
+                    }
                 } else {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-                    fb[k][n][0] = v.x; fb[k][n][1] = v.y;
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const int64_t row = __shfl_sync(0xffffffffu, m < 2 ? tok0 : tok1, (m & 1) * 16 + r);
+                        const bool in = a.base && m * 16 + r < t.count && c0 + lane < s.cols;
+                        copy4(smem_u32(own + m * 512 + staged(r, lane)), in ? (const void *)(a.base + row * a.ldb + c0 + lane) : (const void *)s.wt, in ? 4 : 0);
+                    }
                 }
             }
-    const bool mine = c0 < s.cols;
+            copy_commit();
+        }
+        copy_wait<4>();
+        __syncthreads();
+        if (!mine) continue;
 #pragma unroll
-    for (int m = 0; m < 4; m++) {
-        if (m < mt && mine) {
+        for (int m = 0; m < 4; m++) {
+            if (m >= mt) break;
+            float d[4][4];
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) d[n][k] = 0.f;
+            const uint32_t lm = low + (m * 16 + (lane & 15)) * UB + (lane >> 4) * 16;
+#pragma unroll
+            for (int k = 0; k < KB; k++)
+                if (k < kb) {
+#pragma unroll
+                    for (int p = 2; p >= 0; p--)   // the small parts first
+#pragma unroll
+                        for (int j = 0; j < W / 4; j++) {
+                            uint32_t fa[4];
+                            ldsm4(lm + (p * R + k * 32 + j * 16) * 2, fa);
+#pragma unroll
+                            for (int n = 0; n < 4; n++) mma(d[n], fa, fb[k][n][2 * j], fb[k][n][2 * j + 1]);
+                        }
+                }
+            if (m == 0) copy_wait<3>();
+            else if (m == 1) copy_wait<2>();
+            else if (m == 2) copy_wait<1>();
+            else copy_wait<0>();
+            __syncwarp();
+            float *st = own + m * 512;
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float2 *p = reinterpret_cast<float2 *>(st + staged(g + 8 * h, n * 8 + 2 * q));
+                    float2 v = *p;
+                    v.x += d[n][2 * h];
+                    v.y += d[n][2 * h + 1];
+                    *p = v;
+                }
+            __syncwarp();
             if constexpr (VEC) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int r = (lane >> 3) + 4 * i, c = 4 * (lane & 7);
                     const int64_t row = __shfl_sync(0xffffffffu, m < 2 ? tok0 : tok1, (m & 1) * 16 + r);
-                    const bool in = a.base && m * 16 + r < t.count && c0 + c < s.cols;
-                    copy16(smem_u32(own + m * 512 + staged(r, c)), in ? (const void *)(a.base + row * a.ldb + c0 + c) : (const void *)s.wt, in ? 16 : 0);
+                    const float4 v = *reinterpret_cast<const float4 *>(st + staged(r, c));
+                    if (m * 16 + r < t.count && c0 + c < s.cols) *reinterpret_cast<float4 *>(a.y + row * a.ldy + c0 + c) = v;
                 }
             } else {
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const int64_t row = __shfl_sync(0xffffffffu, m < 2 ? tok0 : tok1, (m & 1) * 16 + r);
-                    const bool in = a.base && m * 16 + r < t.count && c0 + lane < s.cols;
-                    copy4(smem_u32(own + m * 512 + staged(r, lane)), in ? (const void *)(a.base + row * a.ldb + c0 + lane) : (const void *)s.wt, in ? 4 : 0);
+                    const float v = st[staged(r, lane)];
+                    if (m * 16 + r < t.count && c0 + lane < s.cols) a.y[row * a.ldy + c0 + lane] = v;
                 }
             }
         }
-        copy_commit();
-    }
-    copy_wait<4>();
-    __syncthreads();
-    if (!mine) return;
-#pragma unroll
-    for (int m = 0; m < 4; m++) {
-        if (m >= mt) break;
-        float d[4][4];
-#pragma unroll
-        for (int n = 0; n < 4; n++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) d[n][k] = 0.f;
-        const uint32_t lm = low + (m * 16 + (lane & 15)) * UB + (lane >> 4) * 16;
-#pragma unroll
-        for (int k = 0; k < KB; k++)
-            if (k < kb) {
-#pragma unroll
-                for (int p = 2; p >= 0; p--)   // the small parts first
-#pragma unroll
-                    for (int j = 0; j < W / 4; j++) {
-                        uint32_t fa[4];
-                        ldsm4(lm + (p * R + k * 32 + j * 16) * 2, fa);
-#pragma unroll
-                        for (int n = 0; n < 4; n++) mma(d[n], fa, fb[k][n][2 * j], fb[k][n][2 * j + 1]);
-                    }
-            }
-        if (m == 0) copy_wait<3>();
-        else if (m == 1) copy_wait<2>();
-        else if (m == 2) copy_wait<1>();
-        else copy_wait<0>();
-        __syncwarp();
-        float *st = own + m * 512;
-#pragma unroll
-        for (int n = 0; n < 4; n++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                float2 *p = reinterpret_cast<float2 *>(st + staged(g + 8 * h, n * 8 + 2 * q));
-                float2 v = *p;
-                v.x += d[n][2 * h];
-                v.y += d[n][2 * h + 1];
-                *p = v;
-            }
-        __syncwarp();
-        if constexpr (VEC) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int r = (lane >> 3) + 4 * i, c = 4 * (lane & 7);
-                const int64_t row = __shfl_sync(0xffffffffu, m < 2 ? tok0 : tok1, (m & 1) * 16 + r);
-                const float4 v = *reinterpret_cast<const float4 *>(st + staged(r, c));
-                if (m * 16 + r < t.count && c0 + c < s.cols) *reinterpret_cast<float4 *>(a.y + row * a.ldy + c0 + c) = v;
-            }
-        } else {
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int64_t row = __shfl_sync(0xffffffffu, m < 2 ? tok0 : tok1, (m & 1) * 16 + r);
-                const float v = st[staged(r, lane)];
-                if (m * 16 + r < t.count && c0 + lane < s.cols) a.y[row * a.ldy + c0 + lane] = v;
-            }
-        }
-    }
+    } while (MANY && (half += gridDim.x) < 2 * a.tiles_max);
 }
 
 // ---- outer ---------------------------------------------------------------------------------------------------------------
@@ -1240,6 +1270,7 @@ __device__ __forceinline__ void outer(const QmLoraTcArgs &ta) {
         float *part = reinterpret_cast<float *>(smem);   // [R][BN + 4], over the stages once they are done
         constexpr int LD = BN + 4;
         float v[MINE];
+        Progress at_now = {0, 0, true};
         if (warp == READERS) {
             // lanes 0..15: the tokens of four rows of a block; asked for four blocks ahead
             constexpr int AHEAD = 4;
@@ -1281,7 +1312,7 @@ __device__ __forceinline__ void outer(const QmLoraTcArgs &ta) {
                 }
         } else if (warp == READERS + 1) {
             if (lane == 0)
-                pipe_multiply<STAGES, NACC>(pipe, base, STAGE, cn, a.status, [&](uint32_t at, int acc, bool begin) {
+                pipe_multiply<STAGES, NACC>(pipe, at_now, base, STAGE, cn, a.status, [&](uint32_t at, int acc, bool begin) {
                     const uint64_t x = tile_desc(at + AB, 8192);
 #pragma unroll
                     for (int m = 0; m < MM; m++) {
@@ -1293,7 +1324,7 @@ __device__ __forceinline__ void outer(const QmLoraTcArgs &ta) {
                     }
                 });
         } else {
-            pipe_read<MINE, NACC>(pipe, MM * BN, (warp >> 2) * MINE, cn, a.status, v);
+            pipe_read<MINE, NACC>(pipe, at_now, MM * BN, (warp >> 2) * MINE, cn, a.status, v);
         }
         // row m of the accumulators is rank m % R of part m / R: the smallest part first, the others onto it
 #pragma unroll
@@ -1351,18 +1382,26 @@ __device__ __forceinline__ void outer(const QmLoraTcArgs &ta) {
 
 }  // namespace
 
-extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r16(const __grid_constant__ QmLoraTcArgs a) { shrink<1>(a); }
-extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r32(const __grid_constant__ QmLoraTcArgs a) { shrink<2>(a); }
-extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r64(const __grid_constant__ QmLoraTcArgs a) { shrink<4>(a); }
-extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r128(const __grid_constant__ QmLoraTcArgs a) { shrink<8>(a); }
-extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(1) * 32, 3) qm_lora_expand_r16(const __grid_constant__ QmLoraBatchArgs a) { expand<1, true>(a); }
-extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(1) * 32, 3) qm_lora_expand_r16_s(const __grid_constant__ QmLoraBatchArgs a) { expand<1, false>(a); }
-extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(2) * 32, 3) qm_lora_expand_r32(const __grid_constant__ QmLoraBatchArgs a) { expand<2, true>(a); }
-extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(2) * 32, 3) qm_lora_expand_r32_s(const __grid_constant__ QmLoraBatchArgs a) { expand<2, false>(a); }
-extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(4) * 32, 3) qm_lora_expand_r64(const __grid_constant__ QmLoraBatchArgs a) { expand<4, true>(a); }
-extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(4) * 32, 3) qm_lora_expand_r64_s(const __grid_constant__ QmLoraBatchArgs a) { expand<4, false>(a); }
-extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(8) * 32, 2) qm_lora_expand_r128(const __grid_constant__ QmLoraBatchArgs a) { expand<8, true>(a); }
-extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(8) * 32, 2) qm_lora_expand_r128_s(const __grid_constant__ QmLoraBatchArgs a) { expand<8, false>(a); }
+extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r16(const __grid_constant__ QmLoraTcArgs a) { shrink<1, false>(a); }
+extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r32(const __grid_constant__ QmLoraTcArgs a) { shrink<2, false>(a); }
+extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r64(const __grid_constant__ QmLoraTcArgs a) { shrink<4, false>(a); }
+extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r128(const __grid_constant__ QmLoraTcArgs a) { shrink<8, false>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(1) * 32, 3) qm_lora_expand_r16(const __grid_constant__ QmLoraBatchArgs a) { expand<1, true, false>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(1) * 32, 3) qm_lora_expand_r16_s(const __grid_constant__ QmLoraBatchArgs a) { expand<1, false, false>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(2) * 32, 3) qm_lora_expand_r32(const __grid_constant__ QmLoraBatchArgs a) { expand<2, true, false>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(2) * 32, 3) qm_lora_expand_r32_s(const __grid_constant__ QmLoraBatchArgs a) { expand<2, false, false>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(4) * 32, 3) qm_lora_expand_r64(const __grid_constant__ QmLoraBatchArgs a) { expand<4, true, false>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(4) * 32, 3) qm_lora_expand_r64_s(const __grid_constant__ QmLoraBatchArgs a) { expand<4, false, false>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(8) * 32, 2) qm_lora_expand_r128(const __grid_constant__ QmLoraBatchArgs a) { expand<8, true, false>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(8) * 32, 2) qm_lora_expand_r128_s(const __grid_constant__ QmLoraBatchArgs a) { expand<8, false, false>(a); }
+extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r16_m(const __grid_constant__ QmLoraTcArgs a) { shrink<1, true>(a); }
+extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r32_m(const __grid_constant__ QmLoraTcArgs a) { shrink<2, true>(a); }
+extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r64_m(const __grid_constant__ QmLoraTcArgs a) { shrink<4, true>(a); }
+extern "C" __global__ void __launch_bounds__(SHRINK_THREADS) qm_lora_shrink_r128_m(const __grid_constant__ QmLoraTcArgs a) { shrink<8, true>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(1) * 32, 3) qm_lora_expand_r16_m(const __grid_constant__ QmLoraBatchArgs a) { expand<1, true, true>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(2) * 32, 3) qm_lora_expand_r32_m(const __grid_constant__ QmLoraBatchArgs a) { expand<2, true, true>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(4) * 32, 3) qm_lora_expand_r64_m(const __grid_constant__ QmLoraBatchArgs a) { expand<4, true, true>(a); }
+extern "C" __global__ void __launch_bounds__(QM_LORA_EXPAND_WARPS(8) * 32, 2) qm_lora_expand_r128_m(const __grid_constant__ QmLoraBatchArgs a) { expand<8, true, true>(a); }
 extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(1) + 2) * 32) qm_lora_outer_r16(const __grid_constant__ QmLoraTcArgs a) { outer<1>(a); }
 extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(2) + 2) * 32) qm_lora_outer_r32(const __grid_constant__ QmLoraTcArgs a) { outer<2>(a); }
 extern "C" __global__ void __launch_bounds__((QM_LORA_OUTER_READERS(4) + 2) * 32) qm_lora_outer_r64(const __grid_constant__ QmLoraTcArgs a) { outer<4>(a); }

@@ -390,6 +390,43 @@ def test_slots_are_replaced_and_emptied(ctx, adapters, type, kept):
     check()
 
 
+@pytest.mark.parametrize("R,used", [(16, 3), (16, 256), (32, 64), (64, 40), (128, 32)])
+def test_many_slots(ctx, adapters, R, used):
+    """Hundreds of slots, few or all of them with tokens: the grids are smaller than the tiles there may be."""
+    rows, cols, tokens, slots = 4096, 4224, 1100, 256
+    held = list(range(0, slots, slots // used))[:used]
+    ad = adapters(rows, cols, slots, R, tokens, {e: 1 + (R - 1 + 7 * i) % R for i, e in enumerate(held)}, seed=R + used)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(R * used)
+    x = torch.randn(tokens, cols, generator=g, device="cuda").to(BF16)
+    dy = torch.randn(tokens, rows, generator=g, device="cuda").to(BF16)
+    base, dbase = torch.randn(tokens, rows, generator=g, device="cuda"), torch.randn(tokens, cols, generator=g, device="cuda")
+    y, dx = torch.full((tokens + 1, rows), -7.0, device="cuda"), torch.full((tokens + 1, cols), -7.0, device="cuda")
+    names = torch.tensor(held + [-1], dtype=torch.int32, device="cuda")
+    for mixed in (True, False):
+        pick = torch.randint(0, len(names), (tokens,), generator=g, device="cuda")
+        ids = names[pick if mixed else pick.sort().values]
+        torch.cuda.synchronize()
+        ad.h.matmul_bf16(x.data_ptr(), tokens, cols, ids.data_ptr(), base.data_ptr(), rows, y.data_ptr(), rows)
+        ad.h.backward(x.data_ptr(), cols, dy.data_ptr(), rows, tokens, ids.data_ptr(), dbase.data_ptr(), cols, dx.data_ptr(), cols, 0, 0)
+        ctx.sync()
+        want, mag = ad.forward(x.double(), ids, base)
+        low = 2 * (4 + cols // 64 + 8 + 2)                  # as in test_batch and test_backward
+        chain = low + 2 * (3 * ((R + 15) // 16) + 3)
+        assert ((y[:tokens].double() - want).abs() <= chain * U32 * mag).all()
+        want, mag = dbase.double().clone(), dbase.double().abs()
+        for e, at in ad.of(ids):
+            de = dy[at].double()
+            want[at] += ad.s[e] * de @ ad.b[e] @ ad.a[e]
+            mag[at] += ad.s[e] * de.abs() @ ad.b[e].abs() @ ad.a[e].abs()
+        assert ((dx[:tokens].double() - want).abs() <= chain * U32 * mag).all()
+        bare = ids < 0
+        assert torch.equal(y[:tokens][bare], base[bare]) and torch.equal(dx[:tokens][bare], dbase[bare])
+        assert (y[tokens] == -7.0).all() and (dx[tokens] == -7.0).all()
+    where = {l.name for l in capture.launches(ctx, lambda: ad.h.matmul_bf16(x.data_ptr(), tokens, cols, ids.data_ptr(), base.data_ptr(), rows, y.data_ptr(), rows))}
+    assert where == {"qm_lora_lists", "qm_lora_shrink_r%d_m" % R, "qm_lora_expand_r%d_m" % R}
+
+
 def test_rows_far_apart(ctx, adapters):
     """Row pitches whose byte offsets pass 32 bits."""
     rows, cols, ld = 200, 64, 1 << 30
