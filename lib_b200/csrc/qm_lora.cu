@@ -442,9 +442,10 @@ extern "C" __global__ void __launch_bounds__(512) qm_lora_rows(const __grid_cons
 
 // ---- few bf16 tokens -----------------------------------------------------------------------------------------------------
 // Decode batches of up to QM_LORA_FEW tokens in one launch, without lists or a workspace. Up to 16 tokens of one adapter are
-// an item (a token without an adapter is one of its own). Every CTA finds the items from the ids; each gets a cluster of eight
-// CTAs, or as many as share the ones that run at once evenly, and the clusters behind the last item leave (which is not free:
-// 64 tokens on 32 adapters take 9 us with 64 clusters and 14 with 128). As in qm_lora_rows a CTA multiplies an eighth of the
+// an item, and so are up to 16 without an adapter where base has to be copied. So there are at most as many items as tokens,
+// and without ids, when all of them are alike, a sixteenth. Every CTA finds the items from the ids; each gets a cluster of
+// eight CTAs, or as many as share the ones that run at once evenly, and the clusters behind the last item leave (which is not
+// free: 64 tokens on 32 adapters take 9 us with 64 clusters and 14 with 128). As in qm_lora_rows a CTA multiplies an eighth of the
 // columns of x with A, the sums meet in distributed shared memory and the CTA goes on with its own columns of B; the products
 // are mma with fragments straight from memory (see expand), the columns of a warp's first piece of B and of base on their way
 // before the sums meet. All that counts is the number of dependent trips to memory. Against the three launches of larger
@@ -461,27 +462,29 @@ __device__ __forceinline__ void few(const QmLoraFewArgs &a) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
     float *part = reinterpret_cast<float *>(smem);                    // [8 warps][16][LD]; the first one the CTA's sum
     const uint32_t low = smem_u32(smem) + 8 * 16 * LD * 4;            // [16] rows of three parts
-    // behind them: [FEW] adapters, [FEW] tokens of the same adapter before, [FEW] the items' first tokens, [16] the item's
-    // tokens, [8] scratch; over the sums, which come later: [4][256] tokens of a slot in a warp, [256] which slots hold an
-    // adapter
+    // behind them: [FEW] adapters (`slots`: none), [FEW] tokens of the same adapter before, [FEW] the items' first tokens, [16]
+    // the item's tokens, [8] scratch; over the sums, which come later: [4][SLOTS] tokens of a slot in a warp, [256] which slots
+    // hold an adapter
+    constexpr int SLOTS = 260;   // 256, one for none, whole words
     int32_t *ids = reinterpret_cast<int32_t *>(smem + 8 * 16 * LD * 4 + 16 * UB), *earlier = ids + QM_LORA_FEW, *leaders = earlier + QM_LORA_FEW;
     int32_t *rows = leaders + QM_LORA_FEW, *found = rows + 16;
-    uint8_t *count = smem, *known = smem + 1024;
+    uint8_t *count = smem, *known = smem + 4 * SLOTS;
     const int me = (int)cluster_rank();
     int mine = tid < a.tokens ? (a.ids ? a.ids[tid] : 0) : -1;
     known[tid] = tid < a.slots && a.rank[tid] > 0;
-    reinterpret_cast<uint32_t *>(count)[tid] = 0;
+    for (int i = tid; i < SLOTS; i += 256) reinterpret_cast<uint32_t *>(count)[i] = 0;
     if (tid < 16) rows[tid] = -1;
     __syncthreads();
-    if (mine < 0 || mine >= a.slots || !known[mine]) mine = -1;
+    if (mine < 0 || mine >= a.slots || !known[mine]) mine = a.slots;
+    if (tid >= a.tokens) mine = -1;
     if (tid < QM_LORA_FEW) ids[tid] = mine;
     const uint32_t same = __match_any_sync(0xffffffffu, mine);
-    if (mine >= 0 && lane == __ffs(same) - 1) count[warp * 256 + mine] = (uint8_t)__popc(same);
+    if (mine >= 0 && lane == __ffs(same) - 1) count[warp * SLOTS + mine] = (uint8_t)__popc(same);
     __syncthreads();
     int before = __popc(same & ((1u << lane) - 1));   // tokens of the same adapter before this one
     if (mine >= 0)
-        for (int w = 0; w < warp; w++) before += count[w * 256 + mine];
-    const bool leads = tid < a.tokens && (mine < 0 || before % 16 == 0);
+        for (int w = 0; w < warp; w++) before += count[w * SLOTS + mine];
+    const bool leads = mine >= 0 && before % 16 == 0 && (mine < a.slots || a.base != a.y);
     const uint32_t vote = __ballot_sync(0xffffffffu, leads);
     if (lane == 0 && warp < 4) found[warp] = __popc(vote);
     if (tid < QM_LORA_FEW) earlier[tid] = before;
@@ -492,20 +495,29 @@ __device__ __forceinline__ void few(const QmLoraFewArgs &a) {
         leaders[number] = tid;
     }
     __syncthreads();
-    const int items = found[0] + found[1] + found[2] + found[3], parts = max(1, min(a.pieces, a.at_once / items));
+    const int items = found[0] + found[1] + found[2] + found[3], parts = max(1, min(a.pieces, a.at_once / max(1, items)));
     const int np_cta = (((a.np + parts * QM_LORA_CLUSTER - 1) / (parts * QM_LORA_CLUSTER)) + 7) & ~7;
     const int unit = blockIdx.x / QM_LORA_CLUSTER;
     if (unit >= items * parts) return;   // the whole cluster
     const int leader = leaders[unit / parts];
     const int slot = ids[leader];
     const int n0 = min((unit % parts * QM_LORA_CLUSTER + me) * np_cta, a.rows), nn = min(np_cta, a.rows - n0);
-    if (slot < 0) {
-        if (a.base != a.y)
-            for (int c = tid; c < nn; c += 256) a.y[leader * a.ldy + n0 + c] = a.base ? a.base[leader * a.ldb + n0 + c] : 0.f;
+    if (mine == slot && before >= earlier[leader] && before < earlier[leader] + 16) rows[before - earlier[leader]] = tid;
+    __syncthreads();
+    if (slot == a.slots) {   // no adapter: base rows, four at a time
+        for (int i = 0; i < 16 && rows[i] >= 0; i += 4) {
+            const int t[4] = {rows[i], rows[i + 1], rows[i + 2], rows[i + 3]};
+            for (int c = tid; c < nn; c += 256) {
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[k] = a.base && t[k] >= 0 ? a.base[t[k] * a.ldb + n0 + c] : 0.f;
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (t[k] >= 0) a.y[t[k] * a.ldy + n0 + c] = v[k];
+            }
+        }
         return;
     }
-    if (tid < a.tokens && mine == slot && before >= earlier[leader] && before < earlier[leader] + 16) rows[before - earlier[leader]] = tid;
-    __syncthreads();
     const int tok[2] = {rows[g], rows[g + 8]};   // the tokens of this lane's fragment rows, -1: none
     const int rank = a.rank[slot];
     const float scale = a.scale[slot];

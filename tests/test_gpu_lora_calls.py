@@ -1,0 +1,53 @@
+"""Calls of the adapters at the edges of what their documentation allows."""
+import pytest
+import torch
+
+from tests.test_gpu_lora import BF16, U32, adapters  # noqa: F401  (a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 9, 16, 17, 100, 128, 129])
+@pytest.mark.parametrize("rows", [40, 512, 4096, 28673])
+@pytest.mark.parametrize("how", ["apart", "in place", "none"])
+def test_empty_slot_without_ids(ctx, tokens, rows, how):
+    """No ids, slot 0 never filled: every row is its base row, or zeros."""
+    cols = 64
+    h = ctx.lora(rows, cols, 2, 16, tokens)
+    x = torch.full((tokens, cols), float("nan"), dtype=BF16, device="cuda")
+    base = torch.randn(tokens, rows, device="cuda")
+    y = torch.full((tokens + 1, rows + 3), -7.0, device="cuda")
+    if how == "in place":
+        y[:tokens, :rows] = base
+    bp, lb = {"apart": (base.data_ptr(), rows), "in place": (y.data_ptr(), rows + 3), "none": (0, 0)}[how]
+    torch.cuda.synchronize()
+    h.matmul_bf16(x.data_ptr(), tokens, cols, 0, bp, lb, y.data_ptr(), rows + 3)
+    ctx.sync()
+    assert torch.equal(y[:tokens, :rows], base if how != "none" else torch.zeros_like(base))
+    assert (y[:tokens, rows:] == -7.0).all() and (y[tokens] == -7.0).all()
+    h.close()
+
+
+# tokens of slot 1 (rank 5) among bare ones: none, one, a whole item, one item and a bit
+@pytest.mark.parametrize("tokens,held", [(1, 0), (33, 1), (128, 0), (128, 16), (128, 17), (128, 111), (100, 99)])
+@pytest.mark.parametrize("how", ["apart", "in place", "none"])
+def test_mostly_bare_tokens(ctx, adapters, tokens, held, how):  # noqa: F811
+    rows, cols = 6150, 96
+    ad = adapters(rows, cols, 3, 16, tokens, {1: 5}, seed=tokens + held)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(held)
+    ids = torch.tensor([-1, 0, 2, 3, 10 ** 9], dtype=torch.int32, device="cuda")[torch.randint(0, 5, (tokens,), generator=g, device="cuda")]
+    ids[torch.randperm(tokens, generator=g, device="cuda")[:held]] = 1
+    x = torch.randn(tokens, cols, generator=g, device="cuda").to(BF16)
+    x[ids != 1] = float("nan")
+    base = torch.randn(tokens, rows, generator=g, device="cuda")
+    start = base if how != "none" else torch.zeros_like(base)
+    y = base.clone() if how == "in place" else torch.full((tokens, rows), -7.0, device="cuda")
+    bp = {"apart": base.data_ptr(), "in place": y.data_ptr(), "none": 0}[how]
+    torch.cuda.synchronize()
+    ad.h.matmul_bf16(x.data_ptr(), tokens, cols, ids.data_ptr(), bp, rows, y.data_ptr(), rows)
+    ctx.sync()
+    want, mag = ad.forward(x.double(), ids, start)
+    # 4 per stage of 64 columns, two stages, 8 CTAs; 3 parts of 16 ranks, the base, the scale: truncated, a unit each
+    assert ((y.double() - want).abs() <= 2 * (4 + 2 + 8 + 3 + 4) * U32 * mag + 1e-30).all()
+    assert torch.equal(y[ids != 1], start[ids != 1])
