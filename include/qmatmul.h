@@ -201,7 +201,9 @@ QM_API int32_t qm_matmul_bf16(qm_ctx *ctx, qm_weight w, uint64_t a_dev, int32_t 
  * bf16. max_tokens (<= 2^20) bounds the tokens of one bf16 call and sizes the handle's workspace: qm_lora_matmul_bf16 of
  * more than 128 tokens and qm_lora_backward use it, and such calls (and graphs of them) that share a handle must be ordered,
  * on one stream or with events; the calls without it may overlap one another.
- * Capture into a graph is allowed; everything is asynchronous on the context's stream. Device pointers.
+ * Capture into a graph is allowed; everything is asynchronous on the context's stream. Device pointers. Only qm_lora_create
+ * waits for the stream, so that the handle is ready for any other, and is refused under capture
+ * (CUDA_ERROR_STREAM_CAPTURE_UNSUPPORTED).
  *
  * qm_lora_set: fills a slot from device memory, A [rank][cols] and B [rows][rank] row by row, `type` a GGUF tensor type
  *   (QM_TYPE_F32, QM_TYPE_F16, QM_TYPE_BF16; rounded to bf16). rank 0 empties the slot. Ordered with the products on the

@@ -328,6 +328,12 @@ extern "C" int32_t qm_sync(qm_ctx *c) {
     return QM_OK;
 }
 
+int32_t qm_refuse_capture(qm_ctx *c) {
+    CUstreamCaptureStatus status = CU_STREAM_CAPTURE_STATUS_NONE;
+    DRV(c->drv->cuStreamIsCapturing(c->stream, &status));
+    return status == CU_STREAM_CAPTURE_STATUS_NONE ? QM_OK : (int32_t)CUDA_ERROR_STREAM_CAPTURE_UNSUPPORTED;
+}
+
 extern "C" int32_t qm_last_status(qm_ctx *c, uint32_t *status) {
     CHECK_CTX(c);
     if (!status) return QM_ERR_ARG;

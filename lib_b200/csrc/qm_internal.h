@@ -117,6 +117,8 @@ struct CtxGuard {
 
 struct qm_stack;
 QmWeight *qm_weight_from_handle(qm_weight h);
+// CUDA_ERROR_STREAM_CAPTURE_UNSUPPORTED while the context's stream is being captured (the capture goes on).
+int32_t qm_refuse_capture(qm_ctx *c);
 int32_t qm_launch(qm_ctx *c, int kernel, unsigned gx, unsigned gy, unsigned block, unsigned smem, void *args,
                   bool pdl);
 int32_t qm_launch_ex(qm_ctx *c, int kernel, unsigned gx, unsigned block, unsigned smem, void *args, bool pdl,

@@ -80,6 +80,9 @@ extern "C" int32_t qm_lora_create(qm_ctx *c, int64_t rows, int64_t cols, int32_t
     if (rows < 1 || cols < 32 || cols % 32 != 0 || adapters < 1 || max_rank < 1 || max_tokens < 1) return QM_ERR_SHAPE;
     // (cols: eight staged rows of x and a chunk of B fit in the shared memory of qm_lora_rows)
     if (rows > (1 << 22) || cols > 32768 || adapters > 256 || max_rank > 128 || max_tokens > (1 << 20)) return QM_ERR_LIMIT;
+    CtxGuard g(c);
+    DRV(g.rc);
+    if (int32_t rc = qm_refuse_capture(c)) return rc;   // (the clear below would run again with the graph)
     qm_lora *l = new (std::nothrow) qm_lora();
     if (!l) return QM_ERR_NOMEM;
     l->magic = QM_LORA_MAGIC;
@@ -93,8 +96,7 @@ extern "C" int32_t qm_lora_create(qm_ctx *c, int64_t rows, int64_t cols, int32_t
     l->max_tokens = max_tokens;
     const int64_t pitch = QM_LORA_PITCH(l->rpad / 16);
     l->low_rows = ((int64_t)max_tokens + QM_LORA_TILE - 1) / QM_LORA_TILE * QM_LORA_TILE + (std::min(adapters, max_tokens) + 1) * (int64_t)QM_LORA_BLOCK;
-    CtxGuard g(c);
-    CUresult r = g.rc;
+    CUresult r = CUDA_SUCCESS;
     const int64_t low = l->low_rows * pitch * 2;
     struct {
         CUdeviceptr *p;
@@ -107,6 +109,7 @@ extern "C" int32_t qm_lora_create(qm_ctx *c, int64_t rows, int64_t cols, int32_t
     for (auto &n : need)
         if (r == CUDA_SUCCESS) r = c->drv->cuMemAlloc_v2(n.p, (size_t)n.bytes);
     if (r == CUDA_SUCCESS) r = c->drv->cuMemsetD8Async(l->rank, 0, (size_t)adapters * 4, c->stream);
+    if (r == CUDA_SUCCESS) r = c->drv->cuStreamSynchronize(c->stream);   // the next call may be on another stream
     if (r == CUDA_SUCCESS) r = c->drv->cuStreamCreate(&l->side, CU_STREAM_NON_BLOCKING);
     if (r == CUDA_SUCCESS) r = c->drv->cuEventCreate(&l->fork, CU_EVENT_DISABLE_TIMING);
     if (r == CUDA_SUCCESS) r = c->drv->cuEventCreate(&l->join, CU_EVENT_DISABLE_TIMING);
@@ -471,9 +474,7 @@ extern "C" int32_t qm_matmul_bf16_lora(qm_ctx *c, qm_weight h, qm_lora *l, uint6
 static int32_t align_dy(qm_ctx *c, qm_lora *l, uint64_t *dy, int64_t *lddy, int32_t tokens) {
     if (!(*dy & 15) && !(*lddy & 7)) return QM_OK;
     if (!l->aligned) {
-        CUstreamCaptureStatus capturing = CU_STREAM_CAPTURE_STATUS_NONE;
-        DRV(c->drv->cuStreamIsCapturing(c->stream, &capturing));
-        if (capturing != CU_STREAM_CAPTURE_STATUS_NONE) return CUDA_ERROR_STREAM_CAPTURE_UNSUPPORTED;
+        if (int32_t rc = qm_refuse_capture(c)) return rc;
         DRV(c->drv->cuMemAlloc_v2(&l->aligned, (size_t)l->max_tokens * l->np * 2));
     }
     QmLoraAlignArgs a;

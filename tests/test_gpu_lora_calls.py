@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+import lib_b200
+from tests import capture
 from tests.test_gpu_lora import BF16, U32, adapters  # noqa: F401  (a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -51,3 +53,44 @@ def test_mostly_bare_tokens(ctx, adapters, tokens, held, how):  # noqa: F811
     # 4 per stage of 64 columns, two stages, 8 CTAs; 3 parts of 16 ranks, the base, the scale: truncated, a unit each
     assert ((y.double() - want).abs() <= 2 * (4 + 2 + 8 + 3 + 4) * U32 * mag + 1e-30).all()
     assert torch.equal(y[ids != 1], start[ids != 1])
+
+
+def test_handle_made_on_a_busy_stream(ctx):
+    """A handle made while its context's stream has work queued is ready for any other stream."""
+    rows, cols, r = 96, 64, 8
+    a, b = torch.randn(r, cols, device="cuda").to(BF16), torch.randn(rows, r, device="cuda").to(BF16)
+    x, y = torch.randn(2, cols, device="cuda"), torch.zeros(2, rows, device="cuda")
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    try:
+        ctx.set_stream(first.cuda_stream)
+        with torch.cuda.stream(first):
+            torch.cuda._sleep(200_000_000)      # about a tenth of a second
+        h = ctx.lora(rows, cols, 1, r, 2)
+        ctx.set_stream(second.cuda_stream)
+        h.set(0, r, 1.0, a.data_ptr(), b.data_ptr())
+        ctx.sync()
+        first.synchronize()
+        h.matvec(x.data_ptr(), 2, cols, 0, 0, 0, y.data_ptr(), rows)
+        ctx.sync()
+    finally:
+        ctx.set_stream(0)
+    want, mag = x.double() @ a.double().t() @ b.double().t(), x.double().abs() @ a.double().abs().t() @ b.double().abs().t()
+    assert ((y.double() - want).abs() <= 60 * U32 * mag).all()
+    h.close()
+
+
+def test_handle_is_not_made_under_capture(ctx):
+    """The slots' first clear would run again with the graph: refused, and the capture goes on."""
+    codes, made = [], []
+
+    def call():
+        try:
+            made.append(ctx.lora(96, 64, 1, 8, 2))
+        except lib_b200.QmError as e:
+            codes.append(e.code)
+
+    capture.launches(ctx, call)     # (ends the capture: fails if it was invalidated)
+    for h in made:
+        h.close()
+    assert codes == [900]           # CUDA_ERROR_STREAM_CAPTURE_UNSUPPORTED
