@@ -248,7 +248,8 @@ QM_API int32_t qm_matmul_bf16_lora(qm_ctx *ctx, qm_weight w, qm_lora *lora, uint
  * the reference.
  * qm_rope_create: angle_i = position * theta^(-2i/rot_dim) / factors[i] (factors: rot_dim/2 positive floats on the host, or
  *   NULL: ones), taken modulo a turn in float64, so far positions keep their fraction. Pairs are (i, i + rot_dim/2), with
- *   QM_ROPE_INTERLEAVED (2i, 2i+1). head_dim even, <= 512; rot_dim even, 0..head_dim.
+ *   QM_ROPE_INTERLEAVED (2i, 2i+1). head_dim even, <= 512; rot_dim even, 0..head_dim. Waits for the stream, so that the
+ *   handle is ready for any other; refused under capture (CUDA_ERROR_STREAM_CAPTURE_UNSUPPORTED).
  * qm_qk_norm_rope: x float32 [tokens][ldx], q_heads query heads, then k_heads key heads, side by side (either may be 0; a v
  *   part behind them is not touched); gains float32 [head_dim] or 0 (ones); pos int32 [tokens], any value;
  *   q_out [tokens][ldq], k_out [tokens][ldk]: float32, or bf16 with QM_QK_BF16. QM_QK_NO_NORM: rotation only (gains and eps

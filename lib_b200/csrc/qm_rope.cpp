@@ -42,6 +42,9 @@ extern "C" int32_t qm_rope_create(qm_ctx *c, int32_t head_dim, int32_t rot_dim, 
         if (!isfinite(turns)) return QM_ERR_ARG;
         freq[i] = (uint64_t)ldexpl(turns - floorl(turns), 64);
     }
+    CtxGuard g(c);
+    DRV(g.rc);
+    if (int32_t rc = qm_refuse_capture(c)) return rc;   // (the copy below would run again with the graph, from this frame)
     qm_rope *r = new (std::nothrow) qm_rope();
     if (!r) return QM_ERR_NOMEM;
     r->magic = QM_ROPE_MAGIC;
@@ -50,11 +53,11 @@ extern "C" int32_t qm_rope_create(qm_ctx *c, int32_t head_dim, int32_t rot_dim, 
     r->rot = rot_dim;
     r->interleaved = (flags & QM_ROPE_INTERLEAVED) ? 1 : 0;
     r->grad_ctas = 3 * c->sm_count;   // the most that qm_qk_norm_rope_backward launches
-    CtxGuard g(c);
-    CUresult e = g.rc;
-    if (e == CUDA_SUCCESS) e = c->drv->cuMemAlloc_v2(&r->freq, freq.size() * sizeof(uint64_t));
+    CUresult e = c->drv->cuMemAlloc_v2(&r->freq, freq.size() * sizeof(uint64_t));
     if (e == CUDA_SUCCESS) e = c->drv->cuMemAlloc_v2(&r->partial, (size_t)r->grad_ctas * head_dim * sizeof(float));
-    if (e == CUDA_SUCCESS) e = c->drv->cuMemcpyHtoD_v2(r->freq, freq.data(), freq.size() * sizeof(uint64_t));
+    // (a copy on the default stream may return before it has arrived, and nothing orders the context's streams behind it)
+    if (e == CUDA_SUCCESS) e = c->drv->cuMemcpyHtoDAsync_v2(r->freq, freq.data(), freq.size() * sizeof(uint64_t), c->stream);
+    if (e == CUDA_SUCCESS) e = c->drv->cuStreamSynchronize(c->stream);
     if (e != CUDA_SUCCESS) {
         if (r->freq) c->drv->cuMemFree_v2(r->freq);
         if (r->partial) c->drv->cuMemFree_v2(r->partial);
