@@ -355,7 +355,9 @@ __device__ __forceinline__ void backward(const QmQkArgs &a) {
                     sum[2 + u] += p[u][i][v] * b.f[u][i][v] * l.w[i][v] + q[u][i][v] * b.g[u][i][v] * l.z[i][v];
                 }
             }
-        // dx = r dz gain - (r^3 mean(dz gain x)) x
+        // dx = r (dz gain - n (r mean(dz gain x))), n = r x: no factor is far from the values themselves, so heads of any
+        // magnitude keep their bits as long as their squares fit float32 (r^3, as one factor for x, would overflow below
+        // 1e-13 without eps and vanish above 1e13)
         float s = 0.f, r = 1.f;
         if (a.norm) {
             s = warp_sum4(sum) * a.inv_dim;
@@ -363,7 +365,7 @@ __device__ __forceinline__ void backward(const QmQkArgs &a) {
         }
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const float ru = __shfl_sync(0xffffffffu, r, 8 * u), mu = a.norm ? ru * ru * ru * __shfl_sync(0xffffffffu, s, 16 + 8 * u) : 0.f;
+            const float ru = __shfl_sync(0xffffffffu, r, 8 * u), mu = a.norm ? ru * __shfl_sync(0xffffffffu, s, 16 + 8 * u) : 0.f;
             if (h0 + u >= t.last) break;
 #pragma unroll
             for (int i = 0; i < NP; i++) {
@@ -371,11 +373,11 @@ __device__ __forceinline__ void backward(const QmQkArgs &a) {
                 float o[V], e[V];
 #pragma unroll
                 for (int v = 0; v < V; v++) {
-                    const float x = b.f[u][i][v], y = b.g[u][i][v], c = p[u][i][v], d = q[u][i][v];
-                    df[i][v] += c * x * ru;
-                    dg[i][v] += d * y * ru;
-                    o[v] = ru * (c * l.w[i][v]) - mu * x;
-                    e[v] = ru * (d * l.z[i][v]) - mu * y;
+                    const float x = ru * b.f[u][i][v], y = ru * b.g[u][i][v], c = p[u][i][v], d = q[u][i][v];
+                    df[i][v] += c * x;
+                    dg[i][v] += d * y;
+                    o[v] = ru * (c * l.w[i][v] - x * mu);
+                    e[v] = ru * (d * l.z[i][v] - y * mu);
                 }
                 regroup<V>(o, e, adjacent);
                 store_any<V, false>(drow, u * a.dim + l.at[i].at, o);

@@ -5,9 +5,44 @@ import torch
 import lib_b200
 from lib_b200 import _capi
 from tests import capture
-from tests.test_gpu_rope import U32, turned, turns
+from tests.test_gpu_rope import BF16, U32, turned, turns
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("scale", [1e-17, 1e-14, 1e-6, 1.0, 1e14, 1e17])
+@pytest.mark.parametrize("dim", [128, 130, 256, 512])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_gradient_of_heads_of_any_magnitude(ctx, scale, dim, bf16):
+    """As far as the squares fit float32 (eps 0): dx = r (dz g - n mean(dz g n)) holds its bits."""
+    tokens, hq, hk, rot = 21, 3, 2, dim // 2 // 2 * 2
+    g = torch.Generator(device="cuda")
+    g.manual_seed(dim)
+    x = torch.randn(tokens, (hq + hk) * dim, generator=g, device="cuda") * scale
+    gq, gk = (torch.rand(dim, generator=g, device="cuda") + 0.5 for _ in range(2))
+    pos = torch.randint(0, 10 ** 6, (tokens,), generator=g, device="cuda", dtype=torch.int32)
+    dq, dk = (torch.randn(tokens, h * dim, generator=g, device="cuda").to(BF16 if bf16 else torch.float32) for h in (hq, hk))
+    dx, dgq, dgk = torch.empty_like(x), torch.empty(dim, device="cuda"), torch.empty(dim, device="cuda")
+    rope = ctx.rope(dim, rot, 10000.0)
+    torch.cuda.synchronize()
+    rope.qk_norm_backward(x.data_ptr(), x.shape[1], tokens, hq, hk, gq.data_ptr(), gk.data_ptr(), 0.0, pos.data_ptr(), dq.data_ptr(), hq * dim,
+                          dk.data_ptr(), hk * dim, dx.data_ptr(), x.shape[1], dgq.data_ptr(), dgk.data_ptr(), _capi.QK_BF16 if bf16 else 0)
+    ctx.sync()
+    ang = turns(pos, rot, 10000.0, None)
+    at = 0
+    for h, gain, dy, dgain in ((hq, gq, dq, dgq), (hk, gk, dk, dgk)):
+        z, got = (t[:, at * dim:(at + h) * dim].reshape(tokens, h, dim).double() for t in (x, dx))
+        at += h
+        dz = turned(dy.double().reshape(tokens, h, dim), -ang, rot, False)
+        r = 1 / z.square().mean(-1, keepdim=True).sqrt()
+        n, dn = z * r, dz * gain.double()
+        want = r * (dn - n * (dn * n).mean(-1, keepdim=True))
+        # the turn, the factors and the sums of a head: as for ordinary heads
+        top = dn.abs().amax(-1, keepdim=True) * (1 + n.abs() * n.abs().mean(-1, keepdim=True))
+        assert ((got - want).abs() <= (32 + dim // 32) * U32 * r * top).all(), ((got - want).abs() / (U32 * r * top)).max()
+        mag = (dz.abs().amax(-1, keepdim=True) * n.abs()).sum((0, 1))
+        assert ((dgain.double() - (dz * n).sum((0, 1))).abs() <= (48 + tokens * (hq + hk) / 64) * U32 * mag).all()
+    rope.close()
 
 
 def test_handle_is_not_made_under_capture(ctx):
