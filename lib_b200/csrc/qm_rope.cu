@@ -16,9 +16,10 @@
 //
 // The angle of a far position has lost its fraction in 32 bits (position 10^6 is 0.06 off), so the turns (angle / 2 pi) are
 // a product in 64-bit fixed point, position times the fraction of a turn in units of 2^-64, whose overflow is the whole turns:
-// what is left, in a few integer instructions, is off by at most 2^-31 of a turn at every position, before it is rounded to
-// float32 as any fraction would be. (The same in float64 kept the FP64 pipe busy: 52 -> 45 us at the size below, with a grid
-// that needs no division to find its heads.)
+// what is left, in a few integer instructions, is off by at most 2^-64 of a turn for each position, before it is rounded to
+// float32, whose relative error is what the sine of a slow pair's small angle takes over. (Only its upper 32 bits: off by
+// 1.5e-4 of itself at position 1 in the last of 64 pairs of theta 500000. The same in float64 kept the FP64 pipe busy:
+// 52 -> 45 us at the size below, with a grid that needs no division to find its heads.)
 //
 // One B200, 40 heads of 128, half-split: 8192 tokens to bf16 44.7 us (5.6 TB/s, 0.86 of the measured copy rate; the first form
 // with one reduction per head and gains read for every head 64 us, bound by instruction issue); 4096 tokens backward 49.6 us
@@ -142,8 +143,8 @@ struct Lane {
                 cs[i][v] = 1.f;
                 sn[i][v] = 0.f;
                 if (pair < a.rot / 2) {
-                    const int turns = (int)(uint32_t)((pos * a.freq[pair]) >> 32);   // of 2^-32 turns, between minus and plus a half
-                    sincospif((float)turns * 0x1p-31f, &sn[i][v], &cs[i][v]);
+                    const int64_t turns = (int64_t)(pos * a.freq[pair]);   // of 2^-64 turns, between minus and plus a half
+                    sincospif((float)turns * 0x1p-63f, &sn[i][v], &cs[i][v]);
                 }
             }
     }

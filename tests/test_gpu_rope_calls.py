@@ -45,6 +45,33 @@ def test_gradient_of_heads_of_any_magnitude(ctx, scale, dim, bf16):
     rope.close()
 
 
+@pytest.mark.parametrize("dim,interleaved", [(128, False), (128, True), (130, False)])
+def test_slow_pairs_at_small_positions(ctx, dim, interleaved):
+    """The sine of a slow pair's small angle keeps all its bits: (1, 0) turned, and turned back."""
+    theta, half = 500000.0, dim // 2
+    pos = torch.tensor([1, 2, 3, -1, 7, 100, -5], dtype=torch.int32, device="cuda")
+    t = pos.numel()
+    one = torch.zeros(t, dim, device="cuda")
+    one[:, 0:dim:2 if interleaved else 1][:, :half] = 1.0
+    q, dx = torch.empty(t, dim, device="cuda"), torch.empty(t, dim, device="cuda")
+    rope = ctx.rope(dim, dim, theta, interleaved=interleaved)
+    torch.cuda.synchronize()
+    common = (one.data_ptr(), dim, t, 1, 0, 0, 0, 0.0, pos.data_ptr())
+    rope.qk_norm(*common, q.data_ptr(), dim, 0, 0, _capi.QK_NO_NORM)
+    rope.qk_norm_backward(*common, one.data_ptr(), dim, 0, 0, dx.data_ptr(), dim, 0, 0, _capi.QK_NO_NORM)
+    ctx.sync()
+    ang = turns(pos, dim, theta, None)[:, 0]
+    small = ang.abs() < 1.5     # (beyond, a rounding of the angle weighs more than the sine's own)
+    assert small[:, half - 1].all()
+    for got, sign in ((q, 1.0), (dx, -1.0)):
+        sine = (got[:, 1::2] if interleaved else got[:, half:]).double()
+        want = sign * ang.sin()
+        # the angle's rounding to float32 (its weight in the sine is at most one here), a unit of sincospif, and 2^-64 turns
+        # per position of the frequency, 2^-41 of the slowest pair's
+        assert ((sine - want).abs() <= 4 * U32 * want.abs())[small].all(), ((sine - want).abs() / want.abs())[small].max()
+    rope.close()
+
+
 def test_handle_is_not_made_under_capture(ctx):
     codes, made = [], []
 
