@@ -197,8 +197,8 @@ QM_API int32_t qm_matmul_bf16(qm_ctx *ctx, qm_weight w, uint64_t a_dev, int32_t 
  * (cols a multiple of 32, <= 32768; rows <= 2^22); a batch names for each token the adapter of its request:
  *   y[t] = base[t] + scale_a * B_a (A_a f(x[t])),   a = ids[t] (int32, on the device; ids_dev = 0: slot 0 for all).
  * A token whose id is outside [0, adapters) or names an empty slot keeps base[t]. base_dev = 0 stands for zeros; it may be
- * y_dev itself with ldb = ldy, any other overlap of y with an input is refused. All sums are float32; adapters are held in
- * bf16. max_tokens (<= 2^20) bounds the tokens of one bf16 call and sizes the handle's workspace: qm_lora_matmul_bf16 of
+ * y_dev itself with ldb = ldy, any other overlap of y with an input is refused. ldb does not count without a base, nor base
+ * without dx. All sums are float32; adapters are held in bf16. max_tokens (<= 2^20) bounds the tokens of one bf16 call and sizes the handle's workspace: qm_lora_matmul_bf16 of
  * more than 128 tokens and qm_lora_backward use it, and such calls (and graphs of them) that share a handle must be ordered,
  * on one stream or with events; the calls without it may overlap one another.
  * Capture into a graph is allowed; everything is asynchronous on the context's stream. Device pointers. Only qm_lora_create

@@ -237,6 +237,7 @@ extern "C" int32_t qm_lora_matvec(qm_ctx *c, qm_lora *l, uint64_t x_dev, uint64_
                                   uint64_t base_dev, int64_t ldb, uint64_t y_dev, int64_t ldy, uint32_t flags) {
     CHECK_CTX(c);
     int32_t rc = lora_check(c, l);
+    if (!base_dev) ldb = 0;   // (the pitch of nothing: neither refused nor a reason for another kernel)
     if (!rc) rc = rows_check(l, x_dev, x2_dev, m, ldx, ids_dev, base_dev, ldb, y_dev, ldy, flags);
     if (rc) return rc;
     CtxGuard g(c);
@@ -449,6 +450,7 @@ extern "C" int32_t qm_lora_matmul_bf16(qm_ctx *c, qm_lora *l, uint64_t x_bf16_de
                                        uint64_t base_dev, int64_t ldb, uint64_t y_dev, int64_t ldy) {
     CHECK_CTX(c);
     int32_t rc = lora_check(c, l);
+    if (!base_dev) ldb = 0;
     if (!rc) rc = batch_check(l, x_bf16_dev, ldx, tokens, ids_dev, base_dev, ldb, y_dev, ldy, l->cols, l->rows);
     if (rc || tokens == 0) return rc;
     CtxGuard g(c);
@@ -498,6 +500,8 @@ extern "C" int32_t qm_lora_backward(qm_ctx *c, qm_lora *l, uint64_t x_bf16_dev, 
     int32_t rc = lora_check(c, l);
     if (rc) return rc;
     if (!dx_dev && !da_dev && !db_dev) return QM_ERR_ARG;
+    if (!dx_dev) base_dev = 0, lddx = 0;
+    if (!base_dev) ldb = 0;
     if (tokens < 0 || ldx < l->cols || lddy < l->rows || ldx > (1 << 30) || lddy > (1 << 30)) return QM_ERR_SHAPE;
     if (tokens > l->max_tokens) return QM_ERR_LIMIT;
     if (tokens && (!x_bf16_dev || !dy_bf16_dev)) return QM_ERR_ARG;

@@ -94,3 +94,27 @@ def test_handle_is_not_made_under_capture(ctx):
     for h in made:
         h.close()
     assert codes == [900]           # CUDA_ERROR_STREAM_CAPTURE_UNSUPPORTED
+
+
+@pytest.mark.parametrize("tokens", [3, 100, 300])
+def test_pitch_of_an_absent_base(ctx, adapters, tokens):  # noqa: F811
+    """Without a base its pitch means nothing: no other kernel, no refusal."""
+    rows, cols = 256, 128
+    ad = adapters(rows, cols, 1, 16, 300, {0: 16})
+    x, y = torch.randn(tokens, cols, device="cuda").to(BF16), torch.zeros(tokens, rows, device="cuda")
+    torch.cuda.synchronize()
+    call = lambda ldb: ad.h.matmul_bf16(x.data_ptr(), tokens, cols, 0, 0, ldb, y.data_ptr(), rows)  # noqa: E731
+    names = [[l.name for l in capture.launches(ctx, lambda: call(ldb))] for ldb in (0, 1, rows + 1, 1 << 40, -1)]
+    assert names.count(names[0]) == len(names)
+    if tokens <= 8:
+        xf = x.float()
+        torch.cuda.synchronize()
+        for ldb in (0, 1, 1 << 40):
+            ad.h.matvec(xf.data_ptr(), tokens, cols, 0, 0, ldb, y.data_ptr(), rows)
+    # the backward pass without dx: base and its pitch are not used
+    dy = torch.randn(tokens, rows, device="cuda").to(BF16)
+    da, db = torch.zeros(16, cols, device="cuda"), torch.zeros(rows, 16, device="cuda")
+    torch.cuda.synchronize()
+    ad.h.backward(x.data_ptr(), cols, dy.data_ptr(), rows, tokens, 0, da.data_ptr(), 1 << 40, 0, 1 << 62, da.data_ptr(), db.data_ptr())
+    ad.h.backward(x.data_ptr(), cols, dy.data_ptr(), rows, tokens, 0, 0, 1 << 40, y.data_ptr(), cols, da.data_ptr(), db.data_ptr())
+    ctx.sync()
