@@ -95,6 +95,13 @@ static bool on_small(const Span &out, uint64_t pos, int64_t tokens, uint64_t gq,
            (gk && overlap(out, span_of(gk, 1, 0, dim * 4)));
 }
 
+// Without the norm gains and eps do not count, whatever they are.
+static void drop_unused(uint64_t *gq, uint64_t *gk, float *eps, uint32_t flags) {
+    if (!(flags & QM_QK_NO_NORM)) return;
+    *gq = *gk = 0;
+    *eps = 0.f;
+}
+
 // What both directions ask of their arguments. `out`: dx of the backward pass (0 forward); q and k are results or their
 // gradients. Results may lie on the raw heads they come from, place for place; any other overlap of a result is refused.
 static int32_t check(qm_ctx *c, const qm_rope *r, uint64_t x, int64_t ldx, int32_t tokens, int32_t hq, int32_t hk, uint64_t gq,
@@ -162,6 +169,7 @@ extern "C" int32_t qm_qk_norm_rope(qm_ctx *c, qm_rope *r, uint64_t x_dev, int64_
                                    int32_t k_heads, uint64_t q_gain_dev, uint64_t k_gain_dev, float eps, uint64_t pos_dev,
                                    uint64_t q_out, int64_t ldq, uint64_t k_out, int64_t ldk, uint32_t flags) {
     CHECK_CTX(c);
+    drop_unused(&q_gain_dev, &k_gain_dev, &eps, flags);
     int32_t rc = check(c, r, x_dev, ldx, tokens, q_heads, k_heads, q_gain_dev, k_gain_dev, eps, pos_dev, q_out, ldq, k_out, ldk, flags);
     if (rc || tokens == 0) return rc;
     QmQkArgs a;
@@ -196,6 +204,7 @@ extern "C" int32_t qm_qk_norm_rope_backward(qm_ctx *c, qm_rope *r, uint64_t x_de
                                             uint64_t dx_dev, int64_t lddx, uint64_t dq_gain_dev, uint64_t dk_gain_dev,
                                             uint32_t flags) {
     CHECK_CTX(c);
+    drop_unused(&q_gain_dev, &k_gain_dev, &eps, flags);
     int32_t rc = check(c, r, x_dev, ldx, tokens, q_heads, k_heads, q_gain_dev, k_gain_dev, eps, pos_dev, dq_dev, lddq, dk_dev, lddk, flags);
     if (rc) return rc;
     const int64_t dim = r->dim, heads = (int64_t)q_heads + k_heads;

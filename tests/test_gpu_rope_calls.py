@@ -107,3 +107,36 @@ def test_handles_are_ready_at_once(ctx):
             rope.close()
     finally:
         ctx.set_stream(0)
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_rotation_alone_ignores_gains_and_eps(ctx, backward):
+    tokens, dim = 9, 64
+    rope = ctx.rope(dim, dim, 10000.0)
+    x, d = torch.randn(tokens, 2 * dim, device="cuda"), torch.randn(tokens, 2 * dim, device="cuda")
+    pos = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    gain = torch.full((dim + 1,), float("nan"), device="cuda")
+    results, names = [], []
+    for gq, gk, eps in ((0, 0, 0.0), (gain.data_ptr(), gain.data_ptr() + 4, 1e-5), (gain.data_ptr() + 1, 3, float("nan")), (0, 0, -1.0), (0, 0, float("inf"))):
+        out = torch.zeros(tokens, 2 * dim, device="cuda")
+        torch.cuda.synchronize()
+        common = (x.data_ptr(), 2 * dim, tokens, 1, 1, gq, gk, eps, pos.data_ptr())
+        if backward:
+            call = lambda: rope.qk_norm_backward(*common, d.data_ptr(), 2 * dim, d.data_ptr() + 4 * dim, 2 * dim, out.data_ptr(), 2 * dim,  # noqa: E731
+                                                 0, 0, _capi.QK_NO_NORM)
+        else:
+            call = lambda: rope.qk_norm(*common, out.data_ptr(), 2 * dim, out.data_ptr() + 4 * dim, 2 * dim, _capi.QK_NO_NORM)  # noqa: E731
+        call()
+        ctx.sync()
+        results.append(out)
+        names.append([l.name for l in capture.launches(ctx, call)])
+    assert all(torch.equal(results[0], r) for r in results) and names.count(names[0]) == len(names)
+    # a result on what is ignored is an ordinary result
+    out = torch.zeros(tokens, 2 * dim, device="cuda")
+    torch.cuda.synchronize()
+    if not backward:
+        rope.qk_norm(x.data_ptr(), 2 * dim, tokens, 1, 1, out.data_ptr(), 0, 0.0, pos.data_ptr(), out.data_ptr(), 2 * dim, out.data_ptr() + 4 * dim,
+                     2 * dim, _capi.QK_NO_NORM)
+        ctx.sync()
+        assert torch.equal(out, results[0])
+    rope.close()
