@@ -198,9 +198,10 @@ QM_API int32_t qm_matmul_bf16(qm_ctx *ctx, qm_weight w, uint64_t a_dev, int32_t 
  *   y[t] = base[t] + scale_a * B_a (A_a f(x[t])),   a = ids[t] (int32, on the device; ids_dev = 0: slot 0 for all).
  * A token whose id is outside [0, adapters) or names an empty slot keeps base[t]. base_dev = 0 stands for zeros; it may be
  * y_dev itself with ldb = ldy, any other overlap of y with an input is refused. ldb does not count without a base, nor base
- * without dx. All sums are float32; adapters are held in bf16. max_tokens (<= 2^20) bounds the tokens of one bf16 call and sizes the handle's workspace: qm_lora_matmul_bf16 of
- * more than 128 tokens and qm_lora_backward use it, and such calls (and graphs of them) that share a handle must be ordered,
- * on one stream or with events; the calls without it may overlap one another.
+ * without dx. All sums are float32; adapters are held in bf16. max_tokens (<= 2^20) bounds the tokens of one bf16 call and
+ * sizes the handle's workspace: qm_lora_matmul_bf16 of more than 128 tokens and qm_lora_backward use it, and such calls (and
+ * graphs of them) that share a handle must be ordered, on one stream or with events; the calls without it may overlap one
+ * another.
  * Capture into a graph is allowed; everything is asynchronous on the context's stream. Device pointers. Only qm_lora_create
  * waits for the stream, so that the handle is ready for any other, and is refused under capture
  * (CUDA_ERROR_STREAM_CAPTURE_UNSUPPORTED).
@@ -259,7 +260,7 @@ QM_API int32_t qm_matmul_bf16_lora(qm_ctx *ctx, qm_weight w, qm_lora *lora, uint
  *   forward call. dx float32 [tokens][lddx] (the q and k parts; may lie on x, or on float32 dq and dk, place for place),
  *   dq_gain, dk_gain float32 [head_dim] or 0: summed over tokens and heads in a fixed order. Calls with gain gradients, and
  *   graphs of them, that share a handle must be ordered.
- * Asynchronous on the context's stream; zero tokens are allowed. */
+ * Asynchronous on the context's stream; up to 2^30 tokens, none among them. */
 #define QM_ROPE_INTERLEAVED 1u
 #define QM_QK_NO_NORM 1u
 #define QM_QK_BF16 2u

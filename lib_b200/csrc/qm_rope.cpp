@@ -109,6 +109,8 @@ static int32_t check(qm_ctx *c, const qm_rope *r, uint64_t x, int64_t ldx, int32
     if (!r || r->magic != QM_ROPE_MAGIC || r->ctx != c) return QM_ERR_ARG;
     if (flags & ~(QM_QK_NO_NORM | QM_QK_BF16)) return QM_ERR_ARG;
     if (tokens < 0 || hq < 0 || hk < 0 || (int64_t)hq + hk < 1 || (int64_t)hq + hk > (1 << 20)) return QM_ERR_SHAPE;
+    // (the backward pass steps a token number past the last one, and spans of rows are counted in 64-bit bytes)
+    if (tokens > (1 << 30)) return QM_ERR_LIMIT;
     const int64_t dim = r->dim;
     if (ldx < (hq + (int64_t)hk) * dim || ldq < hq * dim || ldk < hk * dim) return QM_ERR_SHAPE;
     if (ldx > (1 << 30) || ldq > (1 << 30) || ldk > (1 << 30)) return QM_ERR_SHAPE;
