@@ -857,9 +857,11 @@ __device__ __forceinline__ void tma_rows4(uint32_t dst, const CUtensorMap *map, 
 // two).
 constexpr int PERIOD = 4;
 
-// A CTA's barriers, behind its stages: full and empty per stage and per accumulator; the accumulators' address.
+// A CTA's barriers, behind its stages: full and empty per stage and per accumulator; the accumulators' address; whether a wait
+// was given up.
 struct Pipe {
     uint32_t full, empty, acc_full, acc_empty, tmem;
+    volatile uint32_t *failed;
 };
 // Everything that needs no input: barriers, and tensor memory. The next kernel may start only after the tensor memory of all
 // CTAs is in their hands, so that none of its CTAs can hold what one of these still asks for.
@@ -870,11 +872,14 @@ __device__ __forceinline__ Pipe pipe_open(unsigned char *bars, uint32_t cols, in
     p.empty = p.full + 8 * STAGES;
     p.acc_full = p.empty + 8 * STAGES;
     p.acc_empty = p.acc_full + 16;
+    p.failed = reinterpret_cast<volatile uint32_t *>(bars + 8 * (2 * STAGES + 4) + 4);
     if (threadIdx.x == 0) {
+        *p.failed = 0;
         for (int s = 0; s < 2 * STAGES + 2; s++) qm::mbar_init(p.full + 8 * s, 1);
         for (int s = 0; s < 2; s++) qm::mbar_init(p.acc_empty + 8 * s, readers);
         qm::fence_barrier_init();
     }
+    __syncwarp();   // the lanes of a warp are together for what is .sync.aligned
     if (threadIdx.x < 32) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(p.acc_empty + 16), "r"(cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -889,6 +894,7 @@ __device__ __forceinline__ Pipe pipe_open(unsigned char *bars, uint32_t cols, in
 __device__ __forceinline__ void pipe_close(const Pipe &p, uint32_t cols) {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    __syncwarp();
     if (threadIdx.x < 32) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(p.tmem), "r"(cols) : "memory");
@@ -896,6 +902,24 @@ __device__ __forceinline__ void pipe_close(const Pipe &p, uint32_t cols) {
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// A wait of a whole warp. Lanes leave a bounded wait at different polls, and at its end may even get different answers: they
+// take one together, so that none waits at a barrier of the warp for lanes that have given up, and are together for the
+// .sync.aligned instructions that follow.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, qm::mbar_wait_bounded(bar, parity)); }
+// A wait that has run out.
+__device__ __forceinline__ void give_up(const Pipe &p, unsigned int *status) {
+    atomicOr(status, QM_STATUS_TIMEOUT);
+    *p.failed = 1;
+}
+// All warps are through with the stages; where a wait was given up, copies and products that are still in flight get two
+// milliseconds to land before the memory they write is used for something else and given back.
+__device__ __forceinline__ void pipe_done(const Pipe &p) {
+    __syncthreads();
+    if (*p.failed) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 4000000ll) {}
+    }
 }
 // Where a CTA that takes one piece of work after another is: stages and periods before this piece, and whether every wait has
 // ended so far (after one that has not, its warp does no more).
@@ -917,7 +941,7 @@ __device__ __forceinline__ void pipe_multiply(const Pipe &p, Progress &g, uint32
         if (c % PERIOD == 0 && period >= NACC) g.ok = qm::mbar_wait_bounded(p.acc_empty + 8 * acc, (uint32_t)(period / NACC - 1) & 1u);
         g.ok = g.ok && qm::mbar_wait_bounded(p.full + 8 * st, (uint32_t)(n / STAGES) & 1u);
         if (!g.ok) {
-            atomicOr(status, QM_STATUS_TIMEOUT);
+            give_up(p, status);
             return;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -934,10 +958,9 @@ __device__ __forceinline__ void pipe_read(const Pipe &p, Progress &g, uint32_t a
     for (int i = 0; i < N; i++) v[i] = 0.f;
     for (int i = 0; i * PERIOD < cn && g.ok; i++) {
         const int period = g.periods + i, acc = period % NACC;
-        // (one answer for the warp, whose lanes are together for what follows)
-        g.ok = __all_sync(0xffffffffu, qm::mbar_wait_bounded(p.acc_full + 8 * acc, (uint32_t)(period / NACC) & 1u));
+        g.ok = warp_wait(p.acc_full + 8 * acc, (uint32_t)(period / NACC) & 1u);
         if (!g.ok) {
-            if (lane == 0) atomicOr(status, QM_STATUS_TIMEOUT);
+            if (lane == 0) give_up(p, status);
             return;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -1008,9 +1031,9 @@ __device__ __forceinline__ void shrink(const QmLoraTcArgs &ta) {
             const uint32_t bytes = __reduce_add_sync(0xffffffffu, one ? (box ? 4096u : 512u) : 0u) + R * 128;
             for (int c = 0; c < cn && at_now.ok; c++) {
                 const int n = at_now.stages + c, st = n % STAGES;
-                at_now.ok = n < STAGES || qm::mbar_wait_bounded(pipe.empty + 8 * st, (uint32_t)(n / STAGES - 1) & 1u);
+                at_now.ok = n < STAGES || warp_wait(pipe.empty + 8 * st, (uint32_t)(n / STAGES - 1) & 1u);
                 if (!at_now.ok) {
-                    if (lane == 0) atomicOr(a.status, QM_STATUS_TIMEOUT);
+                    if (lane == 0) give_up(pipe, a.status);
                     break;
                 }
                 const uint32_t at = base + st * STAGE, bar = pipe.full + 8 * st;
@@ -1036,7 +1059,7 @@ __device__ __forceinline__ void shrink(const QmLoraTcArgs &ta) {
         } else {
             pipe_read<R, 2>(pipe, at_now, R, 0, cn, a.status, v);
         }
-        __syncthreads();   // nothing uses the stages any more
+        pipe_done(pipe);
         if (warp < 4) {
 #pragma unroll
             for (int i = 0; i < R; i += 4)
@@ -1301,8 +1324,8 @@ __device__ __forceinline__ void outer(const QmLoraTcArgs &ta) {
                     const int c = c4 + u, st = c % STAGES;
                     if (c >= cn || !ok) break;
                     const bool box = neighbours(rows[u], 4);
-                    if (c >= STAGES && !qm::mbar_wait_bounded(pipe.empty + 8 * st, (uint32_t)(c / STAGES - 1) & 1u)) {
-                        if (lane == 0) atomicOr(a.status, QM_STATUS_TIMEOUT);
+                    if (c >= STAGES && !warp_wait(pipe.empty + 8 * st, (uint32_t)(c / STAGES - 1) & 1u)) {
+                        if (lane == 0) give_up(pipe, a.status);
                         ok = false;
                         break;
                     }
@@ -1338,10 +1361,11 @@ __device__ __forceinline__ void outer(const QmLoraTcArgs &ta) {
         } else {
             pipe_read<MINE, NACC>(pipe, at_now, MM * BN, (warp >> 2) * MINE, cn, a.status, v);
         }
+        pipe_done(pipe);
         // row m of the accumulators is rank m % R of part m / R: the smallest part first, the others onto it
 #pragma unroll
         for (int p = 2; p >= 0; p--) {
-            __syncthreads();   // before the first: nothing uses the stages any more
+            if (p < 2) __syncthreads();
             if (warp < READERS) {
                 const int c = (warp >> 2) * MINE, m = c / BN, j = c % BN;   // this warp's columns lie in one product
                 const int at = m * 128 + (warp & 3) * 32 + lane - p * R;    // this lane's rank, if it holds one of this part
