@@ -94,13 +94,20 @@ __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w <<
 __device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 __device__ __forceinline__ uint32_t bf_bits(float v) { return (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v)); }
 
-// v as a sum of three bf16: the next 8 bits of what the ones before leave. An infinity stays in the first.
+// v as a sum of three bf16: the next 8 bits of what the ones before leave, cut off and not rounded, so that all parts have v's
+// sign and none is beyond its range. Beside an infinite factor each of them has to give that infinity: an infinite v is
+// infinite in all parts, and a part without bits is the smallest number there is (2^-133; not beside values below 2^-80, of
+// which that would be a share that counts).
 __device__ __forceinline__ void split3(float v, uint32_t (&p)[3]) {
-    p[0] = bf_bits(v);
-    const float h = __uint_as_float(p[0] << 16);
-    const float rest = isfinite(h) ? v - h : 0.f;
-    p[1] = bf_bits(rest);
-    p[2] = bf_bits(rest - __uint_as_float(p[1] << 16));
+    p[0] = __float_as_uint(v) >> 16;
+    float rest = v - __uint_as_float(p[0] << 16);
+    p[1] = __float_as_uint(rest) >> 16;
+    rest -= __uint_as_float(p[1] << 16);
+    p[2] = __float_as_uint(rest) >> 16;
+    const uint32_t least = fabsf(v) >= 0x1p-80f ? (p[0] & 0x8000u) | 1u : 0u;
+    if (p[1] == 0) p[1] = least;
+    if (p[2] == 0) p[2] = least;
+    if (!isfinite(v)) p[0] = p[1] = p[2] = bf_bits(v);
 }
 
 struct Tile {

@@ -3,10 +3,16 @@ import pytest
 import torch
 
 import lib_b200
+from lib_b200 import _capi
 from tests import capture
 from tests.test_gpu_lora import BF16, U32, adapters  # noqa: F401  (a fixture)
 
 pytestmark = pytest.mark.gpu
+
+
+def same_specials(got, want):
+    """The same infinities and NaN, place for place."""
+    return torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf()) and torch.equal(got[got.isinf()] > 0, want[want.isinf()] > 0)
 
 
 @pytest.mark.parametrize("tokens", [1, 2, 9, 16, 17, 100, 128, 129])
@@ -118,3 +124,77 @@ def test_pitch_of_an_absent_base(ctx, adapters, tokens):  # noqa: F811
     ad.h.backward(x.data_ptr(), cols, dy.data_ptr(), rows, tokens, 0, da.data_ptr(), 1 << 40, 0, 1 << 62, da.data_ptr(), db.data_ptr())
     ad.h.backward(x.data_ptr(), cols, dy.data_ptr(), rows, tokens, 0, 0, 1 << 40, y.data_ptr(), cols, da.data_ptr(), db.data_ptr())
     ctx.sync()
+
+
+@pytest.mark.parametrize("tokens", [40, 300])
+@pytest.mark.parametrize("rank", [1, 5, 24, 40, 70])
+@pytest.mark.parametrize("where", ["x", "dy", "A", "B", "x and dy"])
+def test_infinities_are_those_of_the_formulas(ctx, adapters, tokens, rank, where):  # noqa: F811
+    """An infinite element gives the infinities (and the NaN of unlike ones) that the formulas give, in every form."""
+    rows, cols = 136, 96
+    ad = adapters(rows, cols, 2, rank, tokens, {0: rank, 1: max(1, rank // 2)}, seed=rank)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(tokens + rank)
+    x, dy = torch.randn(tokens, cols, generator=g, device="cuda").to(BF16), torch.randn(tokens, rows, generator=g, device="cuda").to(BF16)
+    a, b = ad.a[0].to(BF16), ad.b[0].to(BF16)
+    if "x" in where:
+        x[2, 5] = float("inf")
+    if "dy" in where:
+        dy[4, 7] = -float("inf")
+    if where == "A":
+        a[rank // 2, 9] = float("inf")
+    if where == "B":
+        b[11, rank // 2] = -float("inf")
+    for t in (x, dy, a, b):     # (nothing is zero: an infinity times zero is NaN by the formulas too)
+        t[t == 0] = 1.0
+    ad.put(0, rank, ad.s[0], a, b, _capi.TYPE_BF16)
+    ids = torch.arange(tokens, device="cuda", dtype=torch.int32) // 8 % 3 - 1
+    ids[:8] = 0
+    base, dbase = torch.randn(tokens, rows, generator=g, device="cuda"), torch.randn(tokens, cols, generator=g, device="cuda")
+    y, dx = torch.empty(tokens, rows, device="cuda"), torch.empty(tokens, cols, device="cuda")
+    da, db = torch.empty(2, rank, cols, device="cuda"), torch.empty(2, rows, rank, device="cuda")
+    torch.cuda.synchronize()
+    ad.h.matmul_bf16(x.data_ptr(), tokens, cols, ids.data_ptr(), base.data_ptr(), rows, y.data_ptr(), rows)
+    ad.h.backward(x.data_ptr(), cols, dy.data_ptr(), rows, tokens, ids.data_ptr(), dbase.data_ptr(), cols, dx.data_ptr(), cols, da.data_ptr(), db.data_ptr())
+    ctx.sync()
+    # (sums written out: a matrix product of the library may skip or rearrange what is special)
+    want, wantx = base.double().clone(), dbase.double().clone()
+    for e, at in ad.of(ids):
+        A, B, s, xe, de = ad.a[e], ad.b[e], ad.s[e], x[at].double(), dy[at].double()
+        u, v = s * (xe[:, None] * A[None]).sum(2), s * (de[:, :, None] * B[None]).sum(1)
+        want[at] += (u[:, None] * B[None]).sum(2)
+        wantx[at] += (v[:, :, None] * A[None]).sum(1)
+        r = A.shape[0]
+        assert same_specials(da[e, :r], (v[:, :, None] * xe[:, None]).sum(0))
+        assert same_specials(db[e, :, :r], (de[:, :, None] * u[:, None]).sum(0))
+    assert same_specials(y, want) and same_specials(dx, wantx)
+    xf, yr = x[:8].float(), torch.empty(8, rows, device="cuda")
+    torch.cuda.synchronize()
+    ad.h.matvec(xf.data_ptr(), 8, cols, ids.data_ptr(), base.data_ptr(), rows, yr.data_ptr(), rows)
+    ctx.sync()
+    assert same_specials(yr, want[:8])
+
+
+@pytest.mark.parametrize("tokens", [40, 300])
+def test_values_at_the_ends_of_float32(ctx, adapters, tokens):  # noqa: F811
+    """Narrow products next to the largest float32, and far below the smallest bf16 part, keep their bits."""
+    rows, cols = 40, 32
+    ad = adapters(rows, cols, 1, 1, tokens, {0: 1})
+    a, b = torch.zeros(1, cols, device="cuda").to(BF16), torch.full((rows, 1), 2.0 ** -100, device="cuda").to(BF16)
+    a[0, :2] = torch.tensor([1.0, 2.0 ** -8], device="cuda").to(BF16)
+    ad.put(0, 1, 1.0, a, b, _capi.TYPE_BF16)
+    x = torch.zeros(tokens, cols, device="cuda").to(BF16)
+    x[:, 0] = x[:, 1] = 3.3895313892515355e38       # the largest bf16; the sum rounds to nothing finite there
+    x[1::2, :2] = 2.0 ** -100 * 1.0078125
+    y = torch.empty(tokens, rows, device="cuda")
+    torch.cuda.synchronize()
+    b2 = torch.full((rows, 1), 2.0 ** 90, device="cuda").to(BF16)
+    for bb in (b, b2):
+        ad.put(0, 1, 1.0, a, bb, _capi.TYPE_BF16)
+        torch.cuda.synchronize()
+        ad.h.matmul_bf16(x.data_ptr(), tokens, cols, 0, 0, 0, y.data_ptr(), rows)
+        ctx.sync()
+        want, _ = ad.forward(x.double(), torch.zeros(tokens, dtype=torch.int32, device="cuda"), torch.zeros(tokens, rows, device="cuda"))
+        at = slice(0, None, 2) if bb is b else slice(1, None, 2)     # (the others leave float32's range)
+        # two products, their sum, three parts: a unit each
+        assert ((y[at].double() - want[at]).abs() <= 2 * 6 * U32 * want[at].abs()).all()
