@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import lib_b200
-from lib_b200 import _capi
+from lib_b200 import _capi, synth
 from tests import capture
 from tests.test_gpu_lora import BF16, U32, adapters  # noqa: F401  (a fixture)
 
@@ -126,6 +126,27 @@ def test_pitch_of_an_absent_base(ctx, adapters, tokens):  # noqa: F811
     ctx.sync()
 
 
+@pytest.mark.parametrize("m", [128, 129, 391])
+def test_batched_product_with_adapters(ctx, adapters, m):  # noqa: F811
+    """qm_matmul_bf16_lora in the forms for few tokens and for prompts: the product's own result, the adapters on it."""
+    rows, cols = 520, 1024
+    w = ctx.store_upload(_capi.Q4_K, rows, cols, synth.weights(_capi.Q4_K, rows, cols, seed=3))
+    ad = adapters(rows, cols, 3, 24, m, {0: 24, 2: 7})
+    x = torch.tensor(synth.activations(m, cols, seed=4), device="cuda").to(BF16)
+    ids = torch.tensor([0, -1, 2, 1], dtype=torch.int32, device="cuda")[torch.arange(m, device="cuda") * 4 // m]
+    c, c2 = torch.full((m + 1, rows + 4), -7.0, device="cuda"), torch.empty(m, rows, device="cuda")
+    torch.cuda.synchronize()
+    ctx.matmul_bf16(w, x.data_ptr(), m, cols, c2.data_ptr(), rows)
+    ctx.matmul_bf16_lora(w, ad.h, x.data_ptr(), m, cols, ids.data_ptr(), c.data_ptr(), rows + 4)
+    ctx.sync()
+    want, mag = ad.forward(x.double(), ids, c2)
+    # as in the batches beside a base
+    assert ((c[:m, :rows].double() - want).abs() <= 2 * (4 + cols // 64 + 8 + 3 * 2 + 4) * U32 * mag).all()
+    bare = (ids != 0) & (ids != 2)
+    assert torch.equal(c[:m, :rows][bare], c2[bare]) and (c[:m, rows:] == -7.0).all() and (c[m] == -7.0).all()
+    w.free()
+
+
 @pytest.mark.parametrize("tokens", [40, 300])
 @pytest.mark.parametrize("rank", [1, 5, 24, 40, 70])
 @pytest.mark.parametrize("where", ["x", "dy", "A", "B", "x and dy"])
@@ -198,3 +219,40 @@ def test_values_at_the_ends_of_float32(ctx, adapters, tokens):  # noqa: F811
         at = slice(0, None, 2) if bb is b else slice(1, None, 2)     # (the others leave float32's range)
         # two products, their sum, three parts: a unit each
         assert ((y[at].double() - want[at]).abs() <= 2 * 6 * U32 * want[at].abs()).all()
+
+
+def test_small_calls_of_one_handle_overlap(ctx, adapters):  # noqa: F811
+    """Rows and few tokens use no workspace: calls on one handle may run at once, captured ones among them."""
+    rows, cols, tokens = 4100, 2048, 100
+    ad = adapters(rows, cols, 3, 32, tokens, {0: 32, 2: 9})
+    ids = torch.tensor([0, -1, 2], dtype=torch.int32, device="cuda")[torch.arange(tokens, device="cuda") % 3]
+    x = [torch.randn(tokens, cols, device="cuda").to(BF16) for _ in range(3)]
+    xf = [t[:8].float() for t in x]
+    y = [torch.empty(tokens, rows, device="cuda") for _ in x]
+    yr = [torch.empty(8, rows, device="cuda") for _ in x]
+    streams, graph = [torch.cuda.Stream() for _ in x], torch.cuda.CUDAGraph()
+
+    def both(i):
+        ad.h.matmul_bf16(x[i].data_ptr(), tokens, cols, ids.data_ptr(), 0, 0, y[i].data_ptr(), rows)
+        ad.h.matvec(xf[i].data_ptr(), 8, cols, ids.data_ptr(), 0, 0, yr[i].data_ptr(), rows)
+
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.graph(graph, stream=streams[2]):
+            ctx.set_stream(streams[2].cuda_stream)
+            both(2)
+        for _ in range(10):
+            with torch.cuda.stream(streams[2]):
+                graph.replay()
+            for i in range(2):
+                ctx.set_stream(streams[i].cuda_stream)
+                both(i)
+        torch.cuda.synchronize()
+    finally:
+        ctx.set_stream(0)
+    for i in range(3):
+        for got, inp in ((y[i], x[i]), (yr[i], xf[i])):
+            n = inp.shape[0]
+            want, mag = ad.forward(inp.double(), ids[:n], torch.zeros(n, rows, device="cuda"))
+            assert ((got.double() - want).abs() <= 2 * (4 + cols // 64 + 8 + 3 * 2 + 4) * U32 * mag + 1e-30).all()
+    del graph
