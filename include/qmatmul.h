@@ -206,6 +206,9 @@ QM_API int32_t qm_matmul_bf16(qm_ctx *ctx, qm_weight w, uint64_t a_dev, int32_t 
  * waits for the stream, so that the handle is ready for any other, and is refused under capture
  * (CUDA_ERROR_STREAM_CAPTURE_UNSUPPORTED).
  *
+ * Infinite elements give the infinities and NaN of the formulas (beside narrow products A x, B^T dy of at least 2^-80), and
+ * what a token holds reaches no other token's row.
+ *
  * qm_lora_set: fills a slot from device memory, A [rank][cols] and B [rows][rank] row by row, `type` a GGUF tensor type
  *   (QM_TYPE_F32, QM_TYPE_F16, QM_TYPE_BF16; rounded to bf16). rank 0 empties the slot. Ordered with the products on the
  *   stream, so a training step may set its adapters anew; the two arrays are free again once the stream is past the call.
@@ -248,7 +251,7 @@ QM_API int32_t qm_matmul_bf16_lora(qm_ctx *ctx, qm_weight w, qm_lora *lora, uint
  * and its first rot_dim elements are turned pairwise by the token's position (the other elements stay). No counterpart in
  * the reference.
  * qm_rope_create: angle_i = position * theta^(-2i/rot_dim) / factors[i] (factors: rot_dim/2 positive floats on the host, or
- *   NULL: ones), taken modulo a turn in float64, so far positions keep their fraction. Pairs are (i, i + rot_dim/2), with
+ *   NULL: ones), taken modulo a turn in 64 bits, so far positions keep their fraction. Pairs are (i, i + rot_dim/2), with
  *   QM_ROPE_INTERLEAVED (2i, 2i+1). head_dim even, <= 512; rot_dim even, 0..head_dim. Waits for the stream, so that the
  *   handle is ready for any other; refused under capture (CUDA_ERROR_STREAM_CAPTURE_UNSUPPORTED).
  * qm_qk_norm_rope: x float32 [tokens][ldx], q_heads query heads, then k_heads key heads, side by side (either may be 0; a v
@@ -260,7 +263,7 @@ QM_API int32_t qm_matmul_bf16_lora(qm_ctx *ctx, qm_weight w, qm_lora *lora, uint
  *   forward call. dx float32 [tokens][lddx] (the q and k parts; may lie on x, or on float32 dq and dk, place for place),
  *   dq_gain, dk_gain float32 [head_dim] or 0: summed over tokens and heads in a fixed order. Calls with gain gradients, and
  *   graphs of them, that share a handle must be ordered.
- * Asynchronous on the context's stream; up to 2^30 tokens, none among them. */
+ * Heads may be of any magnitude whose squares fit float32. Asynchronous on the context's stream; 0 to 2^30 tokens. */
 #define QM_ROPE_INTERLEAVED 1u
 #define QM_QK_NO_NORM 1u
 #define QM_QK_BF16 2u

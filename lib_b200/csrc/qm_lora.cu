@@ -15,12 +15,12 @@
 // beyond, and in the backward pass, qm_lora_lists orders the tokens by adapter and shrink, expand and outer are launches of
 // their own. Measured on one B200, calls back to back, floor = what has to move at the measured copy rate of 6.54 TB/s:
 //   1 row, 4096 x 4096, rank 16                       5.5 us   floor 0.05 (launch, five dependent trips to memory)
-//   8 rows, 8 adapters, 6144 x 4096, rank 64          9.0 us   floor 1.4  (the same, 144 KB of A and B per CTA)
+//   8 rows, 8 adapters, 6144 x 4096, rank 64          9.0 us   floor 1.4  (the same, 160 KiB of A and B per CTA)
 //   64 tokens, 32 adapters, 6144 x 4096, rank 16      9.3 us   floor 1.9
 //   391 tokens, 28672 x 4096, rank 32                  35 us   floor 15   (expand: base in, y out)
 //   2048 tokens, 4096 x 14336, rank 64                 48 us   floor 22
-//   backward, 777 tokens, 6144 x 4096, rank 8          44 us   floor 6.5  (seven short launches)
-//   backward, 4096 tokens, 28672 x 4096, rank 32      151 us   floor 63   (dy is read twice: 235 MB more)
+//   backward, 777 tokens, 6144 x 4096, rank 8          44 us   floor 6.5  (six short launches)
+//   backward, 4096 tokens, 28672 x 4096, rank 32      150 us   floor 63   (dy is read twice: 235 MB more)
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -1118,7 +1118,7 @@ __device__ __forceinline__ void shrink(const QmLoraTcArgs &ta) {
 // Legacy mma on purpose: the same step by tcgen05 (operands by TMA, results through tensor memory and shared memory, 128
 // columns per CTA) took 22.5 us instead of 20.5 at 2048 tokens x 4096, rank 64, and 34 instead of 22 at 391 x 28672, rank 32,
 // because every CTA then waits for tensor memory and two barriers more; leaving the products out altogether saves 1 us.
-// Copying base to y by the same steps takes 13.6 and 18 us.
+// Copying base to y by the same steps takes 13.6 and 18 us (10.3 and 13.8 at the measured copy rate).
 // MANY: fewer CTAs than there may be halves of tiles, each takes one after another.
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
